@@ -50,6 +50,11 @@ def default_ref_root() -> Path:
     return Path(env) if env else HERE.parent.parent / "reference"
 
 
+def _have_ref(ref_root: Path) -> bool:
+    """The tree is there with its sources (an empty directory of that name counts as absent)."""
+    return (ref_root / "h3_dit_w4a8.c").is_file()
+
+
 def _run(cmd: list[str]) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
@@ -79,7 +84,7 @@ def build_ref(ref_root: Path, force: bool = False) -> Path | None:
     """Returns the path of libh3_ref.so, or None when the reference tree is absent
     and no prebuilt copy exists."""
     out = REF_OUT / "libh3_ref.so"
-    if not ref_root.is_dir():
+    if not _have_ref(ref_root):
         return out if out.exists() else None
     if out.exists() and not force:
         return out
@@ -124,7 +129,7 @@ def build_ref_cuda(ref_root: Path, force: bool = False) -> Path | None:
     process of its own.  Returns None when the reference tree is absent and nothing was built before."""
     out_dir = REF_OUT / "cuda"
     out = out_dir / "libh3_refcuda.so"
-    if not ref_root.is_dir():
+    if not _have_ref(ref_root):
         return out if out.exists() else None
     if out.exists() and not force:
         return out
@@ -177,7 +182,7 @@ def build_ref_host(ref_root: Path, product_lib: Path, force: bool = False) -> Pa
     out = REF_OUT / "libh3_refhost.so"
     objs = [REF_OUT / f"{name}.o" for name in REF_HOST_OBJECTS]
     if not all(o.exists() for o in objs):
-        if not ref_root.is_dir() or build_ref(ref_root, force) is None:
+        if not _have_ref(ref_root) or build_ref(ref_root, force) is None:
             return out if out.exists() else None
     if not all(o.exists() for o in objs):
         return None
