@@ -1,0 +1,120 @@
+// Attention with a sliding window and first keys that stay visible, over 16-bit keys and values of one sequence or over
+// the paged 8-bit cache of many.
+#include "h3b_attn_win.cuh"
+
+namespace h3b {
+
+template <typename T, bool KV8> __global__ void __launch_bounds__(128) k_attn_rows_plain(const __grid_constant__ WinArgs a) {
+    const int s = blockIdx.z, row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
+    const SeqExt e = seq_ext<KV8>(a, s);
+    if (row >= e.nq || head >= a.heads) return;
+    attn_row_by_warp<T, KV8>(a, s, e, row, head, threadIdx.x & 31);
+}
+
+static int clip(int64_t v) { return v < 0 || v > H3B_WIN_MAX ? H3B_WIN_MAX : (int)v; }
+
+// checks and fields common to both entry points
+static int fill(WinArgs &a, h3_cuda *cuda, const char *who, int dtype, const void *q, size_t q_rs, size_t q_hs, size_t rows,
+                size_t heads, size_t kv_heads, size_t head_dim, float scale, int64_t left, int64_t right, int64_t sinks,
+                int64_t block, void *out, size_t o_rs, size_t o_hs, char *error, size_t error_size) {
+    if (!cuda) return fail(error, error_size, "%s: NULL handle", who);
+    if (dtype != H3B_BF16 && dtype != H3B_F16) return fail(error, error_size, "%s: dtype must be bf16 or f16", who);
+    if (head_dim != 128) return fail(error, error_size, "%s: head_dim %zu unsupported (128 only)", who, head_dim);
+    if (!heads || !kv_heads || heads % kv_heads || heads > 65535)
+        return fail(error, error_size, "%s: %zu heads over %zu K/V heads", who, heads, kv_heads);
+    if (heads / kv_heads > 128) return fail(error, error_size, "%s: more than 128 heads share a K/V head", who);
+    if (sinks < 0) return fail(error, error_size, "%s: sinks must not be negative", who);
+    if (block < 1) return fail(error, error_size, "%s: block must be at least 1", who);
+    if (!(scale > 0.0f) || !(scale < INFINITY)) return fail(error, error_size, "%s: scale must be positive and finite", who);
+    if (rows >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "%s: shape too large", who);
+    if (rows && (!q || !out)) return fail(error, error_size, "%s: NULL tensor", who);
+    if ((q_rs | q_hs | o_rs | o_hs) % 8 || ((uintptr_t)q & 15) || ((uintptr_t)out & 15))
+        return fail(error, error_size, "%s: pointers must be 16-byte aligned and strides multiples of 8 elements", who);
+    if (!q_rs || !q_hs || !o_rs || !o_hs) return fail(error, error_size, "%s: row and head strides must be given", who);
+    if ((q_rs | q_hs | o_rs | o_hs) >> 39) return fail(error, error_size, "%s: stride too large", who);
+    memset(&a, 0, sizeof(a));
+    a.q = q; a.out = out;
+    a.q_rs = (long long)q_rs; a.q_hs = (long long)q_hs; a.o_rs = (long long)o_rs; a.o_hs = (long long)o_hs;
+    a.rows = (int)rows; a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.group = (int)(heads / kv_heads);
+    a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
+    a.win.left = clip(left); a.win.right = clip(right); a.win.sinks = clip(sinks); a.win.block = clip(block);
+    a.status = cuda->d_status;
+    return 1;
+}
+
+template <bool KV8> static int launch(h3_cuda *cuda, const WinArgs &a, int f16, char *error, size_t error_size) {
+    DeviceGuard guard(cuda);
+    ProfScope prof(cuda, PROF_ATTN);
+    const dim3 grid((unsigned)a.max_rows, (unsigned)ceil_div(a.heads, 4), (unsigned)a.n_seq);
+    if (f16) k_attn_rows_plain<__half, KV8><<<grid, 128, 0, cuda->op_stream>>>(a);
+    else k_attn_rows_plain<__nv_bfloat16, KV8><<<grid, 128, 0, cuda->op_stream>>>(a);
+    cuda->launches++;
+    H3B_CUDA_OK(cudaGetLastError(), "windowed attention launch");
+    return 1;
+}
+
+}  // namespace h3b
+
+using namespace h3b;
+
+extern "C" {
+
+int h3b_window_tiles(size_t keys, int64_t pos0, size_t rows, int64_t left, int64_t right, int64_t sinks, int64_t block,
+                     int unit, int *sink_tiles, int *from, int *count) {
+    if (!rows || unit < 1 || block < 1 || sinks < 0 || pos0 < 0 || keys >= (size_t)H3B_WIN_MAX || rows >= (size_t)H3B_WIN_MAX ||
+        pos0 + (int64_t)rows > H3B_WIN_MAX || !sink_tiles || !from || !count)
+        return 0;
+    const h3b_win w = {clip(left), clip(right), clip(sinks), clip(block)};
+    const h3b_win_tiles t = h3b_win_tiles_of(w, (int)pos0, (int)(pos0 + (int64_t)rows - 1), (int)keys, unit);
+    *sink_tiles = t.sink;
+    *from = t.from;
+    *count = t.count;
+    return 1;
+}
+
+int h3b_sdpa_window_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row_stride, size_t q_head_stride, const void *d_k,
+                        size_t k_row_stride, size_t k_head_stride, const void *d_v, size_t v_row_stride, size_t v_head_stride,
+                        size_t lq, size_t lk, size_t heads, size_t kv_heads, size_t head_dim, float scale, int64_t q_pos,
+                        int64_t left, int64_t right, int64_t sinks, int64_t block, void *d_out, size_t o_row_stride,
+                        size_t o_head_stride, char *error, size_t error_size) {
+    WinArgs a;
+    if (!fill(a, cuda, "sdpa_window", dtype, d_q, q_row_stride, q_head_stride, lq, heads, kv_heads, head_dim, scale, left, right,
+              sinks, block, d_out, o_row_stride, o_head_stride, error, error_size))
+        return 0;
+    if (lk >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "sdpa_window: shape too large");
+    if (q_pos < 0 || q_pos + (int64_t)lq > H3B_WIN_MAX) return fail(error, error_size, "sdpa_window: q_pos out of range");
+    if (lk && (!d_k || !d_v)) return fail(error, error_size, "sdpa_window: NULL tensor");
+    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) % 8 || ((uintptr_t)d_k & 15) || ((uintptr_t)d_v & 15))
+        return fail(error, error_size, "sdpa_window: pointers must be 16-byte aligned and strides multiples of 8 elements");
+    if (!k_row_stride || !k_head_stride || !v_row_stride || !v_head_stride)
+        return fail(error, error_size, "sdpa_window: row and head strides must be given");
+    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) >> 39) return fail(error, error_size, "sdpa_window: stride too large");
+    if (!lq) return 1;
+    a.k = d_k; a.v = d_v;
+    a.k_rs = (long long)k_row_stride; a.k_hs = (long long)k_head_stride;
+    a.v_rs = (long long)v_row_stride; a.v_hs = (long long)v_head_stride;
+    a.lk = (int)lk; a.q_pos = (int)q_pos; a.max_rows = (int)lq; a.n_seq = 1;
+    return launch<false>(cuda, a, dtype == H3B_F16, error, error_size);
+}
+
+int h3b_kv8_sdpa_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const void *d_q, size_t q_row_stride,
+                     size_t q_head_stride, size_t rows, const int32_t *d_cu_rows, const int32_t *d_len, const int32_t *d_table,
+                     size_t table_stride, size_t n_seq, size_t max_rows, size_t max_len, size_t heads, float scale, int64_t left,
+                     int64_t right, int64_t sinks, int64_t block, void *d_out, size_t o_row_stride, size_t o_head_stride,
+                     char *error, size_t error_size) {
+    WinArgs a;
+    if (!kv8_cache_ok(cache, "kv8_sdpa", error, error_size)) return 0;
+    if (!fill(a, cuda, "kv8_sdpa", dtype, d_q, q_row_stride, q_head_stride, rows, heads, cache->kv_heads, cache->head_dim, scale,
+              left, right, sinks, block, d_out, o_row_stride, o_head_stride, error, error_size))
+        return 0;
+    if (!kv8_batch_ok(cache, "kv8_sdpa", rows, d_cu_rows, d_len, d_table, table_stride, n_seq, max_rows, error, error_size)) return 0;
+    if (max_len >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "kv8_sdpa: max_len out of range");
+    if (!rows || !n_seq || !max_rows) return 1;
+    a.kc = cache->d_k; a.vc = cache->d_v; a.ks = cache->d_k_scale; a.vs = cache->d_v_scale;
+    a.cu = d_cu_rows; a.len = d_len; a.table = d_table; a.table_stride = (long long)table_stride;
+    a.pages = (int)cache->pages; a.page_blocks = (int)(cache->page_tokens / KV8_BLOCK);
+    a.max_rows = (int)max_rows; a.n_seq = (int)n_seq;
+    return launch<true>(cuda, a, dtype == H3B_F16, error, error_size);
+}
+
+}  // extern "C"

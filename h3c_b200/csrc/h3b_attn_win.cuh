@@ -1,0 +1,160 @@
+// What the windowed attention kernels share: the call's arguments on the device, the extents of one sequence, and the
+// attention of one row by one warp straight from the definition.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "h3b_attn.cuh"
+#include "h3b_internal.h"
+#include "h3b_ptx.cuh"
+#include "h3b_window.h"
+
+namespace h3b {
+
+constexpr int KV8_BLOCK = 64;   // tokens that share a scale
+
+// One call.  16-bit keys and values: one sequence, cu / len / table are NULL.  8-bit: a paged cache.
+struct WinArgs {
+    const void *q;
+    void *out;
+    long long q_rs, q_hs, o_rs, o_hs;        // elements between rows / heads
+    int rows, heads, kv_heads, group;        // rows of q and out; group = heads / kv_heads
+    float scale;                             // of the scores
+    float scale_log2;                        // scale * log2(e)
+    h3b_win win;
+    int *status;
+    // 16-bit K/V
+    const void *k, *v;
+    long long k_rs, k_hs, v_rs, v_hs;
+    int lk, q_pos;
+    // 8-bit cache
+    const uint8_t *kc, *vc;                  // [pages][kv_heads][page_tokens][128]
+    const float *ks, *vs;                    // [pages][kv_heads][page_tokens / 64]
+    const int *cu, *len, *table;
+    long long table_stride;
+    int pages, page_blocks;                  // pages of the pool, 64-token blocks of a page
+    int max_rows, n_seq;
+};
+
+struct SeqExt {
+    int row0, nq, n, pos0;                   // first row of q, rows, keys, position of the first row
+};
+
+// Extents of sequence s; one that does not fit the call's arrays is skipped (nq = 0) and reported.
+template <bool KV8> __device__ __forceinline__ SeqExt seq_ext(const WinArgs &a, int s) {
+    SeqExt e;
+    if (!KV8) {
+        e.row0 = 0;
+        e.nq = a.rows;
+        e.n = a.lk;
+        e.pos0 = a.q_pos;
+        return e;
+    }
+    const int r0 = a.cu[s], r1 = a.cu[s + 1];
+    e.row0 = r0;
+    e.nq = r1 - r0;
+    e.n = a.len[s];
+    e.pos0 = e.n - e.nq;
+    if (r0 < 0 || r1 < r0 || r1 > a.rows || e.nq > a.max_rows || e.n < 0 ||
+        (long long)e.n > a.table_stride * a.page_blocks * KV8_BLOCK) {
+        if (a.status) atomicCAS(a.status, 0, H3B_ST_EXTENT);
+        e.nq = e.n = e.pos0 = 0;
+    }
+    return e;
+}
+
+// 64-token block `blk` of sequence s, as an index of (page, head, block of the page); -1 for a page outside the pool
+// (reported; the caller treats its tokens as masked).
+__device__ __forceinline__ long long kv8_block_index(const WinArgs &a, int s, int blk, int kvh) {
+    const int pg = blk / a.page_blocks, page = a.table[s * a.table_stride + pg];
+    if (page < 0 || page >= a.pages) {
+        if (a.status) atomicCAS(a.status, 0, H3B_ST_EXTENT);
+        return -1;
+    }
+    return ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
+}
+
+template <typename T> __device__ __forceinline__ float4 load4(const T *p) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    float4 r;
+    if (sizeof(T) == 2 && Elem<T>::FMT == 1) {
+        r.x = __uint_as_float(w.x << 16); r.y = __uint_as_float(w.x & 0xffff0000u);
+        r.z = __uint_as_float(w.y << 16); r.w = __uint_as_float(w.y & 0xffff0000u);
+    } else {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+        r = make_float4(a.x, a.y, b.x, b.y);
+    }
+    return r;
+}
+__device__ __forceinline__ float4 codes4(uint32_t w) {
+    const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&lo));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// One row and head by one warp, from the definition: lane l holds dimensions 4l..4l+3; a key costs one warp-wide sum.
+// Only visible keys are touched, so whatever masked places hold has no part in the result.
+template <typename T, bool KV8>
+__device__ __noinline__ void attn_row_by_warp(const WinArgs &a, int s, const SeqExt e, int row, int head, int lane) {
+    const int kvh = head / a.group;
+    const h3b_win_row r = h3b_win_of(a.win, e.pos0 + row, e.n);
+    const float4 q = load4(reinterpret_cast<const T *>(a.q) + (long long)(e.row0 + row) * a.q_rs + head * a.q_hs + lane * 4);
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int count = h3b_win_count(r), gap = max(r.lo - r.s, 0);
+    int blk_have = -1;
+    long long bi = -1;
+    float ks = 1.0f, vs = 1.0f;
+    for (int i = 0; i < count; i++) {
+        const int j = i < r.s ? i : i + gap;
+        float4 k, v;
+        if (KV8) {
+            const int blk = j / KV8_BLOCK;
+            if (blk != blk_have) {
+                blk_have = blk;
+                bi = kv8_block_index(a, s, blk, kvh);
+                if (bi >= 0) {
+                    ks = a.ks[bi];
+                    vs = a.vs[bi];
+                }
+            }
+            if (bi < 0) continue;
+            const long long off = (bi * KV8_BLOCK + (j - blk * KV8_BLOCK)) * 128 + lane * 4;
+            k = codes4(*reinterpret_cast<const uint32_t *>(a.kc + off));
+            v = codes4(*reinterpret_cast<const uint32_t *>(a.vc + off));
+        } else {
+            k = load4(reinterpret_cast<const T *>(a.k) + (long long)j * a.k_rs + kvh * a.k_hs + lane * 4);
+            v = load4(reinterpret_cast<const T *>(a.v) + (long long)j * a.v_rs + kvh * a.v_hs + lane * 4);
+        }
+        float d = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+#pragma unroll
+        for (int w = 16; w; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+        if (KV8) d *= ks;
+        const float x = d * a.scale_log2;
+        if (x != x || x == INFINITY) {   // undefined: so is the row
+            l = __int_as_float(0x7fffffff);
+            break;
+        }
+        if (x > m) {
+            const float f = m == -INFINITY ? 0.0f : exp2f(m - x);
+            l *= f;
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+            m = x;
+        }
+        const float p = x == -INFINITY ? 0.0f : exp2f(x - m);
+        l += p;
+        const float pv = KV8 ? p * vs : p;
+        o.x += pv * v.x; o.y += pv * v.y; o.z += pv * v.z; o.w += pv * v.w;
+    }
+    const float inv = count ? 1.0f / l : 0.0f;
+    uint2 w;
+    w.x = Elem<T>::pack(o.x * inv, o.y * inv);
+    w.y = Elem<T>::pack(o.z * inv, o.w * inv);
+    if (!count) w.x = w.y = 0u;
+    *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + (long long)(e.row0 + row) * a.o_rs + head * a.o_hs + lane * 4) = w;
+}
+
+}  // namespace h3b

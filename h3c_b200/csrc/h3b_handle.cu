@@ -349,6 +349,8 @@ int h3b_cuda_check(h3_cuda *cuda, int *status_out, char *error, size_t error_siz
         cudaMemset(cuda->d_status, 0, sizeof(int));
         // a GEMM that gave up may have left the counters of its split tail tiles mid-count: start them over
         if (cuda->splitk) cudaMemset(cuda->splitk, 0, cuda->splitk_bytes < 1024 ? cuda->splitk_bytes : 1024);
+        if (st == H3B_ST_EXTENT)
+            return fail(error, error_size, "a sequence's rows, length or page indices lie outside the call's arrays; its output is invalid");
         return fail(error, error_size, "a kernel gave up a bounded wait (status %d); its output is invalid", st);
     }
     return 1;

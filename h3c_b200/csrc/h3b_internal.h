@@ -84,6 +84,18 @@ struct ProfScope {
     ~ProfScope();
 };
 
+// The handle's device for the length of a call, whatever device the caller has current.
+struct DeviceGuard {
+    int before;
+    DeviceGuard(const h3_cuda *c) : before(-1) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != c->device && cudaSetDevice(c->device) == cudaSuccess) before = now;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
 static inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
 static inline size_t dtype_bytes(int dt) { return dt == H3B_F32 || dt == H3B_I32 ? 4 : 2; }
 
@@ -121,5 +133,10 @@ int launch_sdpa_bf16(h3_cuda *cuda, const void *q, size_t qs, const void *k, siz
 int launch_sdpa_f16(h3_cuda *cuda, const void *q, size_t qs, const void *k, size_t ks, const void *v, size_t vs,
                     size_t lq, size_t lk, size_t heads, size_t hd, float scale, void *out, size_t os,
                     char *error, size_t error_size);
+
+// checks of the 8-bit key/value cache and of the sequence tables that its two operators share
+int kv8_cache_ok(const h3b_kv8_cache *c, const char *who, char *error, size_t error_size);
+int kv8_batch_ok(const h3b_kv8_cache *c, const char *who, size_t rows, const int32_t *cu, const int32_t *ext, const int32_t *table,
+                 size_t table_stride, size_t n_seq, size_t max_rows, char *error, size_t error_size);
 
 }  // namespace h3b

@@ -1,0 +1,215 @@
+// Paged key/value cache held in E4M3: codes [pages][kv_heads][page_tokens][128], one f32 scale per 64 tokens of a head
+// [pages][kv_heads][page_tokens / 64]; value = code * scale.
+//
+// The scale of a block of 64 tokens x 128 is a power of two: 2^e with the smallest e >= -64 for which the largest
+// magnitude is at most 448 * 2^e (448 = the largest E4M3 number).  E4M3 has the same relative precision over 15
+// binades, so a power of two costs nothing against absmax / 448, and it makes two things exact: dividing by the scale,
+// and raising it later.  Tokens join a half-filled block one by one while a text is decoded; each time the block's
+// largest magnitude crosses a power of two, the codes that are there are moved to the new scale, which is exact but for
+// codes that become subnormal.  With absmax / 448 every such step would round all of them again.
+// A block into which a non-finite value is written gets a NaN scale and zero codes: attention over it gives NaN for
+// the rows that see it and nothing else, like the value itself would.
+//
+// h3b_kv8_append_dev: one CTA per (64-token block of the sequence that receives rows, K/V head); 16 lanes hold a row of
+// 128, every thread keeps its four 16-byte pieces of K and of V in registers between the maximum and the conversion:
+// one read, one write, no second pass.
+#include "h3b_attn_win.cuh"
+
+namespace h3b {
+
+int kv8_cache_ok(const h3b_kv8_cache *c, const char *who, char *error, size_t error_size) {
+    if (!c) return fail(error, error_size, "%s: NULL cache", who);
+    if (c->head_dim != 128) return fail(error, error_size, "%s: head_dim %zu unsupported (128 only)", who, c->head_dim);
+    if (!c->page_tokens || c->page_tokens % KV8_BLOCK || c->page_tokens > 65536)
+        return fail(error, error_size, "%s: page_tokens %zu is not a multiple of %d up to 65536", who, c->page_tokens, KV8_BLOCK);
+    if (!c->kv_heads || c->kv_heads > 65535) return fail(error, error_size, "%s: %zu K/V heads", who, c->kv_heads);
+    if (!c->pages || c->pages >= 0x7fffffffu / c->kv_heads / c->page_tokens)
+        return fail(error, error_size, "%s: a pool of %zu pages is not supported (pages * kv_heads * page_tokens < 2^31)", who, c->pages);
+    if (!c->d_k || !c->d_v || !c->d_k_scale || !c->d_v_scale) return fail(error, error_size, "%s: NULL cache tensor", who);
+    if (((uintptr_t)c->d_k & 15) || ((uintptr_t)c->d_v & 15) || ((uintptr_t)c->d_k_scale & 3) || ((uintptr_t)c->d_v_scale & 3))
+        return fail(error, error_size, "%s: cache codes must be 16-byte aligned, scales 4-byte aligned", who);
+    return 1;
+}
+
+int kv8_batch_ok(const h3b_kv8_cache *c, const char *who, size_t rows, const int32_t *cu, const int32_t *ext, const int32_t *table,
+                 size_t table_stride, size_t n_seq, size_t max_rows, char *error, size_t error_size) {
+    if (n_seq > 65535) return fail(error, error_size, "%s: more than 65535 sequences", who);
+    if (n_seq && (!cu || !ext || !table)) return fail(error, error_size, "%s: NULL sequence table", who);
+    if (((uintptr_t)cu & 3) || ((uintptr_t)ext & 3) || ((uintptr_t)table & 3))
+        return fail(error, error_size, "%s: sequence tables must be 4-byte aligned", who);
+    if (n_seq && !table_stride) return fail(error, error_size, "%s: table_stride must be given", who);
+    if (table_stride >= (size_t)H3B_WIN_MAX / c->page_tokens) return fail(error, error_size, "%s: table_stride out of range", who);
+    if (max_rows > rows) return fail(error, error_size, "%s: max_rows %zu of %zu rows", who, max_rows, rows);
+    return 1;
+}
+
+struct AppendArgs {
+    const void *x[2];                        // K, V rows
+    long long rs[2], hs[2];
+    uint8_t *codes[2];
+    float *scales[2];
+    const int *cu, *start, *table;
+    long long table_stride;
+    int rows, max_rows, kv_heads, pages, page_blocks;
+    int *status;
+};
+
+// 2^e >= a / 448 with the smallest e >= -64; a > 0 finite.  448 = 1.75 * 2^8.
+__device__ __forceinline__ float kv8_scale(uint32_t abs_bits) {
+    const int x = (int)(abs_bits >> 23) - 127;   // subnormal magnitudes give -127: clamped below
+    const int e = max((abs_bits & 0x7fffffu) <= 0x600000u ? x - 8 : x - 7, -64);
+    return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+template <typename T> __device__ __forceinline__ uint32_t abs_max8(const uint4 &w) {
+    uint32_t m = 0;
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t t = v[i] & 0x7fff7fffu;
+        m = max(m, max(t & 0xffffu, t >> 16));
+    }
+    return m;   // 16-bit pattern: magnitudes order like integers, NaN above infinity
+}
+template <typename T> __device__ __forceinline__ uint32_t widen_abs(uint32_t h) {
+    if (Elem<T>::FMT == 1) return h << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+}
+
+template <typename T> __global__ void __launch_bounds__(256) k_kv8_append(const __grid_constant__ AppendArgs a) {
+    __shared__ uint32_t red[2][8];
+    const int s = blockIdx.z, kvh = blockIdx.y, tid = threadIdx.x;
+    const int r0 = a.cu[s], r1 = a.cu[s + 1], start = a.start[s], nr = r1 - r0;
+    if (r0 < 0 || r1 < r0 || r1 > a.rows || nr > a.max_rows || start < 0 ||
+        (long long)start + nr > a.table_stride * a.page_blocks * KV8_BLOCK) {
+        if (tid == 0 && a.status) atomicCAS(a.status, 0, H3B_ST_EXTENT);
+        return;
+    }
+    const int blk = start / KV8_BLOCK + blockIdx.x;              // 64-token block of the sequence
+    const int t0 = blk * KV8_BLOCK;                              // its first token
+    const int from = max(start - t0, 0), to = min(start + nr - t0, KV8_BLOCK);   // tokens [from, to) of it are new
+    if (from >= to) return;
+    const int pg = blk / a.page_blocks, page = a.table[s * a.table_stride + pg];
+    if (page < 0 || page >= a.pages) {
+        if (tid == 0 && a.status) atomicCAS(a.status, 0, H3B_ST_EXTENT);
+        return;
+    }
+    const long long bi = ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
+    const int sub = tid >> 4, c = tid & 15;                      // row of a pass, 16-byte piece of the row
+    uint4 raw[2][4];
+    uint32_t top[2] = {0u, 0u};
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = i * 16 + sub;
+            raw[w][i] = make_uint4(0u, 0u, 0u, 0u);
+            if (t >= from && t < to)
+                raw[w][i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x[w]) +
+                                                                  (long long)(r0 + t0 + t - start) * a.rs[w] + kvh * a.hs[w]) + c);
+        }
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) top[w] = max(top[w], abs_max8<T>(raw[w][i]));
+        top[w] = __reduce_max_sync(0xffffffffu, top[w]);
+        if ((tid & 31) == 0) red[w][tid >> 5] = top[w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) top[w] = max(top[w], red[w][i]);
+        const uint32_t bits = widen_abs<T>(top[w]);
+        const float before = from > 0 ? a.scales[w][bi] : 0.0f;  // tokens in front of the new ones keep it at least
+        float scale = bits >= 0x7f800000u ? __int_as_float(0x7fffffff) : kv8_scale(bits);
+        if (from > 0 && !(before <= scale)) scale = before != before ? before : (scale != scale ? scale : before);
+        __syncthreads();                                         // every thread has read the old scale
+        if (tid == 0) a.scales[w][bi] = scale;
+        const bool dead = scale != scale;
+        const float inv = dead ? 0.0f : 1.0f / scale;
+        uint8_t *dst = a.codes[w] + bi * (KV8_BLOCK * 128);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = i * 16 + sub;
+            if (t >= from && t < to) {
+                const uint32_t v[4] = {raw[w][i].x, raw[w][i].y, raw[w][i].z, raw[w][i].w};
+                uint32_t packed[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    uint32_t out = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t two = v[2 * j + h];
+                        float2 f;
+                        if (Elem<T>::FMT == 1) f = make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+                        else f = __half22float2(*reinterpret_cast<const __half2 *>(&two));
+                        f.x *= inv;
+                        f.y *= inv;
+                        out |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * h);
+                    }
+                    packed[j] = dead ? 0u : out;
+                }
+                *reinterpret_cast<uint2 *>(dst + t * 128 + c * 8) = make_uint2(packed[0], packed[1]);
+            } else if (t < from && scale != before) {            // codes that are there, under the raised scale
+                uint2 old = *reinterpret_cast<const uint2 *>(dst + t * 128 + c * 8);
+                const float f = before * inv;
+                uint32_t words[2] = {old.x, old.y};
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float4 x = codes4(words[j]);
+                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x.x * f, x.y * f), __NV_SATFINITE, __NV_E4M3);
+                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x.z * f, x.w * f), __NV_SATFINITE, __NV_E4M3);
+                    words[j] = dead ? 0u : lo | hi << 16;
+                }
+                *reinterpret_cast<uint2 *>(dst + t * 128 + c * 8) = make_uint2(words[0], words[1]);
+            }
+        }
+    }
+}
+
+}  // namespace h3b
+
+using namespace h3b;
+
+extern "C" {
+
+int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const void *d_k, size_t k_row_stride,
+                       size_t k_head_stride, const void *d_v, size_t v_row_stride, size_t v_head_stride, size_t rows,
+                       const int32_t *d_cu_rows, const int32_t *d_start, const int32_t *d_table, size_t table_stride, size_t n_seq,
+                       size_t max_rows, char *error, size_t error_size) {
+    if (!kv8_cache_ok(cache, "kv8_append", error, error_size)) return 0;
+    if (!cuda) return fail(error, error_size, "kv8_append: NULL handle");
+    if (dtype != H3B_BF16 && dtype != H3B_F16) return fail(error, error_size, "kv8_append: dtype must be bf16 or f16");
+    if (rows >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "kv8_append: shape too large");
+    if (rows && (!d_k || !d_v)) return fail(error, error_size, "kv8_append: NULL tensor");
+    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) % 8 || ((uintptr_t)d_k & 15) || ((uintptr_t)d_v & 15))
+        return fail(error, error_size, "kv8_append: pointers must be 16-byte aligned and strides multiples of 8 elements");
+    if (!k_row_stride || !k_head_stride || !v_row_stride || !v_head_stride)
+        return fail(error, error_size, "kv8_append: row and head strides must be given");
+    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) >> 39) return fail(error, error_size, "kv8_append: stride too large");
+    if (!kv8_batch_ok(cache, "kv8_append", rows, d_cu_rows, d_start, d_table, table_stride, n_seq, max_rows, error, error_size)) return 0;
+    if (!rows || !n_seq || !max_rows) return 1;
+    AppendArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x[0] = d_k; a.x[1] = d_v;
+    a.rs[0] = (long long)k_row_stride; a.rs[1] = (long long)v_row_stride;
+    a.hs[0] = (long long)k_head_stride; a.hs[1] = (long long)v_head_stride;
+    a.codes[0] = cache->d_k; a.codes[1] = cache->d_v;
+    a.scales[0] = cache->d_k_scale; a.scales[1] = cache->d_v_scale;
+    a.cu = d_cu_rows; a.start = d_start; a.table = d_table; a.table_stride = (long long)table_stride;
+    a.rows = (int)rows; a.max_rows = (int)max_rows; a.kv_heads = (int)cache->kv_heads; a.pages = (int)cache->pages;
+    a.page_blocks = (int)(cache->page_tokens / KV8_BLOCK);
+    a.status = cuda->d_status;
+    // max_rows rows that start anywhere in a block reach this many blocks
+    const dim3 grid((unsigned)ceil_div(max_rows + KV8_BLOCK - 1, KV8_BLOCK), (unsigned)cache->kv_heads, (unsigned)n_seq);
+    DeviceGuard guard(cuda);
+    ProfScope prof(cuda, PROF_OTHER);
+    if (dtype == H3B_F16) k_kv8_append<__half><<<grid, 256, 0, cuda->op_stream>>>(a);
+    else k_kv8_append<__nv_bfloat16><<<grid, 256, 0, cuda->op_stream>>>(a);
+    cuda->launches++;
+    H3B_CUDA_OK(cudaGetLastError(), "k_kv8_append launch");
+    return 1;
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ enum : int {
     H3B_ST_TIMEOUT_TMEM_FULL = 3,
     H3B_ST_TIMEOUT_TMEM_EMPTY = 4,
     H3B_ST_TIMEOUT_OTHER = 5,
+    H3B_ST_EXTENT = 6,         // not a wait: a sequence's rows, length or pages lie outside the call's arrays
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {

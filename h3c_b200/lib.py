@@ -19,6 +19,7 @@ ERR_LEN = 512
 vp = C.c_void_p
 sz = C.c_size_t
 i32 = C.c_int
+i64 = C.c_int64
 f32 = C.c_float
 cs = C.c_char_p
 dbl_p = C.POINTER(C.c_double)
@@ -60,6 +61,11 @@ class DitConfig(C.Structure):  # h3b_dit_config
     _fields_ = [("kind", i32), ("stream_dtype", i32), ("convrot_gs", i32), ("dim", sz), ("heads", sz),
                 ("head_dim", sz), ("ffn", sz), ("rope_half", sz), ("n_blocks", sz), ("mod_rows", sz), ("t_dim", sz),
                 ("eps", f32)]
+
+
+class Kv8Cache(C.Structure):  # h3b_kv8_cache
+    _fields_ = [("pages", sz), ("page_tokens", sz), ("kv_heads", sz), ("head_dim", sz), ("d_k", vp), ("d_v", vp),
+                ("d_k_scale", vp), ("d_v_scale", vp)]
 
 
 class UlyssesDirect(C.Structure):  # h3b_ulysses_direct
@@ -284,6 +290,12 @@ _SIGS = {
     "h3_nvfp4_cuda_encode_text_layers": (i32, (vp, vp, sz, C.c_uint) + _ERR),
     "h3_nvfp4_cuda_gqa_causal": (i32, (vp, vp, vp, sz, sz, sz, sz, vp) + _ERR),
     "h3b_sdpa_strided_dev": (i32, (vp, i32, vp, sz, sz, vp, sz, sz, vp, sz, sz, sz, sz, sz, sz, f32, vp, sz, sz) + _ERR),
+    "h3b_sdpa_window_dev": (i32, (vp, i32, vp, sz, sz, vp, sz, sz, vp, sz, sz, sz, sz, sz, sz, sz, f32, i64, i64, i64, i64, i64,
+                                  vp, sz, sz) + _ERR),
+    "h3b_window_tiles": (i32, (sz, i64, sz, i64, i64, i64, i64, i32, C.POINTER(i32), C.POINTER(i32), C.POINTER(i32))),
+    "h3b_kv8_append_dev": (i32, (vp, C.POINTER(Kv8Cache), i32, vp, sz, sz, vp, sz, sz, sz, vp, vp, vp, sz, sz, sz) + _ERR),
+    "h3b_kv8_sdpa_dev": (i32, (vp, C.POINTER(Kv8Cache), i32, vp, sz, sz, sz, vp, vp, vp, sz, sz, sz, sz, sz, f32, i64, i64, i64,
+                               i64, vp, sz, sz) + _ERR),
     "h3_dit_patchify_video": (i32, (vp, i32, i32, i32, i32, vp, sz)),
     "h3_dit_unpatchify_video": (i32, (vp, i32, i32, i32, i32, vp, sz)),
     "h3_dit_pack_audio": (i32, (vp, i32, i32, vp, sz)),
