@@ -42,9 +42,10 @@ static int fill(WinArgs &a, h3_cuda *cuda, const char *who, int dtype, const voi
     return 1;
 }
 
-template <bool KV8> static int launch(h3_cuda *cuda, const WinArgs &a, int f16, char *error, size_t error_size) {
+template <bool KV8> static int launch(h3_cuda *cuda, const WinArgs &a, int f16, size_t len, char *error, size_t error_size) {
     DeviceGuard guard(cuda);
     ProfScope prof(cuda, PROF_ATTN);
+    if ((size_t)a.max_rows * a.group <= 64) return launch_attn_few(cuda, a, f16, KV8, len, error, error_size);
     const dim3 grid((unsigned)a.max_rows, (unsigned)ceil_div(a.heads, 4), (unsigned)a.n_seq);
     if (f16) k_attn_rows_plain<__half, KV8><<<grid, 128, 0, cuda->op_stream>>>(a);
     else k_attn_rows_plain<__nv_bfloat16, KV8><<<grid, 128, 0, cuda->op_stream>>>(a);
@@ -94,7 +95,7 @@ int h3b_sdpa_window_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row_
     a.k_rs = (long long)k_row_stride; a.k_hs = (long long)k_head_stride;
     a.v_rs = (long long)v_row_stride; a.v_hs = (long long)v_head_stride;
     a.lk = (int)lk; a.q_pos = (int)q_pos; a.max_rows = (int)lq; a.n_seq = 1;
-    return launch<false>(cuda, a, dtype == H3B_F16, error, error_size);
+    return launch<false>(cuda, a, dtype == H3B_F16, lk, error, error_size);
 }
 
 int h3b_kv8_sdpa_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const void *d_q, size_t q_row_stride,
@@ -114,7 +115,7 @@ int h3b_kv8_sdpa_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const
     a.cu = d_cu_rows; a.len = d_len; a.table = d_table; a.table_stride = (long long)table_stride;
     a.pages = (int)cache->pages; a.page_blocks = (int)(cache->page_tokens / KV8_BLOCK);
     a.max_rows = (int)max_rows; a.n_seq = (int)n_seq;
-    return launch<true>(cuda, a, dtype == H3B_F16, error, error_size);
+    return launch<true>(cuda, a, dtype == H3B_F16, max_len, error, error_size);
 }
 
 }  // extern "C"

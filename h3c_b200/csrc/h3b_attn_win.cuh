@@ -157,4 +157,7 @@ __device__ __noinline__ void attn_row_by_warp(const WinArgs &a, int s, const Seq
     *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + (long long)(e.row0 + row) * a.o_rs + head * a.o_hs + lane * 4) = w;
 }
 
+// few query rows per K/V head: h3b_attn_few.cu.  len: keys of the longest sequence (an estimate guides the split)
+int launch_attn_few(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t len, char *error, size_t error_size);
+
 }  // namespace h3b
