@@ -1,39 +1,47 @@
 // Windowed attention for few query rows per K/V head (one token of a stream, a handful of drafted ones, shared heads):
 // the time is that of reading the keys and values once, so the whole chip has to read, and nothing else may wait.
 //
-// One warp holds up to 16 rows (query rows x heads of one K/V head; rows beyond them are zero) as the A operand of
-// m16n8k16 tensor-core products and walks over key tiles of its own: S = Q K^T from registers, online softmax in
-// registers, O += P V with P straight from the score fragments.  A warp-private ring of TMA copies feeds it (a warp
-// waits for nobody but its own copies).  Tiles are dealt out over the warps of a CTA and the CTAs of a cluster; the
-// partial results (m, l, O) meet in shared memory, first of the CTA, then across the cluster, so a split over the keys
-// needs neither a workspace nor a second launch.
+// One warp works on up to 8 NT rows (query rows x heads of one K/V head; rows beyond them are zero) with m16n8k16
+// tensor-core products whose 16 rows are KEYS, respectively dimensions: S^T = K Q^T and O^T += V^T P^T, so that nothing is
+// padded from 1 to 16 rows (8 is the least) and the widened keys and values are the operands that are used once.  Q stays
+// in registers, P goes from score fragments to operand fragments through one 8x8 transposition per 8 keys.  The running
+// maximum is looked at by a vote and followed only when it has grown by more than 2^8.  A warp has a stage of its own
+// for TMA copies: those of the next keys are under way while the values are used and the other way round, and a warp waits
+// for nobody but its own copies.  Tiles are dealt out over the warps of a CTA and the CTAs of a cluster; the partial
+// results (m, l, O) meet in shared memory, first of the CTA, then across the cluster, so a split over the keys needs
+// neither a workspace nor a second launch.
 //
 // tcgen05 does not pay here: its smallest product has 64 rows, and S and P would go through tensor memory for 1 to 16.
 //
 // 8-bit cache: codes are widened to f16 in registers (E4M3 fits f16 exactly), Q goes to f16 under a power of two of its
 // row's maximum (bf16 has more range than f16; what is 2^-38 below the row's largest element is lost), and neither K
-// nor V is multiplied by its scale: the key scale multiplies 64 score columns, and log2 of the value scale is added to
+// nor V is multiplied by its scale: the key scale multiplies 64 scores, and log2 of the value scale is added to
 // their exponent, so P carries it (2^(x + log2 vs - m)) and the row sum takes it out again per 64 keys.  The order of
 // the 128 products of a score and of the keys of a sum is free, so every lane takes the 16 bytes it reads as they lie:
 // fragments need no shuffles, and the 128-byte swizzle of the copies keeps the reads free of bank conflicts.
 #include <algorithm>
+#include <type_traits>
 
 #include "h3b_attn_win.cuh"
 
 namespace h3b {
 
 namespace few {
-constexpr int WARPS = 4, STAGES = 3, THREADS = WARPS * 32;
-constexpr int STAGE = 16384;                       // K half | V half
-constexpr int HALF = STAGE / 2;
-// shared memory: rings | partial results of the CTA (16 rows x 128 f32, m, l) | barriers
-constexpr size_t SMEM_BYTES = 1024 + (size_t)WARPS * STAGES * STAGE + 16 * 128 * 4 + 2 * 16 * 4 + WARPS * 16 * 8 + 256;
-constexpr int UNIT8 = 64, UNIT16 = 32;             // keys of a tile
+// WIDE: one CTA of twelve warps on an SM, for a handful of (sequence, K/V head) pairs, whose clusters then reach the most
+// SMs; else three CTAs of four warps, which fill the chip evenly and hide each other's beginnings and ends.
+template <bool KV8, bool WIDE> struct Cfg {
+    static constexpr int U = KV8 ? 64 : 32;         // keys of a tile: 8 KiB of keys, 8 KiB of values
+    static constexpr int WARPS = WIDE ? 12 : 4, CTAS = WIDE ? 1 : 3, THREADS = WARPS * 32;
+    static constexpr int HALF = U * 128 * (KV8 ? 1 : 2), STAGE = 2 * HALF;         // keys | values
+    static_assert(STAGE >= 16 * 128 * 4, "a warp parks its 16 x 128 sums in its stage at the end");
+    // stages of the warps | partial results of the CTA (16 rows x 128 f32, m, l) | m, l of the warps | barriers
+    static constexpr size_t SMEM_BYTES = 1024 + (size_t)WARPS * STAGE + 16 * 128 * 4 + 2 * 16 * 4 + WARPS * 16 * 8 + WARPS * 16 + 64;
+};
 }  // namespace few
 
 struct FewParams {
     WinArgs a;
-    CUtensorMap map_k, map_v;                      // 16-bit: {d, head, row} box {64, 1, 32}; 8-bit: {128, rows} box {128, 64}
+    CUtensorMap map_k, map_v;                      // 16-bit: {d, head, row} box {64, 1, U}; 8-bit: {128, rows} box {128, U}
     int split;                                     // CTAs of a cluster
 };
 
@@ -41,13 +49,13 @@ template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], ui
                                                                uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                              uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                                     uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -63,10 +71,15 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t &r0, uint32_t &r1
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
 }
-// two E4M3 codes (low 16 bits) -> two f16
-__device__ __forceinline__ uint32_t widen2(uint32_t w) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    return (uint32_t)h.x | (uint32_t)h.y << 16;
+// four E4M3 codes -> two pairs of f16 (exact)
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// transposes an 8x8 matrix of 16-bit values: lane (g, t) has row g, columns 2t, 2t + 1
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     float v;
@@ -78,24 +91,27 @@ template <typename T> __device__ __forceinline__ float to_f(uint32_t pair, int h
     return __half2float(__ushort_as_half((unsigned short)(hi ? pair >> 16 : pair & 0xffffu)));
 }
 
-// HALF_M: at most 8 rows, the other half of the fragments stays zero and is left out of the softmax
-template <typename T, bool KV8, bool HALF_M> __global__ void __launch_bounds__(few::THREADS) k_attn_few(const __grid_constant__ FewParams p) {
-    using namespace few;
-    constexpr int U = KV8 ? UNIT8 : UNIT16;
-    constexpr int NT = U / 8;                      // score tiles of 8 keys
+// NT: 8 NT rows
+template <typename T, bool KV8, int NT, bool WIDE> __global__ void __launch_bounds__(few::Cfg<KV8, WIDE>::THREADS, few::Cfg<KV8, WIDE>::CTAS)
+k_attn_few(const __grid_constant__ FewParams p) {
+    using C = few::Cfg<KV8, WIDE>;
+    using E = typename std::conditional<KV8, __half, T>::type;                     // operand type
+    constexpr int U = C::U, WARPS = C::WARPS, STAGE = C::STAGE, HALF = C::HALF;
+    constexpr int MT = U / 16;                                                     // score tiles of 16 keys
+    constexpr int ROWS = 8 * NT;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float *acc = reinterpret_cast<float *>(smem + WARPS * STAGES * STAGE);        // [16][128] of this CTA
+    float *acc = reinterpret_cast<float *>(smem + WARPS * STAGE);                  // [16][128] of this CTA
     float *acc_m = acc + 16 * 128, *acc_l = acc_m + 16;
     float *warp_ml = acc_l + 16;                                                   // [WARPS][16][2]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(warp_ml + WARPS * 16 * 2);
-    volatile int *abort_word = reinterpret_cast<volatile int *>(bars + WARPS * STAGES);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(warp_ml + WARPS * 16 * 2);       // [WARPS][keys | values]
+    volatile int *abort_word = reinterpret_cast<volatile int *>(bars + WARPS * 2);
 
     const WinArgs &a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = (int)blockIdx.x % p.split, mt = (int)blockIdx.x / p.split, kvh = blockIdx.y, s = blockIdx.z;
     const SeqExt e = seq_ext<KV8>(a, s);
-    const int r_first = mt * 16, r_end = min(r_first + 16, e.nq * a.group);        // rows = query * group + head of the group
+    const int r_first = mt * ROWS, r_end = min(r_first + ROWS, e.nq * a.group);    // rows = query * group + head of the group
     if (r_first >= r_end) return;                                                  // the whole cluster alike
     const int R = r_end - r_first;
     const int qi_first = r_first / a.group, qi_last = (r_end - 1) / a.group;
@@ -106,16 +122,17 @@ template <typename T, bool KV8, bool HALF_M> __global__ void __launch_bounds__(f
     const int first = rank * share + warp, last = min((rank + 1) * share, tiles.count);
     const int n_it = first < last ? (last - first + WARPS - 1) / WARPS : 0;
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < WARPS * STAGES; i++) mbar_init(&bars[i], 1);
-        *abort_word = 0;
+    uint8_t *stage = smem + warp * STAGE;
+    uint64_t *bar = bars + warp * 2;
+    if (lane == 0) {
+        mbar_init(&bar[0], 1);
+        mbar_init(&bar[1], 1);
+        if (warp == 0) *abort_word = 0;
         mbar_fence_init();
     }
     __syncthreads();
 
     // ---- copies: lane 0 issues, all lanes together look up 32 tiles at a time
-    uint8_t *ring = smem + warp * STAGES * STAGE;
-    uint64_t *bar = bars + warp * STAGES;
     int look_base = 0;
     int my_row = 0;                                // 8-bit: first row of the tile's codes, -1: page outside the pool
     float my_ks = 1.0f, my_vs = 1.0f;
@@ -124,60 +141,56 @@ template <typename T, bool KV8, bool HALF_M> __global__ void __launch_bounds__(f
         if (KV8) {
             const int it = it0 + lane;
             if (it < n_it) {
-                const long long bi = kv8_block_index(a, s, h3b_win_tile(tiles, first + it * WARPS), kvh);
-                my_row = bi < 0 ? -1 : (int)(bi * KV8_BLOCK);
+                const int tile = h3b_win_tile(tiles, first + it * WARPS);
+                const long long bi = kv8_block_index(a, s, tile * U / KV8_BLOCK, kvh);
+                my_row = bi < 0 ? -1 : (int)(bi * KV8_BLOCK) + tile * U % KV8_BLOCK;
                 my_ks = bi < 0 ? 1.0f : __ldg(a.ks + bi);
                 my_vs = bi < 0 ? 1.0f : __ldg(a.vs + bi);
             }
         }
     };
-    auto issue = [&](int it, int row) {
-        const int st = it % STAGES;
+    int next_row = 0;                              // of the tile whose keys were asked for last
+    float next_ks = 1.0f, next_vs = 1.0f;
+    auto copy = [&](int it, int row, int which) {                                  // which: 0 keys, 1 values
         if (lane == 0) {
-            uint8_t *dst = ring + st * STAGE;
-            mbar_expect_tx(&bar[st], STAGE);
+            uint8_t *dst = stage + which * HALF;
+            mbar_expect_tx(&bar[which], HALF);
+            const CUtensorMap *map = which ? &p.map_v : &p.map_k;
             if (KV8) {
-                tma_load_2d(dst, &p.map_k, &bar[st], 0, max(row, 0));
-                tma_load_2d(dst + HALF, &p.map_v, &bar[st], 0, max(row, 0));
+                tma_load_2d(dst, map, &bar[which], 0, max(row, 0));
             } else {
                 const int key = h3b_win_tile(tiles, first + it * WARPS) * U;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    tma_load_3d(dst + h * (HALF / 2), &p.map_k, &bar[st], h * 64, kvh, key);
-                    tma_load_3d(dst + HALF + h * (HALF / 2), &p.map_v, &bar[st], h * 64, kvh, key);
-                }
+                tma_load_3d(dst, map, &bar[which], 0, kvh, key);
+                tma_load_3d(dst + HALF / 2, map, &bar[which], 64, kvh, key);
             }
         }
     };
-    // rows of tiles whose copies are in flight, in issue order (STAGES of them at most)
-    int rows_q[STAGES];
-    float ks_q[STAGES], vs_q[STAGES];
-    auto fetch = [&](int it, int slot) {           // page and scales of tile `it` (warp-uniform), then its copies
+    auto fetch_keys = [&](int it) {                // page and scales of tile `it` (warp-uniform), then its keys
         if (it - look_base >= 32) look_up(it);
-        const int src = it - look_base;
-        rows_q[slot] = KV8 ? __shfl_sync(0xffffffffu, my_row, src) : 0;
-        ks_q[slot] = KV8 ? __shfl_sync(0xffffffffu, my_ks, src) : 1.0f;
-        vs_q[slot] = KV8 ? __shfl_sync(0xffffffffu, my_vs, src) : 1.0f;
-        issue(it, rows_q[slot]);
+        if (KV8) {
+            next_row = __shfl_sync(0xffffffffu, my_row, it - look_base);
+            next_ks = __shfl_sync(0xffffffffu, my_ks, it - look_base);
+            next_vs = __shfl_sync(0xffffffffu, my_vs, it - look_base);
+        }
+        copy(it, next_row, 0);
     };
     if (n_it) {
         look_up(0);
-#pragma unroll
-        for (int i = 0; i < STAGES; i++)
-            if (i < n_it) fetch(i, i);
+        fetch_keys(0);
+        copy(0, next_row, 1);
     }
 
-    // ---- Q fragments: rows g and g + 8.  16-bit keys: the product's own order of d.  8-bit: lane t takes d = 16 t .. 16 t + 15
-    // and 64 + 16 t .., the 16-byte pieces of a key that it reads.
-    uint32_t qf[8][4];
-    float row_scale[2];                            // scale * log2(e), and what brings Q to f16
+    // ---- Q as the other operand: lane (g, t) has row g of every 8.  16-bit keys: the product's own order of d.  8-bit:
+    // lane t takes d = 16 t .. 16 t + 15 and 64 + 16 t .., the 16-byte pieces of a key that it reads.
+    uint32_t qf[8][NT][2];
+    float row_scale[NT][2];                        // rows 2t, 2t + 1: scale * log2(e), and what brings Q to f16
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int r = r_first + g + 8 * h;
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = r_first + nt * 8 + g;
         const bool live = r < r_end;
         const int qi = live ? r / a.group : qi_first, hd = live ? r - qi * a.group : 0;
         const T *src = reinterpret_cast<const T *>(a.q) + (long long)(e.row0 + qi) * a.q_rs + (long long)(kvh * a.group + hd) * a.q_hs;
-        row_scale[h] = a.scale_log2;
+        float rs = a.scale_log2;
         if (KV8) {
             uint32_t w[16];
 #pragma unroll
@@ -203,218 +216,252 @@ template <typename T, bool KV8, bool HALF_M> __global__ void __launch_bounds__(f
             int sh = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
             sh = odd || top == 0.0f ? 0 : max(min(sh, 120), -120);
             const float up = __uint_as_float((uint32_t)(127 + sh) << 23), down = __uint_as_float((uint32_t)(127 - sh) << 23);
-            row_scale[h] *= down;
+            rs *= down;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {          // step i: words 2i (k 2t, 2t+1) and 2i + 1 (k 2t+8, 2t+9)
-                qf[i][h] = Elem<__half>::pack(to_f<T>(w[2 * i], 0) * up, to_f<T>(w[2 * i], 1) * up);
-                qf[i][2 + h] = Elem<__half>::pack(to_f<T>(w[2 * i + 1], 0) * up, to_f<T>(w[2 * i + 1], 1) * up);
-            }
+            for (int i = 0; i < 8; i++)            // step i: words 2i (k 2t, 2t+1) and 2i + 1 (k 2t+8, 2t+9)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    qf[i][nt][j] = Elem<__half>::pack(to_f<T>(w[2 * i + j], 0) * up, to_f<T>(w[2 * i + j], 1) * up);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
 #pragma unroll
                 for (int j = 0; j < 2; j++)
-                    qf[i][2 * j + h] = live ? __ldg(reinterpret_cast<const uint32_t *>(src + i * 16 + j * 8 + t * 2)) : 0u;
+                    qf[i][nt][j] = live ? __ldg(reinterpret_cast<const uint32_t *>(src + i * 16 + j * 8 + t * 2)) : 0u;
         }
+#pragma unroll
+        for (int j = 0; j < 2; j++) row_scale[nt][j] = KV8 ? __shfl_sync(0xffffffffu, rs, (2 * t + j) * 4) : rs;
     }
-    h3b_win_row wr[2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) wr[h] = h3b_win_of(a.win, e.pos0 + min(r_first + g + 8 * h, r_end - 1) / a.group, e.n);
 
-    float o[16][4];
+    float o[8][NT][4];                             // O^T: 16 dimensions x 8 rows each
 #pragma unroll
-    for (int i = 0; i < 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
-    constexpr int MH = HALF_M ? 1 : 2;
-    const int perm_t = ((t & 1) << 1) | (t >> 1);  // swap of the two bits: see the key order below
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+    float m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) m_run[nt][0] = m_run[nt][1] = -INFINITY, l_run[nt][0] = l_run[nt][1] = 0.0f;
+    // Rows of a tile in shared memory are 128 bytes under the 128-byte swizzle.  8-bit: row g of a 16-key tile is key
+    // swap(g) (bits 0 and 2 exchanged), row g + 8 key 8 + swap(g), and a lane's 16 dimensions of a value are piece
+    // swap(g), so that the eight lanes of one shared-memory phase meet all eight 16-byte banks.
+    const int swap_g = (g & 2) | ((g & 1) << 2) | (g >> 2);
+    const int swap_t = ((t & 1) << 1) | (t >> 1);  // swap(2t); swap(2t + 1) = swap_t + 4
+    const uint32_t kb = smem_u32(stage), vb = kb + HALF;
     bool ok = true;
-    int gave_up = 0;
 
-    auto step = [&](int it, auto slot_c) {
-        constexpr int slot = decltype(slot_c)::value;
-        const int tile = h3b_win_tile(tiles, first + it * WARPS), k0 = tile * U;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar[slot], (it / STAGES) & 1, abort_word, a.status, H3B_ST_TIMEOUT_FULL));
-        if (!ok) {
-            gave_up = it;
-            return;
-        }
-        const uint32_t kb = smem_u32(ring + slot * STAGE), vb = kb + HALF;
-        float sc[NT][4];
+    for (int it = 0; it < n_it; it++) {
+        const int k0 = h3b_win_tile(tiles, first + it * WARPS) * U;
+        const float ks = next_ks, vs = next_vs;
+        const bool absent = KV8 && next_row < 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar[0], it & 1, abort_word, a.status, H3B_ST_TIMEOUT_FULL));
+        if (!ok) break;
+        float sc[MT][NT][4];
 #pragma unroll
-        for (int i = 0; i < NT; i++) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) sc[i][nt][0] = sc[i][nt][1] = sc[i][nt][2] = sc[i][nt][3] = 0.0f;
         if (KV8) {
-            // key of column c of a tile: bits 0 and 2 of c swapped, so that the eight lanes of one shared-memory phase
-            // (two columns) meet all eight 16-byte banks of the swizzled rows
-            const int kr = (g & 2) | ((g & 1) << 2) | (g >> 2);
+            const uint32_t at0 = kb + swap_g * 128 + ((t ^ swap_g) << 4), at1 = kb + swap_g * 128 + (((t + 4) ^ swap_g) << 4);
+            // two tiles at a time: their products do not depend on one another
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const uint32_t row = kb + (i * 8 + kr) * 128;
-                const uint4 x = lds128(row + ((t ^ kr) << 4)), y = lds128(row + (((t + 4) ^ kr) << 4));
-                const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            for (int i = 0; i < MT; i += 2)
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    mma16816<__half>(sc[i], qf[k][0], qf[k][1], qf[k][2], qf[k][3], widen2(w[k]), widen2(w[k] >> 16));
-            }
+                for (int h = 0; h < 2; h++) {      // half of the dimensions
+                    uint32_t w[2][2][4];           // [tile][row half][word]
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            const uint4 x = lds128((h ? at1 : at0) + ((i + u) * 16 + r * 8) * 128);
+                            w[u][r][0] = x.x; w[u][r][1] = x.y; w[u][r][2] = x.z; w[u][r][3] = x.w;
+                        }
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            uint32_t a0, a1, a2, a3;
+                            widen4(w[u][0][k], a0, a2);
+                            widen4(w[u][1][k], a1, a3);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma16816<E>(sc[i + u][nt], a0, a1, a2, a3, qf[4 * h + k][nt][0], qf[4 * h + k][nt][1]);
+                        }
+                }
         } else {
+            const int key = lane & 15;
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const int key = i * 8 + (lane & 7), mat = lane >> 3;           // lane's row of matrix `mat` (16-byte piece of d)
+            for (int k = 0; k < 8; k++)
 #pragma unroll
-                for (int k = 0; k < 8; k += 2) {
-                    const int piece = k * 2 + mat;                              // of 16
-                    uint32_t b0, b1, b2, b3;
-                    ldsm4(kb + (piece >> 3) * (HALF / 2) + key * 128 + (((piece & 7) ^ (key & 7)) << 4), b0, b1, b2, b3);
-                    mma16816<T>(sc[i], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b0, b1);
-                    mma16816<T>(sc[i], qf[k + 1][0], qf[k + 1][1], qf[k + 1][2], qf[k + 1][3], b2, b3);
+                for (int i = 0; i < MT; i++) {
+                    const int piece = 2 * k + (lane >> 4);                          // 16-byte piece of d, of 16
+                    uint32_t a0, a1, a2, a3;
+                    ldsm4(kb + (piece >> 3) * (HALF / 2) + (i * 16 + key) * 128 + (((piece & 7) ^ (key & 7)) << 4), a0, a1, a2, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma16816<E>(sc[i][nt], a0, a1, a2, a3, qf[k][nt][0], qf[k][nt][1]);
+                }
+        }
+        __syncwarp();                                                               // every lane has read the keys
+        if (it + 1 < n_it) fetch_keys(it + 1);
+
+        // exponents: score * scale (+ log2 of the value scale), masked ones -inf; probabilities
+        const float lvs = KV8 ? log2f(vs) : 0.0f, ivs = KV8 ? 1.0f / vs : 1.0f;
+        const bool masked = !h3b_win_full(row_a, row_z, k0, U) || absent;
+        uint32_t pf[MT][NT][2];                                                     // P^T as operand: keys 2t.. and 2t + 8..
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            bool grow = false;
+            float top[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float f = KV8 ? row_scale[nt][j] * ks : row_scale[nt][j];
+                h3b_win_row wr;
+                if (masked) wr = h3b_win_of(a.win, e.pos0 + min(r_first + nt * 8 + 2 * t + j, r_end - 1) / a.group, e.n);
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        float x = KV8 ? fmaf(sc[i][nt][2 * r + j], f, lvs) : sc[i][nt][2 * r + j] * f;
+                        if (masked) {
+                            const int key = k0 + i * 16 + r * 8 + (KV8 ? swap_g : g);
+                            if (!h3b_win_sees(wr, key) || absent) x = -INFINITY;
+                        }
+                        sc[i][nt][2 * r + j] = x;
+                        mx = fmaxf(mx, x);
+                    }
+                top[j] = mx;
+                grow |= mx > m_run[nt][j] + 8.0f || (m_run[nt][j] == -INFINITY && mx > -INFINITY);
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float mx = top[j];
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float m_new = fmaxf(m_run[nt][j], mx);
+                    const float alpha = m_run[nt][j] == -INFINITY ? 0.0f : ex2_approx(m_run[nt][j] - m_new);
+                    m_run[nt][j] = m_new;
+                    l_run[nt][j] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        o[i][nt][j] *= alpha;
+                        o[i][nt][2 + j] *= alpha;
+                    }
                 }
             }
-        }
-        // exponents: score * scale (+ log2 of the value scale), masked ones -inf
-        const float ks = ks_q[slot], vs = vs_q[slot];
-        const float lvs = KV8 ? log2f(vs) : 0.0f, ivs = KV8 ? 1.0f / vs : 1.0f;
-        const bool masked = !h3b_win_full(row_a, row_z, k0, U) || rows_q[slot] < 0;
-        if (!KV8 && masked) {
-            // a value that no row sees must not meet its zero probability (0 * NaN): such rows of the tile become zero
-            const int j = k0 + lane;
-            if (j > row_z.hi || (j < row_a.lo && j >= row_z.s)) {
 #pragma unroll
-                for (int c = 0; c < 16; c++)
-                    *reinterpret_cast<uint4 *>(ring + slot * STAGE + HALF + (c >> 3) * (HALF / 2) + lane * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                fence_proxy_async_smem();          // the next copy into the stage comes behind these stores
+            for (int j = 0; j < 2; j++) {
+                const float m_use = m_run[nt][j] == -INFINITY ? 0.0f : m_run[nt][j];
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const float x = ex2_approx(sc[i][nt][2 * r + j] - m_use);
+                        sc[i][nt][2 * r + j] = x;
+                        sum += x;
+                    }
+                l_run[nt][j] += KV8 ? (sum == 0.0f ? 0.0f : sum * ivs) : sum;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) pf[i][nt][r] = transpose8(Elem<E>::pack(sc[i][nt][2 * r], sc[i][nt][2 * r + 1]));
+        }
+
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar[1], it & 1, abort_word, a.status, H3B_ST_TIMEOUT_FULL));
+        if (!ok) break;
+        if (masked) {
+            // a value that no row sees must not meet its zero probability (0 * NaN; behind a cached sequence lie stale
+            // bytes): such rows of the tile become zero
+#pragma unroll
+            for (int i = 0; i < U; i += 32) {
+                const int j = k0 + i + lane;
+                if (i + lane < U && (j > row_z.hi || (j < row_a.lo && j >= row_z.s))) {
+                    uint8_t *dst = stage + HALF + (i + lane) * 128;
+#pragma unroll
+                    for (int c = 0; c < (KV8 ? 8 : 16); c++)
+                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * (HALF / 2) + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async_smem();      // the next copy into the stage comes behind these stores
+                }
             }
             __syncwarp();
         }
+        // O^T += V^T P^T, 16 keys at a time
 #pragma unroll
-        for (int h = 0; h < MH; h++) {
-            const float f = KV8 ? row_scale[h] * ks : row_scale[h];
-            float mx = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float x = KV8 ? fmaf(sc[i][2 * h + j], f, lvs) : sc[i][2 * h + j] * f;
-                    if (masked) {
-                        const int key = k0 + i * 8 + (KV8 ? perm_t + 4 * j : 2 * t + j);
-                        if (!h3b_win_sees(wr[h], key) || rows_q[slot] < 0) x = -INFINITY;
-                    }
-                    sc[i][2 * h + j] = x;
-                    mx = fmaxf(mx, x);
-                }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m_run[h], mx);
-            // the maximum is followed only when it has grown by more than 2^8: P stays below 2^8, sums undo it
-            const bool grow = m_new > m_run[h] + 8.0f || (m_run[h] == -INFINITY && m_new > -INFINITY);
-            if (__any_sync(0xffffffffu, grow)) {
-                float alpha = 1.0f;
-                if (grow) {
-                    alpha = m_run[h] == -INFINITY ? 0.0f : ex2_approx(m_run[h] - m_new);
-                    m_run[h] = m_new;
-                }
-                l_run[h] *= alpha;
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    o[i][2 * h] *= alpha;
-                    o[i][2 * h + 1] *= alpha;
-                }
-            }
-            const float m_use = m_run[h] == -INFINITY ? 0.0f : m_run[h];
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float x = ex2_approx(sc[i][2 * h + j] - m_use);
-                    sc[i][2 * h + j] = x;
-                    sum += x;
-                }
-            l_run[h] += KV8 ? (sum == 0.0f ? 0.0f : sum * ivs) : sum;
-        }
-        // O += P V, 16 keys at a time
-#pragma unroll
-        for (int i = 0; i < NT; i += 2) {
-            uint32_t pf[4];
+        for (int i = 0; i < MT; i++) {
             if (KV8) {
-                pf[0] = Elem<__half>::pack(sc[i][0], sc[i][1]);
-                pf[1] = HALF_M ? 0u : Elem<__half>::pack(sc[i][2], sc[i][3]);
-                pf[2] = Elem<__half>::pack(sc[i + 1][0], sc[i + 1][1]);
-                pf[3] = HALF_M ? 0u : Elem<__half>::pack(sc[i + 1][2], sc[i + 1][3]);
-                // lane: keys perm_t, perm_t + 4 of both tiles, d piece with bits 0 and 2 of g swapped (as for the keys)
-                const int piece = (g & 2) | ((g & 1) << 2) | (g >> 2);
+                // column c of P^T is key swap(c): lane t has keys swap_t, swap_t + 4 and the same + 8
                 uint4 x[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int key = (i + (r >> 1)) * 8 + perm_t + 4 * (r & 1);
-                    x[r] = lds128(vb + key * 128 + ((piece ^ (key & 7)) << 4));
-                    if (k0 + key >= e.n) x[r] = make_uint4(0u, 0u, 0u, 0u);    // stale bytes behind the sequence
+                    const int key = swap_t + 4 * (r & 1);
+                    x[r] = lds128(vb + (i * 16 + (r >> 1) * 8 + key) * 128 + ((swap_g ^ key) << 4));
                 }
                 const uint32_t w0[4] = {x[0].x, x[0].y, x[0].z, x[0].w}, w1[4] = {x[1].x, x[1].y, x[1].z, x[1].w};
                 const uint32_t w2[4] = {x[2].x, x[2].y, x[2].z, x[2].w}, w3[4] = {x[3].x, x[3].y, x[3].z, x[3].w};
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t lo0 = __byte_perm(w0[j], w1[j], 0x5140), hi0 = __byte_perm(w0[j], w1[j], 0x7362);
-                    const uint32_t lo1 = __byte_perm(w2[j], w3[j], 0x5140), hi1 = __byte_perm(w2[j], w3[j], 0x7362);
-                    mma16816<__half>(o[4 * j], pf[0], pf[1], pf[2], pf[3], widen2(lo0), widen2(lo1));
-                    mma16816<__half>(o[4 * j + 1], pf[0], pf[1], pf[2], pf[3], widen2(lo0 >> 16), widen2(lo1 >> 16));
-                    mma16816<__half>(o[4 * j + 2], pf[0], pf[1], pf[2], pf[3], widen2(hi0), widen2(hi1));
-                    mma16816<__half>(o[4 * j + 3], pf[0], pf[1], pf[2], pf[3], widen2(hi0 >> 16), widen2(hi1 >> 16));
+                for (int j = 0; j < 4; j++) {      // dimensions 4j .. 4j + 3 of the lane's 16: rows g, g + 8 of products 2j, 2j + 1
+                    uint32_t lo[4], hi[4];
+                    widen4(__byte_perm(w0[j], w1[j], 0x5140), lo[0], lo[1]);
+                    widen4(__byte_perm(w0[j], w1[j], 0x7362), lo[2], lo[3]);
+                    widen4(__byte_perm(w2[j], w3[j], 0x5140), hi[0], hi[1]);
+                    widen4(__byte_perm(w2[j], w3[j], 0x7362), hi[2], hi[3]);
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            mma16816<E>(o[2 * j + b][nt], lo[2 * b], lo[2 * b + 1], hi[2 * b], hi[2 * b + 1], pf[i][nt][0], pf[i][nt][1]);
                 }
             } else {
-                pf[0] = Elem<T>::pack(sc[i][0], sc[i][1]);
-                pf[1] = HALF_M ? 0u : Elem<T>::pack(sc[i][2], sc[i][3]);
-                pf[2] = Elem<T>::pack(sc[i + 1][0], sc[i + 1][1]);
-                pf[3] = HALF_M ? 0u : Elem<T>::pack(sc[i + 1][2], sc[i + 1][3]);
-                const int key = i * 8 + (lane & 15);                            // matrices: keys 0-7 | 8-15 of two d pieces
+                const int key = i * 16 + (lane & 7) + ((lane >> 4) << 3);           // matrices: d 0-7 | 8-15, then keys + 8
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int piece = 2 * j + (lane >> 4);
-                    uint32_t b0, b1, b2, b3;
-                    ldsm4t(vb + (piece >> 3) * (HALF / 2) + key * 128 + (((piece & 7) ^ (key & 7)) << 4), b0, b1, b2, b3);
-                    mma16816<T>(o[2 * j], pf[0], pf[1], pf[2], pf[3], b0, b1);
-                    mma16816<T>(o[2 * j + 1], pf[0], pf[1], pf[2], pf[3], b2, b3);
+                    const int piece = 2 * j + ((lane >> 3) & 1);
+                    uint32_t a0, a1, a2, a3;
+                    ldsm4t(vb + (piece >> 3) * (HALF / 2) + key * 128 + (((piece & 7) ^ (key & 7)) << 4), a0, a1, a2, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma16816<E>(o[j][nt], a0, a1, a2, a3, pf[i][nt][0], pf[i][nt][1]);
                 }
             }
         }
-        __syncwarp();                                                           // every lane has read the stage
-        if (it + STAGES < n_it) fetch(it + STAGES, slot);
-    };
-    for (int it = 0; it < n_it && ok; it += STAGES) {
-        step(it, std::integral_constant<int, 0>{});
-        if (ok && it + 1 < n_it) step(it + 1, std::integral_constant<int, 1>{});
-        if (ok && it + 2 < n_it) step(it + 2, std::integral_constant<int, 2>{});
+        __syncwarp();                                                               // every lane has read the values
+        if (it + 1 < n_it) copy(it + 1, next_row, 1);
     }
-    static_assert(STAGES == 3, "the loop above is unrolled by the ring");
-    // a wait that gave up: the copies in flight (of this tile and the STAGES - 1 behind it) get a last, bounded chance to land
+    // a wait that gave up: the copies in flight (one on each barrier) get a last, bounded chance to land
     if (!ok)
-        for (int it = gave_up; it < min(n_it, gave_up + STAGES); it++)
-            for (int spin = 0; spin < 100000 && !mbar_try_wait(&bar[it % STAGES], (it / STAGES) & 1); spin++) {}
+        for (int i = 0; i < 4; i++)
+            for (int spin = 0; spin < 1000 && !mbar_try_wait(&bar[i >> 1], i & 1); spin++) {}
 
     // ---- meet: warps of the CTA
+    float *mine = reinterpret_cast<float *>(stage);                                 // 16 x 128 f32 of this warp
+    __syncwarp();
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
-        l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
-        if (t == 0) {
-            warp_ml[(warp * 16 + g + 8 * h) * 2] = m_run[h];
-            warp_ml[(warp * 16 + g + 8 * h) * 2 + 1] = l_run[h];
-        }
-    }
-    float *mine = reinterpret_cast<float *>(ring);                               // 16 x 128 f32 of this warp
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-    for (int i = 0; i < 16; i++)
+        for (int j = 0; j < 2; j++) {
+            const int r = nt * 8 + 2 * t + j;
+            float l = l_run[nt][j];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            if (g == 0) {
+                warp_ml[(warp * 16 + r) * 2] = m_run[nt][j];
+                warp_ml[(warp * 16 + r) * 2 + 1] = l;
+            }
 #pragma unroll
-        for (int h = 0; h < MH; h++) {
-            const int r = g + 8 * h;
-            if (KV8) {
-                mine[r * 128 + perm_t * 16 + i] = o[i][2 * h];
-                mine[r * 128 + 64 + perm_t * 16 + i] = o[i][2 * h + 1];
-            } else {
-                *reinterpret_cast<float2 *>(&mine[r * 128 + i * 8 + 2 * t]) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+            for (int i = 0; i < 8; i++) {
+                if (KV8) {
+                    *reinterpret_cast<float2 *>(&mine[r * 128 + swap_g * 16 + 2 * i]) = make_float2(o[i][nt][j], o[i][nt][2 + j]);
+                } else {
+                    mine[r * 128 + i * 16 + g] = o[i][nt][j];
+                    mine[r * 128 + i * 16 + g + 8] = o[i][nt][2 + j];
+                }
             }
         }
     __syncthreads();
-    const int d = threadIdx.x;                                                   // THREADS = 128 = head size
-    for (int r = 0; r < R; r++) {
+    for (int i = threadIdx.x; i < R * 128; i += C::THREADS) {
+        const int r = i >> 7;
         float m = -INFINITY, l = 0.0f, v = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; w++) m = fmaxf(m, warp_ml[(w * 16 + r) * 2]);
@@ -424,10 +471,10 @@ template <typename T, bool KV8, bool HALF_M> __global__ void __launch_bounds__(f
             const float c = mw == -INFINITY ? 0.0f : ex2_approx(mw - m);
             // a warp whose l is NaN saw something undefined: it counts even if it has no maximum
             l += lw != lw ? lw : c * lw;
-            v += c * reinterpret_cast<const float *>(smem + w * STAGES * STAGE)[r * 128 + d];
+            v += c * reinterpret_cast<const float *>(smem + w * STAGE)[i];
         }
-        acc[r * 128 + d] = v;
-        if (d == 0) {
+        acc[i] = v;
+        if ((i & 127) == 0) {
             acc_m[r] = m;
             acc_l[r] = l;
         }
@@ -435,50 +482,68 @@ template <typename T, bool KV8, bool HALF_M> __global__ void __launch_bounds__(f
     // ---- CTAs of the cluster: each finishes some rows
     cluster_sync_all();
     const uint32_t acc_addr = smem_u32(acc);
+    const int d = threadIdx.x;                                                   // threads 0..127: one dimension each
     for (int r = rank; r < R; r += p.split) {
-        float m = -INFINITY, l = 0.0f, v = 0.0f;
-        for (int c = 0; c < p.split; c++) m = fmaxf(m, ld_cluster_f32(mapa_shared(acc_addr, c) + (16 * 128 + r) * 4));
-        for (int c = 0; c < p.split; c++) {
-            const uint32_t base = mapa_shared(acc_addr, c);
-            const float mc = ld_cluster_f32(base + (16 * 128 + r) * 4), lc = ld_cluster_f32(base + (16 * 128 + 16 + r) * 4);
-            const float w = mc == -INFINITY ? 0.0f : ex2_approx(mc - m);
-            l += lc != lc ? lc : w * lc;
-            v += w * ld_cluster_f32(base + (r * 128 + d) * 4);
-        }
         const int qi = (r_first + r) / a.group, hd = (r_first + r) - qi * a.group;
-        const h3b_win_row wr_r = h3b_win_of(a.win, e.pos0 + qi, e.n);
-        const int seen = h3b_win_count(wr_r);
-        const float res = seen ? v * (1.0f / l) : 0.0f;
-        T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qi) * a.o_rs + (long long)(kvh * a.group + hd) * a.o_hs;
-        const uint32_t w2 = Elem<T>::pack(res, res);
-        reinterpret_cast<unsigned short *>(dst)[d] = (unsigned short)(w2 & 0xffffu);
+        bool odd = false;
+        if (d < 128) {
+            float m = -INFINITY, l = 0.0f, v = 0.0f;
+            for (int c = 0; c < p.split; c++) m = fmaxf(m, ld_cluster_f32(mapa_shared(acc_addr, c) + (16 * 128 + r) * 4));
+            for (int c = 0; c < p.split; c++) {
+                const uint32_t base = mapa_shared(acc_addr, c);
+                const float mc = ld_cluster_f32(base + (16 * 128 + r) * 4), lc = ld_cluster_f32(base + (16 * 128 + 16 + r) * 4);
+                const float w = mc == -INFINITY ? 0.0f : ex2_approx(mc - m);
+                l += lc != lc ? lc : w * lc;
+                v += w * ld_cluster_f32(base + (r * 128 + d) * 4);
+            }
+            const float res = h3b_win_count(h3b_win_of(a.win, e.pos0 + qi, e.n)) ? v * (1.0f / l) : 0.0f;
+            T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qi) * a.o_rs + (long long)(kvh * a.group + hd) * a.o_hs;
+            reinterpret_cast<unsigned short *>(dst)[d] = (unsigned short)(Elem<T>::pack(res, res) & 0xffffu);
+            odd = !(fabsf(res) < INFINITY);
+        }
         // a value that is not finite and that other rows of the tile see: such a row is computed again from its own keys
-        if (!KV8 && __syncthreads_or(!(fabsf(res) < INFINITY))) {
+        if (!KV8 && __syncthreads_or(odd)) {
             if (warp == 0) attn_row_by_warp<T, KV8>(a, s, e, qi, kvh * a.group + hd, lane);
         }
     }
     cluster_sync_all();                                                          // nobody leaves while its memory is read
 }
 
-// CTAs that share the keys of one (sequence, K/V head, 16 rows): as many as fill the chip once, but no fewer than
-// `WARPS` tiles each (a ring is then filled once), and at most 8 (the portable cluster size).
-static int few_split(const h3_cuda *cuda, size_t units, size_t tiles) {
-    const size_t by_chip = units >= (size_t)cuda->sm_count ? 1 : (size_t)cuda->sm_count / units;
-    const size_t by_work = std::max<size_t>(tiles / few::WARPS, 1);
-    return (int)std::min<size_t>(std::min(by_chip, by_work), 8);
+// How the keys of one (sequence, K/V head, row tile) are shared out.
+struct FewPlan {
+    bool wide;
+    int split;                                     // CTAs of a cluster
+};
+// Measured on 148 SMs (us; an E4M3 cache unless said otherwise):
+//   8 pairs of 100,000 keys: WIDE in clusters of 8 50, of 4 90; narrow of 8 81.  16 pairs of 20,000: WIDE of 6 19.4, of 8
+//   (which fit the chip 15 times only) 31; narrow of 8 24.8.  24 pairs of 20,000: WIDE of 5 28.2, narrow of 8 27.8, of 1 126.
+//   96 pairs of up to 12,000: narrow of 4 (384 CTAs, one wave) 33.6, of 1 77.6, of 5 41.7; WIDE 40.
+//   512 pairs of up to 16,000: narrow of 4 157, of 1 182; 1536 pairs of up to 2,000: of 1 80.6, of 2 96.7.
+// So: one wave where that is possible; beyond it shares of 32 tiles, below which a CTA's beginning and end cost more than
+// even shares gain.
+static FewPlan few_plan(const h3_cuda *cuda, size_t units, size_t tiles) {
+    const size_t sms = (size_t)cuda->sm_count, some = std::max<size_t>(tiles / 4, 1);   // a tile for every warp of four
+    const size_t room_wide = sms * 89 / 100, room = sms * 29 / 10;                      // CTAs that clusters find room for
+    FewPlan p;
+    p.wide = units * 6 <= room_wide;
+    if (p.wide) p.split = (int)std::min(std::min<size_t>(room_wide / units, 8), some);
+    else if (2 * units <= room) p.split = (int)std::min(std::min<size_t>(room / units, 8), some);
+    else p.split = (int)std::min<size_t>(std::max<size_t>(tiles / 32, 1), 4);
+    return p;
 }
 
-template <typename T, bool KV8> static int launch_few_t(h3_cuda *cuda, const FewParams &p, dim3 grid, bool half_m, char *error, size_t error_size) {
-    void (*kernel)(const FewParams) = half_m ? k_attn_few<T, KV8, true> : k_attn_few<T, KV8, false>;
-    H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few::SMEM_BYTES), "attention smem attribute");
+template <typename T, bool KV8, bool WIDE> static int launch_few_t(h3_cuda *cuda, const FewParams &p, dim3 grid, int nt, char *error, size_t error_size) {
+    void (*kernel)(const FewParams) = nt == 1 ? k_attn_few<T, KV8, 1, WIDE> : k_attn_few<T, KV8, 2, WIDE>;
+    using C = few::Cfg<KV8, WIDE>;
+    H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM_BYTES), "attention smem attribute");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)p.split; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(few::THREADS);
-    cfg.dynamicSmemBytes = few::SMEM_BYTES;
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM_BYTES;
     cfg.stream = cuda->op_stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
@@ -499,24 +564,28 @@ int launch_attn_few(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t l
     p.a = a;
     if (kv8) {
         const uint64_t n = (uint64_t)a.pages * a.kv_heads * a.page_blocks * KV8_BLOCK;
-        if (h3b_encode_tmap_2d(&p.map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.kc, 128, n, 128, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
-            h3b_encode_tmap_2d(&p.map_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.vc, 128, n, 128, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B))
+        if (h3b_encode_tmap_2d(&p.map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.kc, 128, n, 128, 128, few::Cfg<true, false>::U, CU_TENSOR_MAP_SWIZZLE_128B) ||
+            h3b_encode_tmap_2d(&p.map_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.vc, 128, n, 128, 128, few::Cfg<true, false>::U, CU_TENSOR_MAP_SWIZZLE_128B))
             return fail(error, error_size, "kv8_sdpa: cuTensorMapEncodeTiled failed");
     } else if (a.lk) {
         const CUtensorMapDataType dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        if (h3b_encode_tmap_3d(&p.map_k, dt, 2, a.k, 128, a.kv_heads, a.lk, a.k_hs * 2, a.k_rs * 2, 64, 1, 32, CU_TENSOR_MAP_SWIZZLE_128B) ||
-            h3b_encode_tmap_3d(&p.map_v, dt, 2, a.v, 128, a.kv_heads, a.lk, a.v_hs * 2, a.v_rs * 2, 64, 1, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+        if (h3b_encode_tmap_3d(&p.map_k, dt, 2, a.k, 128, a.kv_heads, a.lk, a.k_hs * 2, a.k_rs * 2, 64, 1, few::Cfg<false, false>::U, CU_TENSOR_MAP_SWIZZLE_128B) ||
+            h3b_encode_tmap_3d(&p.map_v, dt, 2, a.v, 128, a.kv_heads, a.lk, a.v_hs * 2, a.v_rs * 2, 64, 1, few::Cfg<false, false>::U, CU_TENSOR_MAP_SWIZZLE_128B))
             return fail(error, error_size, "sdpa_window: cuTensorMapEncodeTiled failed");
     }
-    const size_t rows = (size_t)a.max_rows * a.group, mtiles = ceil_div(rows, 16);
+    const size_t rows = (size_t)a.max_rows * a.group;
+    const int nt = rows <= 8 ? 1 : 2;
+    const size_t mtiles = ceil_div(rows, 8 * (size_t)nt);
     const size_t keys = window_keys(a.win, len, (size_t)a.max_rows);
-    p.split = few_split(cuda, mtiles * a.kv_heads * a.n_seq, ceil_div(keys, kv8 ? few::UNIT8 : few::UNIT16));
+    const FewPlan plan = few_plan(cuda, mtiles * a.kv_heads * a.n_seq, ceil_div(keys, kv8 ? few::Cfg<true, false>::U : few::Cfg<false, false>::U));
+    p.split = plan.split;
     const dim3 grid((unsigned)(mtiles * p.split), (unsigned)a.kv_heads, (unsigned)a.n_seq);
-    const bool half = rows <= 8;
-    if (kv8) return f16 ? launch_few_t<__half, true>(cuda, p, grid, half, error, error_size)
-                        : launch_few_t<__nv_bfloat16, true>(cuda, p, grid, half, error, error_size);
-    return f16 ? launch_few_t<__half, false>(cuda, p, grid, half, error, error_size)
-               : launch_few_t<__nv_bfloat16, false>(cuda, p, grid, half, error, error_size);
+    int (*launch)(h3_cuda *, const FewParams &, dim3, int, char *, size_t);
+    if (kv8) launch = f16 ? (plan.wide ? launch_few_t<__half, true, true> : launch_few_t<__half, true, false>)
+                          : (plan.wide ? launch_few_t<__nv_bfloat16, true, true> : launch_few_t<__nv_bfloat16, true, false>);
+    else launch = f16 ? (plan.wide ? launch_few_t<__half, false, true> : launch_few_t<__half, false, false>)
+                      : (plan.wide ? launch_few_t<__nv_bfloat16, false, true> : launch_few_t<__nv_bfloat16, false, false>);
+    return launch(cuda, p, grid, nt, error, error_size);
 }
 
 }  // namespace h3b
