@@ -552,12 +552,6 @@ template <typename T, bool KV8, bool WIDE> static int launch_few_t(h3_cuda *cuda
     return 1;
 }
 
-// Keys that one sequence's rows can see at most, for the split (an estimate is enough).
-static size_t window_keys(const h3b_win &w, size_t len, size_t rows) {
-    const size_t reach = (size_t)w.left + (size_t)w.right + (size_t)w.block + rows;
-    return std::min(len, reach >= (size_t)H3B_WIN_MAX ? len : reach + (size_t)w.sinks);
-}
-
 int launch_attn_few(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t len, char *error, size_t error_size) {
     FewParams p;
     memset(&p, 0, sizeof(p));
@@ -576,7 +570,7 @@ int launch_attn_few(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t l
     const size_t rows = (size_t)a.max_rows * a.group;
     const int nt = rows <= 8 ? 1 : 2;
     const size_t mtiles = ceil_div(rows, 8 * (size_t)nt);
-    const size_t keys = window_keys(a.win, len, (size_t)a.max_rows);
+    const size_t keys = attn_window_keys(a.win, len, (size_t)a.max_rows);
     const FewPlan plan = few_plan(cuda, mtiles * a.kv_heads * a.n_seq, ceil_div(keys, kv8 ? few::Cfg<true, false>::U : few::Cfg<false, false>::U));
     p.split = plan.split;
     const dim3 grid((unsigned)(mtiles * p.split), (unsigned)a.kv_heads, (unsigned)a.n_seq);

@@ -4,13 +4,6 @@
 
 namespace h3b {
 
-template <typename T, bool KV8> __global__ void __launch_bounds__(128) k_attn_rows_plain(const __grid_constant__ WinArgs a) {
-    const int s = blockIdx.z, row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
-    const SeqExt e = seq_ext<KV8>(a, s);
-    if (row >= e.nq || head >= a.heads) return;
-    attn_row_by_warp<T, KV8>(a, s, e, row, head, threadIdx.x & 31);
-}
-
 static int clip(int64_t v) { return v < 0 || v > H3B_WIN_MAX ? H3B_WIN_MAX : (int)v; }
 
 // checks and fields common to both entry points
@@ -46,12 +39,7 @@ template <bool KV8> static int launch(h3_cuda *cuda, const WinArgs &a, int f16, 
     DeviceGuard guard(cuda);
     ProfScope prof(cuda, PROF_ATTN);
     if ((size_t)a.max_rows * a.group <= 64) return launch_attn_few(cuda, a, f16, KV8, len, error, error_size);
-    const dim3 grid((unsigned)a.max_rows, (unsigned)ceil_div(a.heads, 4), (unsigned)a.n_seq);
-    if (f16) k_attn_rows_plain<__half, KV8><<<grid, 128, 0, cuda->op_stream>>>(a);
-    else k_attn_rows_plain<__nv_bfloat16, KV8><<<grid, 128, 0, cuda->op_stream>>>(a);
-    cuda->launches++;
-    H3B_CUDA_OK(cudaGetLastError(), "windowed attention launch");
-    return 1;
+    return launch_attn_tile(cuda, a, f16, KV8, len, error, error_size);
 }
 
 }  // namespace h3b

@@ -157,7 +157,14 @@ __device__ __noinline__ void attn_row_by_warp(const WinArgs &a, int s, const Seq
     *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + (long long)(e.row0 + row) * a.o_rs + head * a.o_hs + lane * 4) = w;
 }
 
-// few query rows per K/V head: h3b_attn_few.cu.  len: keys of the longest sequence (an estimate guides the split)
+// Keys that the rows of one CTA can see at most (an estimate that guides how the keys are split).
+static inline size_t attn_window_keys(const h3b_win &w, size_t len, size_t rows) {
+    const size_t reach = (size_t)w.left + (size_t)w.right + (size_t)w.block + rows + (size_t)w.sinks;
+    return reach < len ? reach : len;
+}
+
+// many query rows per K/V head: h3b_attn_tile.cu; few: h3b_attn_few.cu.  len: keys of the longest sequence (an estimate guides the split)
+int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t len, char *error, size_t error_size);
 int launch_attn_few(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t len, char *error, size_t error_size);
 
 }  // namespace h3b
