@@ -39,8 +39,9 @@ constexpr int TMEM_COLS = 512;
 constexpr uint32_t S_COL = 0, O_COL = 256;                // + 128 * row tile
 constexpr int SOFTMAX_WARP = 4, WIDEN_WARP = 12;
 constexpr int PART_ROW = 132;                             // floats of a parked row: 16-byte lanes of 8 rows hit all banks
-// Q_A Q_B | K0 K1 | V0 V1 (at the end: parked rows) | barriers | scales
-constexpr size_t SMEM_BYTES = 1024 + 6 * (size_t)TILE + 512;
+constexpr int CODES = 128 * 128;                          // E4M3 codes of a tile
+// Q_A Q_B | K0 K1 | V0 V1 (at the end: parked rows) | 8-bit: codes of a key and of a value tile | barriers | scales
+template <bool KV8> constexpr size_t smem_bytes() { return 1024 + 6 * (size_t)TILE + (KV8 ? 2 * CODES : 0) + 512; }
 static_assert(256 * PART_ROW * 4 + 2 * 256 * 4 <= 6 * TILE, "parked rows");
 }  // namespace wtile
 
@@ -76,8 +77,8 @@ template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setm
 
 template <bool KV8> struct TileCfg {
     static constexpr int THREADS = KV8 ? 512 : 384;
-    // 8-bit: 512 threads start with 128 registers; 4 warps x 32 x (72 + 2 * 176 + 88) = 65,536
-    static constexpr int REG_ISSUE = 72, REG_SOFTMAX = 176, REG_WIDEN = 88;
+    // 8-bit: 512 threads start with 128 registers each, 72 + 2 * 184 + 72 = 4 * 128; 16-bit: 384 with 168, 88 + 2 * 208 = 3 * 168
+    static constexpr int REG_ISSUE = KV8 ? 72 : 88, REG_SOFTMAX = KV8 ? 184 : 208, REG_WIDEN = 72;
 };
 
 // EMU: bit q set = the q-th group of four probabilities of every 32 on the FMA pipe (ex2_emu2)
@@ -88,13 +89,14 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     using E = typename std::conditional<KV8, __half, T>::type;          // operand type
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *sQ = smem, *sK = smem + 2 * TILE, *sV = smem + 4 * TILE;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + 6 * TILE);
+    uint8_t *sQ = smem, *sK = smem + 2 * TILE, *sV = smem + 4 * TILE, *sC = smem + 6 * TILE;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sC + (KV8 ? 2 * CODES : 0));
     uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7, *s_full = bars + 9,
              *p_full = bars + 11 /* [tile][half] */, *o_done = bars + 15, *v_raw = bars + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+    uint64_t *c_full = bars + 17 /* [keys, values] */, *c_empty = bars + 19;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 21);
     volatile int *abort_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    float4 *scales = reinterpret_cast<float4 *>(smem + 6 * TILE + 160);  // [4]: key scale of either half, value scale of either half
+    float4 *scales = reinterpret_cast<float4 *>(bars + 24);               // [4]: key scale of either half, value scale of either half
 
     const WinArgs &a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -126,6 +128,10 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         }
         mbar_init(o_done, 1);
         mbar_init(v_raw, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&c_full[i], 1);
+            mbar_init(&c_empty[i], 4);
+        }
         *abort_word = 0;
         mbar_fence_init();
     }
@@ -140,7 +146,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     bool ok = true;
 
     if (warp < SOFTMAX_WARP) {
-        if (KV8) regs_dec<C::REG_ISSUE>();
+        regs_dec<C::REG_ISSUE>();
         if (warp == 0 && !KV8) {
             // ------------------------------------------------------------ K and V by TMA
             uint32_t raw = 0;
@@ -176,6 +182,43 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&v_full[st]);
+                }
+            }
+        } else if (warp == 0 && n_kv > 0) {
+            // ------------------------------------------------------------ codes of the pages by bulk copies, 64 tokens each
+            // (8 KiB that lie together).  Lanes look up the blocks of 16 tiles at a time.
+            int look = 0, bi = -1;
+            float bks = 1.0f, bvs = 1.0f;
+            for (int j = 0; j < n_kv && ok; j++) {
+                if (j % 16 == 0) {
+                    look = j;
+                    bi = -1;
+                    const int jj = j + (lane >> 1);
+                    if (jj < n_kv) {
+                        const int blk = key_of(jj) / KV8_BLOCK + (lane & 1);
+                        if (blk * KV8_BLOCK < e.n) bi = (int)kv8_block_index(a, s, blk, kvh);
+                    }
+                    bks = bi >= 0 ? __ldg(a.ks + bi) : 1.0f;
+                    bvs = bi >= 0 ? __ldg(a.vs + bi) : 1.0f;
+                }
+                const int src = 2 * (j - look);
+                const int b0 = __shfl_sync(0xffffffffu, bi, src), b1 = __shfl_sync(0xffffffffu, bi, src + 1);
+                const float4 sc = make_float4(__shfl_sync(0xffffffffu, bks, src), __shfl_sync(0xffffffffu, bks, src + 1),
+                                              __shfl_sync(0xffffffffu, bvs, src), __shfl_sync(0xffffffffu, bvs, src + 1));
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&c_empty[w], (j & 1) ^ 1, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
+                    if (!ok) break;
+                    if (lane == 0) {
+                        // scales of tile j: the softmax warps read them behind s_full(j); the slot is that of tile j - 4,
+                        // whose scores were done with before the codes of tile j - 1 could be widened
+                        if (w == 0) scales[j & 3] = sc;
+                        const uint8_t *codes = w ? a.vc : a.kc;
+                        // a block outside the pool (reported) or behind the last token is not read: its rows are hidden or invalid
+                        mbar_expect_tx(&c_full[w], (b0 >= 0 ? CODES / 2 : 0) + (b1 >= 0 ? CODES / 2 : 0));
+                        if (b0 >= 0) bulk_load(sC + w * CODES, codes + (long long)b0 * (CODES / 2), CODES / 2, &c_full[w]);
+                        if (b1 >= 0) bulk_load(sC + w * CODES + CODES / 2, codes + (long long)b1 * (CODES / 2), CODES / 2, &c_full[w]);
+                    }
                 }
             }
         } else if (warp == 1 && n_kv > 0) {
@@ -250,51 +293,48 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         __syncwarp();
     } else if (warp < WIDEN_WARP) {
         // ---------------------------------------------------------------- softmax
-        if (KV8) regs_inc<C::REG_SOFTMAX>();
+        regs_inc<C::REG_SOFTMAX>();
         const int t = (warp - SOFTMAX_WARP) >> 2, q = warp & 3;          // row tile, TMEM lane quarter
         const int my = r0 + t * BM + q * 32 + lane;                      // row of this thread
         const bool live = my < r_end;
         const int qi = (live ? my : r_end - 1) / a.group, hd = (live ? my : r_end - 1) - qi * a.group;
         float row_scale = a.scale_log2;
         if (t < n_tiles && n_kv) {                                       // without keys the memory is the epilogue's at once
-            // Q row -> shared memory (8-bit: f16 under a power of two of the row's maximum, undone by row_scale)
-            const T *src = reinterpret_cast<const T *>(a.q) + (long long)(e.row0 + qi) * a.q_rs + (long long)(kvh * a.group + hd) * a.q_hs;
-            uint8_t *dst = sQ + t * TILE + (q * 32 + lane) * 128;
+            // Q -> shared memory, sixteen lanes per 256-byte row (8-bit: f16 under a power of two of the row's maximum,
+            // undone by row_scale)
+            const long long mine = live ? (long long)(e.row0 + qi) * a.q_rs + (long long)(kvh * a.group + hd) * a.q_hs : -1;
+            const int sub = lane >> 4, c = lane & 15;
             uint4 w[16];
 #pragma unroll
-            for (int c = 0; c < 16; c++) w[c] = live ? __ldg(reinterpret_cast<const uint4 *>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
-            if (KV8) {
-                float top = 0.0f;
-                bool odd = false;
-                auto value = [](uint32_t v, int hi) {
-                    if (Elem<T>::FMT == 1) return __uint_as_float(hi ? v & 0xffff0000u : v << 16);
-                    return __half2float(__ushort_as_half((unsigned short)(hi ? v >> 16 : v & 0xffffu)));
-                };
-#pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    const uint32_t v[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float f = fabsf(value(v[i >> 1], i & 1));
-                        odd |= !(f < INFINITY);
-                        top = fmaxf(top, f);
-                    }
-                }
-                int sh = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
-                sh = odd || top == 0.0f ? 0 : max(min(sh, 120), -120);
-                const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-                row_scale *= __uint_as_float((uint32_t)(127 - sh) << 23);
-#pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    uint32_t v[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = Elem<__half>::pack(value(v[i], 0) * up, value(v[i], 1) * up);
-                    w[c] = make_uint4(v[0], v[1], v[2], v[3]);
-                }
+            for (int i = 0; i < 16; i++) {
+                const long long off = __shfl_sync(0xffffffffu, mine, 2 * i + sub);
+                w[i] = off >= 0 ? __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + off) + c) : make_uint4(0u, 0u, 0u, 0u);
             }
 #pragma unroll
-            for (int c = 0; c < 16; c++)
-                *reinterpret_cast<uint4 *>(dst + (c >> 3) * SLAB + (((c & 7) ^ (lane & 7)) << 4)) = w[c];
+            for (int i = 0; i < 16; i++) {
+                if (KV8) {
+                    uint32_t top = abs_max8<T>(w[i]);
+#pragma unroll
+                    for (int x = 1; x < 16; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const uint32_t bits = widen_abs<T>(top);
+                    int sh = 14 - ((int)(bits >> 23) - 127);
+                    sh = bits >= 0x7f800000u || bits == 0u ? 0 : max(min(sh, 120), -120);   // not finite: as it is
+                    const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+                    const int down = __shfl_sync(0xffffffffu, 127 - sh, (lane & 1) * 16);
+                    if ((lane >> 1) == i) row_scale *= __uint_as_float((uint32_t)down << 23);
+                    uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        float2 f;
+                        if (Elem<T>::FMT == 1) f = make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u));
+                        else f = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
+                        v[k] = Elem<__half>::pack(f.x * up, f.y * up);
+                    }
+                    w[i] = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+                const int row = q * 32 + 2 * i + sub;
+                *reinterpret_cast<uint4 *>(sQ + t * TILE + (c >> 3) * SLAB + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = w[i];
+            }
             fence_proxy_async_smem();
         }
         __syncwarp();
@@ -499,25 +539,17 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         // ---------------------------------------------------------------- widen the codes of a tile
         regs_dec<C::REG_WIDEN>();
         const int w4 = warp - WIDEN_WARP, sub = lane >> 3, piece = lane & 7;   // row within four, 16 codes of the row
-        // rows i * 16 + w4 * 4 + sub of a tile, i = 0..7: the first four in its first 64 keys
-        auto blocks_of = [&](int j, int (&bi)[2]) {
-            const int blk = key_of(j) / KV8_BLOCK;
+        // 16 codes -> 32 bytes: pieces 2 * (piece & 3), + 1 of slab piece >> 2; lanes of the second slab write their second
+        // piece first, so that the eight lanes of a row hit all banks
+        const int second = piece >> 2, c = 2 * (piece & 3);
+        auto widen = [&](uint8_t *tile, const uint8_t *codes, int key, bool unseen) {
+            uint4 raw[8];
 #pragma unroll
-            for (int h = 0; h < 2; h++) bi[h] = (blk + h) * KV8_BLOCK < e.n ? (int)kv8_block_index(a, s, blk + h, kvh) : -1;
-        };
-        auto ask = [&](const uint8_t *codes, const int (&bi)[2], int key, uint4 (&raw)[8]) {
+            for (int i = 0; i < 8; i++) raw[i] = *reinterpret_cast<const uint4 *>(codes + (i * 16 + w4 * 4 + sub) * 128 + piece * 16);
+            if (unseen)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int row = i * 16 + w4 * 4 + sub;
-                raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (bi[i >> 2] >= 0 && !hidden(key + row))
-                    raw[i] = __ldg(reinterpret_cast<const uint4 *>(codes + ((long long)bi[i >> 2] * KV8_BLOCK + (row & 63)) * 128) + piece);
-            }
-        };
-        auto put = [&](uint8_t *tile, const uint4 (&raw)[8]) {
-            // 16 codes -> 32 bytes: pieces 2 * (piece & 3), + 1 of slab piece >> 2; lanes of the second slab write their
-            // second piece first, so that the eight lanes of a row hit all banks
-            const int first = piece >> 2;
+                for (int i = 0; i < 8; i++)
+                    if (hidden(key + i * 16 + w4 * 4 + sub)) raw[i] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int row = i * 16 + w4 * 4 + sub;
@@ -529,42 +561,28 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     h[2 * k + 1] = widen2_e4m3((uint16_t)(v[k] >> 16));
                 }
                 const uint4 x = make_uint4(h[0], h[1], h[2], h[3]), y = make_uint4(h[4], h[5], h[6], h[7]);
-                uint8_t *dst = tile + first * SLAB + row * 128;
-                const int c = 2 * (piece & 3);
-                *reinterpret_cast<uint4 *>(dst + (((c + first) ^ (row & 7)) << 4)) = first ? y : x;
-                *reinterpret_cast<uint4 *>(dst + (((c + 1 - first) ^ (row & 7)) << 4)) = first ? x : y;
+                uint8_t *dst = tile + second * SLAB + row * 128;
+                *reinterpret_cast<uint4 *>(dst + (((c + second) ^ (row & 7)) << 4)) = second ? y : x;
+                *reinterpret_cast<uint4 *>(dst + (((c + 1 - second) ^ (row & 7)) << 4)) = second ? x : y;
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
-        uint4 kr[8], vr[8];
-        int bi[2] = {-1, -1};
-        if (n_kv) {
-            blocks_of(0, bi);
-            ask(a.kc, bi, key_of(0), kr);
-            ask(a.vc, bi, key_of(0), vr);
-        }
         for (int j = 0; j < n_kv && ok; j++) {
-            const int st = j & 1;
+            const int st = j & 1, key = key_of(j);
             const uint32_t ph = ((j >> 1) & 1) ^ 1;
-            int nb[2] = {-1, -1};
-            if (j + 1 < n_kv) blocks_of(j + 1, nb);
-            ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
-            if (!ok) break;
-            // scales of tile j: read by the softmax warps behind s_full(j); the slot was last read for tile j - 4
-            if (w4 == 0 && lane == 0)
-                scales[j & 3] = make_float4(bi[0] >= 0 ? __ldg(a.ks + bi[0]) : 1.0f, bi[1] >= 0 ? __ldg(a.ks + bi[1]) : 1.0f,
-                                            bi[0] >= 0 ? __ldg(a.vs + bi[0]) : 1.0f, bi[1] >= 0 ? __ldg(a.vs + bi[1]) : 1.0f);
-            put(sK + st * TILE, kr);
-            if (lane == 0) mbar_arrive(&k_full[st]);
-            if (j + 1 < n_kv) ask(a.kc, nb, key_of(j + 1), kr);
-            ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
-            if (!ok) break;
-            put(sV + st * TILE, vr);
-            if (lane == 0) mbar_arrive(&v_full[st]);
-            if (j + 1 < n_kv) ask(a.vc, nb, key_of(j + 1), vr);
-            bi[0] = nb[0];
-            bi[1] = nb[1];
+            const bool unseen = hidden(key + BN - 1) || hidden(key) || (key < row_a.lo && key + BN > row_z.s);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&c_full[w], j & 1, abort_word, a.status, H3B_ST_TIMEOUT_FULL) &&
+                                                 mbar_wait(w ? &v_empty[st] : &k_empty[st], ph, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
+                if (!ok) break;
+                widen((w ? sV : sK) + st * TILE, sC + w * CODES, key, unseen);
+                if (lane == 0) {
+                    mbar_arrive(w ? &v_full[st] : &k_full[st]);
+                    mbar_arrive(&c_empty[w]);
+                }
+            }
         }
     }
 
@@ -611,7 +629,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
 
 template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const TileParams &p, dim3 grid, char *error, size_t error_size) {
     void (*kernel)(const TileParams) = k_attn_tile<T, KV8, 0x11>;
-    H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wtile::SMEM_BYTES), "attention smem attribute");
+    H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wtile::smem_bytes<KV8>()), "attention smem attribute");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attr;
@@ -619,7 +637,7 @@ template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const Ti
     attr.val.clusterDim.x = (unsigned)p.split; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
     cfg.gridDim = grid;
     cfg.blockDim = dim3(TileCfg<KV8>::THREADS);
-    cfg.dynamicSmemBytes = wtile::SMEM_BYTES;
+    cfg.dynamicSmemBytes = wtile::smem_bytes<KV8>();
     cfg.stream = cuda->op_stream;
     cfg.attrs = &attr;
     cfg.numAttrs = p.split > 1 ? 1 : 0;

@@ -74,6 +74,23 @@ __device__ __forceinline__ long long kv8_block_index(const WinArgs &a, int s, in
     return ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
 }
 
+// largest magnitude of eight 16-bit floats as their bit pattern: magnitudes order like integers, NaN above infinity
+template <typename T> __device__ __forceinline__ uint32_t abs_max8(const uint4 &w) {
+    uint32_t m = 0;
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t t = v[i] & 0x7fff7fffu;
+        m = max(m, max(t & 0xffffu, t >> 16));
+    }
+    return m;
+}
+// such a pattern as that of an f32
+template <typename T> __device__ __forceinline__ uint32_t widen_abs(uint32_t h) {
+    if (Elem<T>::FMT == 1) return h << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+}
+
 template <typename T> __device__ __forceinline__ float4 load4(const T *p) {
     const uint2 w = *reinterpret_cast<const uint2 *>(p);
     float4 r;

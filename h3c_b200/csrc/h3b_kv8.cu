@@ -61,21 +61,6 @@ __device__ __forceinline__ float kv8_scale(uint32_t abs_bits) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-template <typename T> __device__ __forceinline__ uint32_t abs_max8(const uint4 &w) {
-    uint32_t m = 0;
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t t = v[i] & 0x7fff7fffu;
-        m = max(m, max(t & 0xffffu, t >> 16));
-    }
-    return m;   // 16-bit pattern: magnitudes order like integers, NaN above infinity
-}
-template <typename T> __device__ __forceinline__ uint32_t widen_abs(uint32_t h) {
-    if (Elem<T>::FMT == 1) return h << 16;
-    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
-}
-
 template <typename T> __global__ void __launch_bounds__(256) k_kv8_append(const __grid_constant__ AppendArgs a) {
     __shared__ uint32_t red[2][8];
     const int s = blockIdx.z, kvh = blockIdx.y, tid = threadIdx.x;
