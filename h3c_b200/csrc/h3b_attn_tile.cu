@@ -1,30 +1,38 @@
 // Windowed attention for many query rows per K/V head on tcgen05: the tensor core is the bound, so it has to be fed
 // without a pause.
 //
-// One CTA per (256 rows of one K/V head = two 128-row tiles A and B, range of keys).  A row is a (query, head) pair of
-// the K/V head's group, queries outermost: shared heads fill tiles with few queries, and K and V are read once for all
-// heads of the group.  The key tiles (128 keys) that a CTA visits are the tiles of the sinks and of the union of its
+// A work item is (two row tiles A and B of one K/V head, range of keys).  A row is a (query, head) pair of the K/V head's
+// group, queries outermost: shared heads fill tiles with few queries, and K and V are read once for all heads of the
+// group.  A tile holds as many whole queries as fit 128 rows (126 rows for groups of 3, 6, 7), so that one TMA box of
+// {64 dimensions, group, queries} brings half of its Q.  The key tiles (128 keys) that an item visits are the tiles of the sinks and of the union of its
 // rows' windows (h3b_window.h); only a tile that some row does not see wholly pays for a mask.
-//   warp 0       16-bit: K and V tiles by TMA, two-deep.  8-bit: idle
+// A CTA stays on its SM and takes item after item (cluster launch control hands it the CTAs that have not started yet,
+// in grid order, so the chip balances itself), and the roles run ahead into the next item: its Q, K and V arrive while
+// the last softmax and the stores of the current one are under way.  With one item per CTA, a window of 256 keys took
+// 17 us per item, 8 of them waiting for Q and the first keys and 4 storing; frames of the 6,144-token step 234 us.
+//   warp 0       16-bit: K and V tiles by TMA; 8-bit: the codes of a tile by bulk copies, one tile ahead
 //   warp 1       MMA issuer: per key tile and row tile S = Q K^T (128x128x128) into TMEM, then O += P V with P from TMEM,
 //                the two row tiles interleaved so that the tensor core works on one while the other is in its softmax
-//   warps 4-7    softmax of tile A, warps 8-11 of tile B: one row per thread.  They bring Q to shared memory first, read
-//                the 128 scores once, and write P back over the score columns in two halves of 64 keys; the accumulator
-//                is rescaled only when the running maximum grew by more than 2^8
-//   warps 12-15  8-bit: widen the codes of a tile from registers (asked for one tile ahead, 16 bytes per lane, whole
-//                128-byte rows) to f16 in the swizzled layout that the MMAs read
+//   warp 2       Q of the next item by TMA as soon as the last S of the current one has been computed (by ordinary loads,
+//                one warp takes 12 us for the 64 KiB, eight warps 7)
+//   warp 3       the next item; 16-bit: zeroes the value rows of edge tiles that no row sees; 8-bit: helps to convert Q
+//   warps 4-7    softmax of tile A, warps 8-11 of tile B: one row per thread.  They read the 128 scores once, write P back
+//                over the score columns in two halves of 64 keys, and store the rows at the end; the accumulator is
+//                rescaled only when the running maximum grew by more than 2^8
+//   warps 12-15  8-bit: widen the codes of a tile to f16 in the swizzled layout that the MMAs read
 // TMEM: S_A 0..127, S_B 128..255 (P overlays the first 64 columns of each), O_A 256..383, O_B 384..511.
 //
-// 8-bit cache: f16 operands whatever the type of Q (E4M3 fits f16 exactly; Q under a power of two of its row's maximum).
-// Scales cost nothing per element: the key scale of 64 keys is part of the factor that the scores are multiplied by
-// anyway, log2 of the value scale part of the offset that is subtracted anyway (P carries the value scale), and the row
-// sum of 64 keys is divided by it once.
+// 8-bit cache: f16 operands whatever the type of Q (E4M3 fits f16 exactly; bf16 rows of Q go to f16 under a power of two of
+// their maximum).  Scales cost nothing per element: the key scale of 64 keys is part of the factor that the scores are
+// multiplied by anyway, log2 of the value scale part of the offset that is subtracted anyway (P carries the value scale),
+// and the row sum of 64 keys is divided by it once.
 //
-// Values that no row of the CTA sees are zeroed on their way (a probability of 0 times a NaN of stale memory is not 0);
+// Values that no row of the item sees are zeroed on their way (a probability of 0 times a NaN of stale memory is not 0);
 // a row that comes out non-finite because of a value that only other rows of its tile see is computed again from its own
 // keys.
 //
-// Few row tiles and many keys: the keys are split over the CTAs of a cluster, whose partial results meet in shared memory.
+// Few items and many keys: the keys are split over the CTAs of a cluster (one item each), whose partial results meet in
+// shared memory.
 #include <algorithm>
 #include <type_traits>
 
@@ -40,15 +48,30 @@ constexpr uint32_t S_COL = 0, O_COL = 256;                // + 128 * row tile
 constexpr int SOFTMAX_WARP = 4, WIDEN_WARP = 12;
 constexpr int PART_ROW = 132;                             // floats of a parked row: 16-byte lanes of 8 rows hit all banks
 constexpr int CODES = 128 * 128;                          // E4M3 codes of a tile
-// Q_A Q_B | K0 K1 | V0 V1 (at the end: parked rows) | 8-bit: codes of a key and of a value tile | barriers | scales
-template <bool KV8> constexpr size_t smem_bytes() { return 1024 + 6 * (size_t)TILE + (KV8 ? 2 * CODES : 0) + 512; }
+// Q_A Q_B | K0 K1 | V0 V1 (at the end of a split: parked rows) | 8-bit: codes of a key and of a value tile | control
+struct Control {
+    uint64_t q_full, q_empty, q_raw, k_full[2], v_full[2], k_empty[2], v_empty[2], v_raw[2], s_full[2], p_full[4] /* [tile][half] */, o_done[2];
+    uint64_t c_full[4], c_empty[4] /* codes of 64 keys: [keys | values][half] */, item_full[2], item_empty[2], clc_full;
+    uint32_t tmem_base;
+    int abort_word;
+    alignas(16) uint32_t clc[4];
+    alignas(16) int item[2][12];
+    alignas(16) float4 scales[4];                         // of a tile: key scale of either half, log2 of the value scale of either half
+    float2 inv_scales[4];                                 // 1 / value scale of either half
+    int8_t q_shift[2][256];                               // 8-bit: rows of Q are here times 2^shift; by item
+};
+template <bool KV8> constexpr size_t smem_bytes() { return 1024 + 6 * (size_t)TILE + (KV8 ? 2 * CODES : 0) + sizeof(Control); }
 static_assert(256 * PART_ROW * 4 + 2 * 256 * 4 <= 6 * TILE, "parked rows");
 }  // namespace wtile
 
 struct TileParams {
     WinArgs a;
+    CUtensorMap map_q;                                    // {d, head, row}, box {64, group, queries of a tile}
     CUtensorMap map_k, map_v;                             // 16-bit: {d, head, row}, box {64, 1, 128}
     int split;                                            // CTAs of a cluster, each with a range of the key tiles
+    int heads_first;                                      // grid x = K/V heads, y = row tiles (else the other way round)
+    int wide_stores;                                      // rows of the output are 32-byte aligned
+    int bm;                                               // rows of a row tile: whole queries, at most 128
 };
 
 // largest of three, NaN if one is NaN
@@ -75,10 +98,42 @@ __device__ __forceinline__ float ld_cluster_f(uint32_t addr) {
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// 32 bytes of one row
+__device__ __forceinline__ void store32(void *dst, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+// Cluster launch control: asks for a CTA of this grid that has not started; 16 bytes of answer land in shared memory.
+__device__ __forceinline__ void clc_ask(uint32_t *answer, uint64_t *bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+                 "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool clc_answer(const uint32_t *answer, int &x, int &y, int &z) {
+    uint32_t got, cx, cy, cz;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tld.shared.b128 r, [%4];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
+        : "=&r"(got), "=&r"(cx), "=&r"(cy), "=&r"(cz) : "r"(smem_u32(answer)) : "memory");
+    x = (int)cx; y = (int)cy; z = (int)cz;
+    return got != 0;
+}
+
 template <bool KV8> struct TileCfg {
     static constexpr int THREADS = KV8 ? 512 : 384;
-    // 8-bit: 512 threads start with 128 registers each, 72 + 2 * 184 + 72 = 4 * 128; 16-bit: 384 with 168, 88 + 2 * 208 = 3 * 168
-    static constexpr int REG_ISSUE = KV8 ? 72 : 88, REG_SOFTMAX = KV8 ? 184 : 208, REG_WIDEN = 72;
+    // 8-bit: 512 threads start with 128 registers each, 80 + 2 * 184 + 64 = 4 * 128; 16-bit: 384 with 168, 88 + 2 * 208 = 3 * 168
+    static constexpr int REG_ISSUE = KV8 ? 80 : 88, REG_SOFTMAX = KV8 ? 184 : 208, REG_WIDEN = 64;
+    static constexpr int ITEM_READERS = KV8 ? 15 : 11;   // warps 0 to 2, softmax, widening
+};
+
+struct TileItem {
+    int kvh, s, r0, r_end, row0, n, pos0, sink, from, n_kv, t_first, nq;
+    __device__ __forceinline__ int key(int j) const {                    // first key of the j-th tile
+        const int i = t_first + j;
+        return (i < sink ? i : from + i - sink) * wtile::BN;
+    }
+    __device__ __forceinline__ int row_tiles(int bm) const { return r_end - r0 > bm ? 2 : 1; }
 };
 
 // EMU: bit q set = the q-th group of four probabilities of every 32 on the FMA pipe (ex2_emu2)
@@ -87,141 +142,156 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     using namespace wtile;
     using C = TileCfg<KV8>;
     using E = typename std::conditional<KV8, __half, T>::type;          // operand type
+    constexpr bool CONVERT = KV8 && !std::is_same<T, __half>::value;    // Q has to become f16
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sQ = smem, *sK = smem + 2 * TILE, *sV = smem + 4 * TILE, *sC = smem + 6 * TILE;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(sC + (KV8 ? 2 * CODES : 0));
-    uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7, *s_full = bars + 9,
-             *p_full = bars + 11 /* [tile][half] */, *o_done = bars + 15, *v_raw = bars + 16;
-    uint64_t *c_full = bars + 17 /* [keys, values] */, *c_empty = bars + 19;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 21);
-    volatile int *abort_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    float4 *scales = reinterpret_cast<float4 *>(bars + 24);               // [4]: key scale of either half, value scale of either half
+    Control &ctl = *reinterpret_cast<Control *>(sC + (KV8 ? 2 * CODES : 0));
+    volatile int *abort_word = &ctl.abort_word;
 
     const WinArgs &a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)blockIdx.x % p.split, kvh = blockIdx.y, s = blockIdx.z;
-    const SeqExt e = seq_ext<KV8>(a, s);
-    const int r0 = ((int)blockIdx.x / p.split) * (2 * BM);
-    const long long rows_all = (long long)e.nq * a.group;
-    if (r0 >= rows_all) return;                                          // the whole cluster alike
-    const int r_end = (int)(rows_all < r0 + 2 * BM ? rows_all : r0 + 2 * BM);
-    const int n_tiles = r_end - r0 > BM ? 2 : 1;
-    const h3b_win_tiles tiles = h3b_win_tiles_of(a.win, e.pos0 + r0 / a.group, e.pos0 + (r_end - 1) / a.group, e.n, BN);
-    const h3b_win_row row_a = h3b_win_of(a.win, e.pos0 + r0 / a.group, e.n), row_z = h3b_win_of(a.win, e.pos0 + (r_end - 1) / a.group, e.n);
-    const int share = (tiles.count + p.split - 1) / p.split;
-    const int t_first = rank * share, n_kv = max(min(t_first + share, tiles.count) - t_first, 0);
-    auto key_of = [&](int j) { return h3b_win_tile(tiles, t_first + j) * BN; };
-    // no row of the CTA sees key j
-    auto hidden = [&](int j) { return j > row_z.hi || (j < row_a.lo && j >= row_z.s); };
+    const int rank = (int)blockIdx.x % p.split;
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 8);
+        mbar_init(&ctl.q_full, CONVERT ? 2 : 1);
+        mbar_init(&ctl.q_raw, 1);
+        mbar_init(&ctl.q_empty, 1);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&k_full[i], KV8 ? 4 : 1);
-            mbar_init(&v_full[i], KV8 ? 4 : 1);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_empty[i], 1);
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[2 * i], 4);
-            mbar_init(&p_full[2 * i + 1], 4);
+            mbar_init(&ctl.k_full[i], KV8 ? 4 : 1);
+            mbar_init(&ctl.v_full[i], KV8 ? 4 : 1);
+            mbar_init(&ctl.k_empty[i], 1);
+            mbar_init(&ctl.v_empty[i], 1);
+            mbar_init(&ctl.v_raw[i], 1);
+            mbar_init(&ctl.s_full[i], 1);
+            mbar_init(&ctl.o_done[i], 1);
+            mbar_init(&ctl.p_full[2 * i], 4);
+            mbar_init(&ctl.p_full[2 * i + 1], 4);
+            for (int h = 0; h < 4; h += 2) {
+                mbar_init(&ctl.c_full[h + i], 1);
+                mbar_init(&ctl.c_empty[h + i], 4);
+            }
+            mbar_init(&ctl.item_full[i], 1);
+            mbar_init(&ctl.item_empty[i], C::ITEM_READERS);
         }
-        mbar_init(o_done, 1);
-        mbar_init(v_raw, 1);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&c_full[i], 1);
-            mbar_init(&c_empty[i], 4);
-        }
-        *abort_word = 0;
+        mbar_init(&ctl.clc_full, 1);
+        ctl.abort_word = 0;
         mbar_fence_init();
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, TMEM_COLS);
+        tmem_alloc(&ctl.tmem_base, TMEM_COLS);
         tmem_relinquish();
     }
+    // rows behind the whole queries of a tile stay zero
+    for (int i = threadIdx.x; i < 2 * (BM - p.bm) * 16; i += C::THREADS) {
+        const int r = p.bm + (i >> 5), t = i >> 4 & 1, h = i & 15;
+        *reinterpret_cast<uint4 *>(sQ + t * TILE + (h >> 3) * SLAB + r * 128 + (h & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = ctl.tmem_base;
+
+    // every wait: the whole warp together, bounded
+    auto wait = [&](uint64_t *b, uint32_t parity, int code) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, a.status, code)) != 0;
+    };
+    // the k-th item of this CTA; false: no more (or a wait gave up)
+    auto next_item = [&](int k, TileItem &it) -> bool {
+        if (!wait(&ctl.item_full[k & 1], (k >> 1) & 1, H3B_ST_TIMEOUT_OTHER)) return false;
+        const int4 *src = reinterpret_cast<const int4 *>(ctl.item[k & 1]);
+        const int4 x = src[0], y = src[1], z = src[2];
+        it.kvh = x.x; it.s = x.y; it.r0 = x.z; it.r_end = x.w;
+        it.row0 = y.x; it.n = y.y; it.pos0 = y.z; it.sink = y.w;
+        it.from = z.x; it.n_kv = z.y; it.t_first = z.z; it.nq = z.w;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.item_empty[k & 1]);
+        return it.r0 >= 0;
+    };
+    // no row of the item sees key j: j > hi or s <= j < lo
+    auto seen_by_any = [&](const TileItem &it, int &hi, int &lo, int &sn) {
+        const h3b_win_row ra = h3b_win_of(a.win, it.pos0 + it.r0 / a.group, it.n), rz = h3b_win_of(a.win, it.pos0 + (it.r_end - 1) / a.group, it.n);
+        hi = rz.hi; lo = ra.lo; sn = rz.s;
+    };
+    // a tile has such keys among those that exist (16-bit: what lies behind the last key comes as zeros)
+    auto edge = [&](int key, int end, int hi, int lo, int sn) { return min(key + BN, end) - 1 > hi || max(key, sn) < min(key + BN, lo); };
     bool ok = true;
 
     if (warp < SOFTMAX_WARP) {
         regs_dec<C::REG_ISSUE>();
-        if (warp == 0 && !KV8) {
-            // ------------------------------------------------------------ K and V by TMA
-            uint32_t raw = 0;
-            for (int j = 0; j < n_kv && ok; j++) {
-                const int st = j & 1, key = key_of(j);
-                const uint32_t ph = ((j >> 1) & 1) ^ 1;
-                ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
-                if (!ok) break;
-                if (lane == 0) {
-                    mbar_expect_tx(&k_full[st], TILE);
-                    tma_load_3d(sK + st * TILE, &p.map_k, &k_full[st], 0, kvh, key);
-                    tma_load_3d(sK + st * TILE + SLAB, &p.map_k, &k_full[st], 64, kvh, key);
-                }
-                ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
-                if (!ok) break;
-                // keys of the tile that no row sees (those behind the last key come as zeros)
-                const int key_end = min(key + BN, e.n);
-                const bool unseen = key_end - 1 > row_z.hi || (max(key, row_z.s) < min(key_end, row_a.lo));
-                if (lane == 0) {
-                    uint64_t *b = unseen ? v_raw : &v_full[st];
-                    mbar_expect_tx(b, TILE);
-                    tma_load_3d(sV + st * TILE, &p.map_v, b, 0, kvh, key);
-                    tma_load_3d(sV + st * TILE + SLAB, &p.map_v, b, 64, kvh, key);
-                }
-                if (unseen) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(v_raw, raw & 1, abort_word, a.status, H3B_ST_TIMEOUT_FULL));
-                    if (!ok) break;
-                    raw++;
-                    for (int i = lane; i < BN; i += 32)
-                        if (hidden(key + i))
-                            for (int c = 0; c < 16; c++)
-                                *reinterpret_cast<uint4 *>(sV + st * TILE + (c >> 3) * SLAB + i * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&v_full[st]);
-                }
-            }
-        } else if (warp == 0 && n_kv > 0) {
-            // ------------------------------------------------------------ codes of the pages by bulk copies, 64 tokens each
-            // (8 KiB that lie together).  Lanes look up the blocks of 16 tiles at a time.
-            int look = 0, bi = -1;
-            float bks = 1.0f, bvs = 1.0f;
-            for (int j = 0; j < n_kv && ok; j++) {
-                if (j % 16 == 0) {
-                    look = j;
-                    bi = -1;
-                    const int jj = j + (lane >> 1);
-                    if (jj < n_kv) {
-                        const int blk = key_of(jj) / KV8_BLOCK + (lane & 1);
-                        if (blk * KV8_BLOCK < e.n) bi = (int)kv8_block_index(a, s, blk, kvh);
+        TileItem it;
+        if (warp == 0) {
+            // ------------------------------------------------------------ K and V
+            int c = 0;                                                   // tiles so far
+            for (int k = 0; ok && next_item(k, it); k++) {
+                if (!KV8) {
+                    int hi, lo, sn;
+                    seen_by_any(it, hi, lo, sn);
+                    for (int j = 0; j < it.n_kv && ok; j++, c++) {
+                        const int st = c & 1, key = it.key(j);
+                        const uint32_t ph = ((c >> 1) & 1) ^ 1;
+                        ok = wait(&ctl.k_empty[st], ph, H3B_ST_TIMEOUT_EMPTY);
+                        if (!ok) break;
+                        if (lane == 0) {
+                            mbar_expect_tx(&ctl.k_full[st], TILE);
+                            tma_load_3d(sK + st * TILE, &p.map_k, &ctl.k_full[st], 0, it.kvh, key);
+                            tma_load_3d(sK + st * TILE + SLAB, &p.map_k, &ctl.k_full[st], 64, it.kvh, key);
+                        }
+                        ok = wait(&ctl.v_empty[st], ph, H3B_ST_TIMEOUT_EMPTY);
+                        if (!ok) break;
+                        if (lane == 0) {                                 // edge tiles pass through warp 3
+                            uint64_t *b = edge(key, it.n, hi, lo, sn) ? &ctl.v_raw[st] : &ctl.v_full[st];
+                            mbar_expect_tx(b, TILE);
+                            tma_load_3d(sV + st * TILE, &p.map_v, b, 0, it.kvh, key);
+                            tma_load_3d(sV + st * TILE + SLAB, &p.map_v, b, 64, it.kvh, key);
+                        }
                     }
-                    bks = bi >= 0 ? __ldg(a.ks + bi) : 1.0f;
-                    bvs = bi >= 0 ? __ldg(a.vs + bi) : 1.0f;
-                }
-                const int src = 2 * (j - look);
-                const int b0 = __shfl_sync(0xffffffffu, bi, src), b1 = __shfl_sync(0xffffffffu, bi, src + 1);
-                const float4 sc = make_float4(__shfl_sync(0xffffffffu, bks, src), __shfl_sync(0xffffffffu, bks, src + 1),
-                                              __shfl_sync(0xffffffffu, bvs, src), __shfl_sync(0xffffffffu, bvs, src + 1));
+                } else {
+                    // 64 tokens of a head lie together (8 KiB) and are asked for as soon as the widening warps are through with
+                    // the same quarter of the tile before.  Lanes look up the blocks of 16 tiles at a time.
+                    int bi = -1;
+                    float bks = 1.0f, blvs = 0.0f, bivs = 1.0f;
+                    for (int j = 0; j < it.n_kv && ok; j++, c++) {
+                        if (j % 16 == 0) {
+                            bi = -1;
+                            if (j + (lane >> 1) < it.n_kv) {
+                                const int blk = it.key(j + (lane >> 1)) / KV8_BLOCK + (lane & 1);
+                                if (blk * KV8_BLOCK < it.n) bi = (int)kv8_block_index(a, it.s, blk, it.kvh);
+                            }
+                            bks = bi >= 0 ? __ldg(a.ks + bi) : 1.0f;
+                            const float vs = bi >= 0 ? __ldg(a.vs + bi) : 1.0f;
+                            blvs = log2f(vs);
+                            bivs = 1.0f / vs;
+                        }
+                        const int src = 2 * (j % 16);
+                        const int b[2] = {__shfl_sync(0xffffffffu, bi, src), __shfl_sync(0xffffffffu, bi, src + 1)};
+                        const float4 sc = make_float4(__shfl_sync(0xffffffffu, bks, src), __shfl_sync(0xffffffffu, bks, src + 1),
+                                                      __shfl_sync(0xffffffffu, blvs, src), __shfl_sync(0xffffffffu, blvs, src + 1));
+                        const float2 isc = make_float2(__shfl_sync(0xffffffffu, bivs, src), __shfl_sync(0xffffffffu, bivs, src + 1));
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&c_empty[w], (j & 1) ^ 1, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
-                    if (!ok) break;
-                    if (lane == 0) {
-                        // scales of tile j: the softmax warps read them behind s_full(j); the slot is that of tile j - 4,
-                        // whose scores were done with before the codes of tile j - 1 could be widened
-                        if (w == 0) scales[j & 3] = sc;
-                        const uint8_t *codes = w ? a.vc : a.kc;
-                        // a block outside the pool (reported) or behind the last token is not read: its rows are hidden or invalid
-                        mbar_expect_tx(&c_full[w], (b0 >= 0 ? CODES / 2 : 0) + (b1 >= 0 ? CODES / 2 : 0));
-                        if (b0 >= 0) bulk_load(sC + w * CODES, codes + (long long)b0 * (CODES / 2), CODES / 2, &c_full[w]);
-                        if (b1 >= 0) bulk_load(sC + w * CODES + CODES / 2, codes + (long long)b1 * (CODES / 2), CODES / 2, &c_full[w]);
+                        for (int w = 0; w < 4 && ok; w++) {
+                            ok = wait(&ctl.c_empty[w], (c & 1) ^ 1, H3B_ST_TIMEOUT_EMPTY);
+                            if (ok && lane == 0) {
+                                // the softmax warps read the scales of tile c behind s_full(c); the slot is that of tile c - 4,
+                                // whose scores were done with before the codes of tile c - 1 could be widened
+                                if (w == 0) {
+                                    ctl.scales[c & 3] = sc;
+                                    ctl.inv_scales[c & 3] = isc;
+                                }
+                                // a block outside the pool (reported) or behind the last token is not read: its rows are invalid or hidden
+                                if (b[w & 1] >= 0) {
+                                    mbar_expect_tx(&ctl.c_full[w], CODES / 2);
+                                    bulk_load(sC + w * (CODES / 2), (w >> 1 ? a.vc : a.kc) + (long long)b[w & 1] * (CODES / 2), CODES / 2, &ctl.c_full[w]);
+                                } else {
+                                    mbar_arrive(&ctl.c_full[w]);
+                                }
+                            }
+                        }
                     }
                 }
             }
-        } else if (warp == 1 && n_kv > 0) {
+        } else if (warp == 1) {
             // ------------------------------------------------------------ MMA issuer
             // The whole warp walks the loop, converged; one lane, elected once, issues every tcgen05 instruction.  The
             // stage barriers of the next iteration are polled behind an issued block, while the queue drains.
@@ -237,10 +307,10 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 const uint32_t d_tmem = tmem_base + S_COL + 128u * t;
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++) {
-                    const uint32_t c = (uint32_t)(k >> 2) * (SLAB >> 4) + (uint32_t)(k & 3) * 2;
-                    if (lead) umma_f16_ss_lh(d_tmem, qa + c, kb + c, DESC_HI, idesc_s, (uint32_t)(k != 0));
+                    const uint32_t x = (uint32_t)(k >> 2) * (SLAB >> 4) + (uint32_t)(k & 3) * 2;
+                    if (lead) umma_f16_ss_lh(d_tmem, qa + x, kb + x, DESC_HI, idesc_s, (uint32_t)(k != 0));
                 }
-                if (lead) tc_commit(&s_full[t]);
+                if (lead) tc_commit(&ctl.s_full[t]);
             };
             auto issue_pv = [&](int t, int stage, int half, bool first) {
                 const uint32_t vb = v_lo0 + (uint32_t)stage * (TILE >> 4);
@@ -250,230 +320,357 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         umma_f16_ts_lh(tmem_base + O_COL + 128u * t, tmem_base + S_COL + 128u * t + (uint32_t)k * 8,
                                        vb + (uint32_t)k * (2048 >> 4), DESC_HI, idesc_o, (uint32_t)(!first || k != 0));
             };
-            auto wait = [&](uint64_t *b, uint32_t parity, int code) {
-                return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, a.status, code)) != 0;
-            };
-            ok = wait(q_full, 0, H3B_ST_TIMEOUT_OTHER) && wait(&k_full[0], 0, H3B_ST_TIMEOUT_FULL);
-            if (ok) {
+            int c = 0, q = 0, pc[2] = {0, 0};                            // tiles, items with keys, tiles of either row tile so far
+            for (int k = 0; ok && next_item(k, it); k++) {
+                const int n_kv = it.n_kv, n_tiles = it.row_tiles(p.bm);
+                if (!n_kv) continue;
+                ok = wait(&ctl.q_full, q & 1, H3B_ST_TIMEOUT_OTHER) && wait(&ctl.k_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL);
+                if (!ok) break;
                 tc_fence_after();
-                for (int t = 0; t < n_tiles; t++) issue_s(t, 0);
-                if (lead) tc_commit(&k_empty[0]);
-                ok = wait(&v_full[0], 0, H3B_ST_TIMEOUT_FULL) && (n_kv < 2 || wait(&k_full[1], 0, H3B_ST_TIMEOUT_FULL));
+                for (int t = 0; t < n_tiles; t++) issue_s(t, c & 1);
+                if (lead) {
+                    tc_commit(&ctl.k_empty[c & 1]);
+                    if (n_kv == 1) tc_commit(&ctl.q_empty);
+                }
+                ok = wait(&ctl.v_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL) &&
+                     (n_kv < 2 || wait(&ctl.k_full[(c + 1) & 1], ((c + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL));
+                auto step = [&](int j, auto stage_c) {
+                    constexpr int st = decltype(stage_c)::value, nx = st ^ 1;
+                    const bool more = j + 1 < n_kv;
+                    for (int t = 0; t < n_tiles && ok; t++) {
+                        const uint32_t ph = (uint32_t)((t ? pc[1] : pc[0]) + j) & 1;
+                        ok = wait(&ctl.p_full[2 * t], ph, H3B_ST_TIMEOUT_OTHER);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_pv(t, st, 0, j == 0);
+                        ok = wait(&ctl.p_full[2 * t + 1], ph, H3B_ST_TIMEOUT_OTHER);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_pv(t, st, 1, false);
+                        if (t == n_tiles - 1 && lead) tc_commit(&ctl.v_empty[st]);
+                        if (more) {
+                            issue_s(t, nx);
+                            if (t == n_tiles - 1 && lead) {
+                                tc_commit(&ctl.k_empty[nx]);
+                                if (j + 2 == n_kv) tc_commit(&ctl.q_empty);   // the last scores of the item
+                            }
+                        }
+                    }
+                    if (ok && more) {
+                        ok = wait(&ctl.v_full[nx], ((c + j + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
+                        if (ok && j + 2 < n_kv) ok = wait(&ctl.k_full[st], ((c + j + 2) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
+                        tc_fence_after();
+                    }
+                };
+                for (int j = 0; ok && j < n_kv; j++) {
+                    if ((c + j) & 1) step(j, std::integral_constant<int, 1>{});
+                    else step(j, std::integral_constant<int, 0>{});
+                }
+                for (int t = 0; t < n_tiles; t++)
+                    if (lead) tc_commit(&ctl.o_done[t]);
+                c += n_kv;
+                q++;
+                pc[0] += n_kv;
+                if (n_tiles == 2) pc[1] += n_kv;
             }
-            auto step = [&](int j, auto stage_c) {
-                constexpr int st = decltype(stage_c)::value, nx = st ^ 1;
-                const bool more = j + 1 < n_kv;
-                for (int t = 0; t < n_tiles && ok; t++) {
-                    ok = wait(&p_full[2 * t], j & 1, H3B_ST_TIMEOUT_OTHER);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_pv(t, st, 0, j == 0);
-                    ok = wait(&p_full[2 * t + 1], j & 1, H3B_ST_TIMEOUT_OTHER);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_pv(t, st, 1, false);
-                    if (t == n_tiles - 1 && lead) tc_commit(&v_empty[st]);
-                    if (more) {
-                        issue_s(t, nx);
-                        if (t == n_tiles - 1 && lead) tc_commit(&k_empty[nx]);
+        } else {
+            // ------------------------------------------------------------ Q, items, value rows that nobody sees
+            // Q of the q-th item with keys (warp 2)
+            auto load_q = [&](const TileItem &x, int q) -> bool {
+                if (!wait(&ctl.q_empty, (q & 1) ^ 1, H3B_ST_TIMEOUT_EMPTY)) return false;
+                if (lane == 0) {
+                    uint64_t *b = CONVERT ? &ctl.q_raw : &ctl.q_full;
+                    const int n = x.row_tiles(p.bm);
+                    mbar_expect_tx(b, (uint32_t)(n * p.bm * 256));
+                    for (int t = 0; t < n; t++) {
+                        const int row = x.row0 + (x.r0 + t * p.bm) / a.group;
+                        tma_load_3d(sQ + t * TILE, &p.map_q, b, 0, x.kvh * a.group, row);
+                        tma_load_3d(sQ + t * TILE + SLAB, &p.map_q, b, 64, x.kvh * a.group, row);
                     }
                 }
-                if (ok && more) {
-                    ok = wait(&v_full[nx], ((j + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
-                    if (ok && j + 2 < n_kv) ok = wait(&k_full[st], ((j + 2) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
-                    tc_fence_after();
-                }
+                __syncwarp();
+                return true;
             };
-            for (int j = 0; ok && j < n_kv; j += 2) {
-                step(j, std::integral_constant<int, 0>{});
-                if (ok && j + 1 < n_kv) step(j + 1, std::integral_constant<int, 1>{});
+            // bf16 rows to f16 under a power of two of their maximum, which the softmax undoes; sixteen lanes per row, every
+            // other pair of rows is this warp's
+            auto convert_q = [&](const TileItem &x, int q) -> bool {
+                if (!wait(&ctl.q_raw, q & 1, H3B_ST_TIMEOUT_FULL)) return false;
+                const int sub = lane >> 4, ch = lane & 15, tiles = x.row_tiles(p.bm);
+                for (int t = 0; t < tiles; t++) {
+                    uint8_t *base = sQ + t * TILE + (ch >> 3) * SLAB;
+#pragma unroll 4
+                    for (int r0 = 2 * (warp & 1); r0 < BM; r0 += 4) {
+                        const int r = r0 + sub;
+                        uint4 *at = reinterpret_cast<uint4 *>(base + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                        const uint4 w = *at;
+                        uint32_t top = abs_max8<T>(w);
+#pragma unroll
+                        for (int y = 1; y < 16; y <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, y));
+                        const uint32_t bits = widen_abs<T>(top);
+                        int sh = 14 - ((int)(bits >> 23) - 127);
+                        sh = bits >= 0x7f800000u || bits == 0u ? 0 : max(min(sh, 120), -120);   // not finite: as it is
+                        const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+                        uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            v[i] = Elem<__half>::pack(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
+                        *at = make_uint4(v[0], v[1], v[2], v[3]);
+                        if (ch == 0) ctl.q_shift[q & 1][t * BM + r] = (int8_t)sh;
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl.q_full);
+                return true;
+            };
+            int q = 0;
+            if (warp == 2) {
+                for (int k = 0; ok && next_item(k, it); k++)
+                    if (it.n_kv) {
+                        ok = load_q(it, q) && (!CONVERT || convert_q(it, q));
+                        q++;
+                    }
+            } else {
+                // item k of the CTA; `more`: there may be another
+                auto publish = [&](int k, const TileItem &x) -> bool {
+                    if (!wait(&ctl.item_empty[k & 1], ((k >> 1) & 1) ^ 1, H3B_ST_TIMEOUT_EMPTY)) return false;
+                    if (lane == 0) {
+                        int4 *dst = reinterpret_cast<int4 *>(ctl.item[k & 1]);
+                        dst[0] = make_int4(x.kvh, x.s, x.r0, x.r_end);
+                        dst[1] = make_int4(x.row0, x.n, x.pos0, x.sink);
+                        dst[2] = make_int4(x.from, x.n_kv, x.t_first, x.nq);
+                        mbar_arrive(&ctl.item_full[k & 1]);
+                    }
+                    return true;
+                };
+                // what the CTA at (x, y, z) of the grid has to do; false: nothing
+                auto describe = [&](int x, int y, int z, TileItem &d) -> bool {
+                    const SeqExt e = seq_ext<KV8>(a, z);
+                    // late rows first: under a window that is open to the left they see the most
+                    const int row_tile = p.heads_first ? (int)gridDim.y - 1 - y : ((int)gridDim.x - 1 - x) / p.split;
+                    d.kvh = p.heads_first ? x : y;
+                    d.s = z;
+                    d.r0 = row_tile * (2 * p.bm);
+                    const long long rows = (long long)e.nq * a.group;
+                    if (d.r0 >= rows) return false;
+                    d.r_end = (int)(rows < d.r0 + 2 * p.bm ? rows : d.r0 + 2 * p.bm);
+                    d.row0 = e.row0; d.n = e.n; d.pos0 = e.pos0; d.nq = e.nq;
+                    const h3b_win_tiles w = h3b_win_tiles_of(a.win, e.pos0 + d.r0 / a.group, e.pos0 + (d.r_end - 1) / a.group, e.n, BN);
+                    const int share = (w.count + p.split - 1) / p.split;
+                    d.sink = w.sink; d.from = w.from;
+                    d.t_first = rank * share;
+                    d.n_kv = max(min(d.t_first + share, w.count) - d.t_first, 0);
+                    return true;
+                };
+                int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z, asked = 0;
+                bool more = p.split == 1;
+                // the next item with rows in `d`; r0 = -1: none
+                auto find = [&](bool own, TileItem &d) -> bool {
+                    d.r0 = -1;
+                    if (own && describe(x, y, z, d)) return true;
+                    d.r0 = -1;
+                    while (more) {
+                        if (lane == 0) {
+                            mbar_expect_tx(&ctl.clc_full, 16);
+                            clc_ask(ctl.clc, &ctl.clc_full);
+                        }
+                        if (!wait(&ctl.clc_full, asked & 1, H3B_ST_TIMEOUT_OTHER)) return false;
+                        asked++;
+                        more = clc_answer(ctl.clc, x, y, z);
+                        fence_proxy_async_smem();                        // the next answer comes behind this reading
+                        __syncwarp();
+                        if (more && describe(x, y, z, d)) return true;
+                        d.r0 = -1;
+                    }
+                    return true;
+                };
+                int c = 0, raw[2] = {0, 0};
+                ok = find(true, it) && publish(0, it);
+                for (int k = 1; ok && it.r0 >= 0; k++) {
+                    TileItem nx;
+                    ok = find(false, nx) && publish(k, nx);
+                    if (!ok) break;
+                    if (CONVERT) {
+                        if (it.n_kv) ok = convert_q(it, q++);
+                    } else if (!KV8) {
+                        int hi, lo, sn;
+                        seen_by_any(it, hi, lo, sn);
+                        for (int j = 0; j < it.n_kv && ok; j++, c++) {
+                            const int st = c & 1, key = it.key(j);
+                            if (!edge(key, it.n, hi, lo, sn)) continue;
+                            ok = wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1, H3B_ST_TIMEOUT_FULL);
+                            if (!ok) break;
+                            if (st) raw[1]++;
+                            else raw[0]++;
+                            for (int i = lane; i < BN; i += 32)
+                                if (key + i > hi || (key + i < lo && key + i >= sn))
+#pragma unroll
+                                    for (int h = 0; h < 16; h++)
+                                        *reinterpret_cast<uint4 *>(sV + st * TILE + (h >> 3) * SLAB + i * 128 + ((h & 7) ^ (i & 7)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&ctl.v_full[st]);
+                        }
+                    }
+                    it = nx;
+                }
             }
-            if (lead) tc_commit(o_done);
         }
         __syncwarp();
     } else if (warp < WIDEN_WARP) {
         // ---------------------------------------------------------------- softmax
         regs_inc<C::REG_SOFTMAX>();
-        const int t = (warp - SOFTMAX_WARP) >> 2, q = warp & 3;          // row tile, TMEM lane quarter
-        const int my = r0 + t * BM + q * 32 + lane;                      // row of this thread
-        const bool live = my < r_end;
-        const int qi = (live ? my : r_end - 1) / a.group, hd = (live ? my : r_end - 1) - qi * a.group;
-        float row_scale = a.scale_log2;
-        if (t < n_tiles && n_kv) {                                       // without keys the memory is the epilogue's at once
-            // Q -> shared memory, sixteen lanes per 256-byte row (8-bit: f16 under a power of two of the row's maximum,
-            // undone by row_scale)
-            const long long mine = live ? (long long)(e.row0 + qi) * a.q_rs + (long long)(kvh * a.group + hd) * a.q_hs : -1;
-            const int sub = lane >> 4, c = lane & 15;
-            uint4 w[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const long long off = __shfl_sync(0xffffffffu, mine, 2 * i + sub);
-                w[i] = off >= 0 ? __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + off) + c) : make_uint4(0u, 0u, 0u, 0u);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                if (KV8) {
-                    uint32_t top = abs_max8<T>(w[i]);
-#pragma unroll
-                    for (int x = 1; x < 16; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
-                    const uint32_t bits = widen_abs<T>(top);
-                    int sh = 14 - ((int)(bits >> 23) - 127);
-                    sh = bits >= 0x7f800000u || bits == 0u ? 0 : max(min(sh, 120), -120);   // not finite: as it is
-                    const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-                    const int down = __shfl_sync(0xffffffffu, 127 - sh, (lane & 1) * 16);
-                    if ((lane >> 1) == i) row_scale *= __uint_as_float((uint32_t)down << 23);
-                    uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float2 f;
-                        if (Elem<T>::FMT == 1) f = make_float2(__uint_as_float(v[k] << 16), __uint_as_float(v[k] & 0xffff0000u));
-                        else f = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
-                        v[k] = Elem<__half>::pack(f.x * up, f.y * up);
-                    }
-                    w[i] = make_uint4(v[0], v[1], v[2], v[3]);
-                }
-                const int row = q * 32 + 2 * i + sub;
-                *reinterpret_cast<uint4 *>(sQ + t * TILE + (c >> 3) * SLAB + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = w[i];
-            }
-            fence_proxy_async_smem();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-
-        const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+        const int t = (warp - SOFTMAX_WARP) >> 2, quarter = warp & 3;    // row tile, TMEM lane quarter
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem_base + lane_base + S_COL + 128u * t, o_addr = tmem_base + lane_base + O_COL + 128u * t;
-        const h3b_win_row wr = h3b_win_of(a.win, e.pos0 + qi, e.n);
-        const h3b_win_row wa = h3b_win_of(a.win, e.pos0 + (r0 + t * BM) / a.group, e.n);
-        const h3b_win_row wz = h3b_win_of(a.win, e.pos0 + (min(r0 + t * BM + BM, r_end) - 1) / a.group, e.n);
-        float m_run = -INFINITY, l_run = 0.0f;
-        ok = t < n_tiles;
-        for (int j = 0; j < n_kv && ok; j++) {
-            const int key = key_of(j);
-            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, abort_word, a.status, H3B_ST_TIMEOUT_TMEM_FULL));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t sv[BN];
+        TileItem it;
+        int c = 0, mine = 0, q = 0, mine_q = 0;                          // tiles and items with keys so far, and those of this row tile
+        for (int k = 0; ok && next_item(k, it); k++) {
+            const int n_kv = it.n_kv;
+            if (t >= it.row_tiles(p.bm)) {
+                c += n_kv;
+                q += n_kv > 0;
+                continue;
+            }
+            const int slot = t * BM + quarter * 32 + lane;                      // place of this thread's row in the row tiles
+            const int my = it.r0 + t * p.bm + quarter * 32 + lane;              // and the row
+            const bool live = quarter * 32 + lane < p.bm && my < it.r_end;
+            const int qi = (live ? my : it.r_end - 1) / a.group, hd = (live ? my : it.r_end - 1) - qi * a.group;
+            const h3b_win_row wr = h3b_win_of(a.win, it.pos0 + qi, it.n);
+            const h3b_win_row wa = h3b_win_of(a.win, it.pos0 + (it.r0 + t * p.bm) / a.group, it.n);
+            const h3b_win_row wz = h3b_win_of(a.win, it.pos0 + (min(it.r0 + (t + 1) * p.bm, it.r_end) - 1) / a.group, it.n);
+            float m_run = -INFINITY, l_run = 0.0f, row_scale = a.scale_log2;
+            for (int j = 0; j < n_kv; j++) {
+                const int key = it.key(j);
+                ok = wait(&ctl.s_full[t], (mine + j) & 1, H3B_ST_TIMEOUT_TMEM_FULL);
+                if (!ok) break;
+                if (CONVERT && j == 0) row_scale *= __uint_as_float((uint32_t)(127 - ctl.q_shift[q & 1][slot]) << 23);
+                tc_fence_after();
+                uint32_t sv[BN];
 #pragma unroll
-            for (int ch = 0; ch < BN / 32; ch++) tmem_ld_32x32b_x32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[ch * 32]));
-            tmem_ld_wait();
-            if (!h3b_win_full(wa, wz, key, BN)) {
+                for (int ch = 0; ch < BN / 32; ch++) tmem_ld_32x32b_x32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[ch * 32]));
+                tmem_ld_wait();
+                if (!h3b_win_full(wa, wz, key, BN)) {
 #pragma unroll
-                for (int ch = 0; ch < BN / 32; ch++) {
-                    // bits of the 32 keys that the row sees
-                    const int b = wr.hi - key - ch * 32, lo = wr.lo - key - ch * 32, sn = wr.s - key - ch * 32;
-                    const uint32_t upto = b >= 31 ? 0xffffffffu : b < 0 ? 0u : (2u << b) - 1u;
-                    const uint32_t from = lo <= 0 ? 0xffffffffu : lo > 31 ? 0u : 0xffffffffu << lo;
-                    const uint32_t sink = sn <= 0 ? 0u : sn > 31 ? 0xffffffffu : (1u << sn) - 1u;
-                    const uint32_t see = upto & (from | sink);
+                    for (int ch = 0; ch < BN / 32; ch++) {
+                        // bits of the 32 keys that the row sees
+                        const int b = wr.hi - key - ch * 32, lo = wr.lo - key - ch * 32, sn = wr.s - key - ch * 32;
+                        const uint32_t upto = b >= 31 ? 0xffffffffu : b < 0 ? 0u : (2u << b) - 1u;
+                        const uint32_t from = lo <= 0 ? 0xffffffffu : lo > 31 ? 0u : 0xffffffffu << lo;
+                        const uint32_t sink = sn <= 0 ? 0u : sn > 31 ? 0xffffffffu : (1u << sn) - 1u;
+                        const uint32_t see = upto & (from | sink);
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (!(see >> i & 1u)) sv[ch * 32 + i] = 0xff800000u;
+                        for (int i = 0; i < 32; i++)
+                            if (!(see >> i & 1u)) sv[ch * 32 + i] = 0xff800000u;
+                    }
                 }
-            }
-            float mxh[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float mxc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < 64; i += 8)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        mxc[c] = max3_nan(mxc[c], __uint_as_float(sv[h * 64 + i + 2 * c]), __uint_as_float(sv[h * 64 + i + 2 * c + 1]));
-                mxh[h] = max3_nan(max3_nan(mxc[0], mxc[1], mxc[2]), mxc[3], mxc[3]);
-            }
-            float f[2] = {row_scale, row_scale}, off[2] = {0.0f, 0.0f}, inv_vs[2] = {1.0f, 1.0f};
-            float mx;
-            if (KV8) {
-                const float4 sc = scales[j & 3];
+                float mxh[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float vs = h ? sc.w : sc.z;
-                    f[h] = row_scale * (h ? sc.y : sc.x);
-                    off[h] = log2f(vs);
-                    inv_vs[h] = 1.0f / vs;
-                    // nothing of the 64 seen: its scales (of another sequence's tokens, or NaN) have no part
-                    if (mxh[h] == -INFINITY) f[h] = 1.0f, off[h] = 0.0f, inv_vs[h] = 1.0f;
-                    mxh[h] = fmaf(mxh[h], f[h], off[h]);
+                    float mxc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 64; i += 8)
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+                            mxc[x] = max3_nan(mxc[x], __uint_as_float(sv[h * 64 + i + 2 * x]), __uint_as_float(sv[h * 64 + i + 2 * x + 1]));
+                    mxh[h] = max3_nan(max3_nan(mxc[0], mxc[1], mxc[2]), mxc[3], mxc[3]);
                 }
-                mx = max3_nan(mxh[0], mxh[1], mxh[1]);
-            } else {
-                mx = max3_nan(mxh[0], mxh[1], mxh[1]) * row_scale;
-            }
-            if (mx != mx) l_run = mx;                                    // undefined, and so is the row from here on
-            const float m_new = fmaxf(m_run, mx);
-            const bool grow = m_new > m_run + 8.0f || (m_run == -INFINITY && m_new > -INFINITY);
-            if (__any_sync(0xffffffffu, grow)) {
-                float alpha = 1.0f;
-                if (grow) {
-                    alpha = m_run == -INFINITY ? 0.0f : ex2_approx(m_run - m_new);
-                    m_run = m_new;
-                    l_run *= alpha;
+                float f[2] = {row_scale, row_scale}, off[2] = {0.0f, 0.0f}, inv_vs[2] = {1.0f, 1.0f};
+                float mx;
+                if (KV8) {
+                    const float4 scl = ctl.scales[(c + j) & 3];
+                    const float2 inv = ctl.inv_scales[(c + j) & 3];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        f[h] = row_scale * (h ? scl.y : scl.x);
+                        off[h] = h ? scl.w : scl.z;
+                        inv_vs[h] = h ? inv.y : inv.x;
+                        // nothing of the 64 seen: its scales (of tokens that others see, perhaps NaN) have no part
+                        if (mxh[h] == -INFINITY) f[h] = 1.0f, off[h] = 0.0f, inv_vs[h] = 1.0f;
+                        mxh[h] = fmaf(mxh[h], f[h], off[h]);
+                    }
+                    mx = max3_nan(mxh[0], mxh[1], mxh[1]);
+                } else {
+                    mx = max3_nan(mxh[0], mxh[1], mxh[1]) * row_scale;
                 }
-                // s_full of tile j came behind the P V product of tile j - 1: the accumulator is at rest
-                if (j > 0) {
+                if (mx != mx) l_run = mx;                                // undefined, and so is the row from here on
+                const float m_new = fmaxf(m_run, mx);
+                const bool grow = m_new > m_run + 8.0f || (m_run == -INFINITY && m_new > -INFINITY);
+                if (__any_sync(0xffffffffu, grow)) {
+                    float alpha = 1.0f;
+                    if (grow) {
+                        alpha = m_run == -INFINITY ? 0.0f : ex2_approx(m_run - m_new);
+                        m_run = m_new;
+                        l_run *= alpha;
+                    }
+                    // s_full of tile j came behind the P V product of tile j - 1: the accumulator is at rest
+                    if (j > 0) {
 #pragma unroll 1
-                    for (int ch = 0; ch < HD / 16; ch++) {
-                        uint32_t o[16];
-                        tmem_ld_32x32b_x16(o_addr + ch * 16, o);
-                        tmem_ld_wait();
+                        for (int ch = 0; ch < HD / 16; ch++) {
+                            uint32_t o[16];
+                            tmem_ld_32x32b_x16(o_addr + ch * 16, o);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_st_32x32b_x16(o_addr + ch * 16, o);
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st_32x32b_x16(o_addr + ch * 16, o);
+                        }
                     }
                 }
-            }
-            const float m_use = m_run == -INFINITY ? 0.0f : m_run;
-            float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
-            auto chunk = [&](int ch, uint32_t (&packed)[16]) {
-                const float fh = f[ch >> 1], c = KV8 ? off[ch >> 1] - m_use : -m_use;
+                const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+                float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+                auto chunk = [&](int ch, uint32_t (&packed)[16]) {
+                    const float fh = f[ch >> 1], cc = KV8 ? off[ch >> 1] - m_use : -m_use;
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    float x0, x1, x2, x3;
-                    fma2(x0, x1, __uint_as_float(sv[ch * 32 + i]), __uint_as_float(sv[ch * 32 + i + 1]), fh, c);
-                    fma2(x2, x3, __uint_as_float(sv[ch * 32 + i + 2]), __uint_as_float(sv[ch * 32 + i + 3]), fh, c);
-                    float p0, p1, p2, p3;
-                    if ((EMU >> (i >> 2)) & 1u) {
-                        ex2_emu2(p0, p1, x0, x1);
-                        ex2_emu2(p2, p3, x2, x3);
-                    } else {
-                        p0 = ex2_approx(x0); p1 = ex2_approx(x1); p2 = ex2_approx(x2); p3 = ex2_approx(x3);
+                    for (int i = 0; i < 32; i += 4) {
+                        float x0, x1, x2, x3;
+                        fma2(x0, x1, __uint_as_float(sv[ch * 32 + i]), __uint_as_float(sv[ch * 32 + i + 1]), fh, cc);
+                        fma2(x2, x3, __uint_as_float(sv[ch * 32 + i + 2]), __uint_as_float(sv[ch * 32 + i + 3]), fh, cc);
+                        float p0, p1, p2, p3;
+                        if ((EMU >> (i >> 2)) & 1u) {
+                            ex2_emu2(p0, p1, x0, x1);
+                            ex2_emu2(p2, p3, x2, x3);
+                        } else {
+                            p0 = ex2_approx(x0); p1 = ex2_approx(x1); p2 = ex2_approx(x2); p3 = ex2_approx(x3);
+                        }
+                        add2(l0, l1, p0, p1);
+                        add2(l2, l3, p2, p3);
+                        packed[i >> 1] = Elem<E>::pack(p0, p1);
+                        packed[(i >> 1) + 1] = Elem<E>::pack(p2, p3);
                     }
-                    add2(l0, l1, p0, p1);
-                    add2(l2, l3, p2, p3);
-                    packed[i >> 1] = Elem<E>::pack(p0, p1);
-                    packed[(i >> 1) + 1] = Elem<E>::pack(p2, p3);
+                };
+                auto hand_over = [&](int half) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl.p_full[2 * t + half]);
+                };
+                uint32_t pk[16];
+                chunk(0, pk);
+                tmem_st_32x32b_x16(s_addr, pk);
+                chunk(1, pk);
+                tmem_st_32x32b_x16(s_addr + 16, pk);
+                if (KV8) {
+                    l_run += ((l0 + l1) + (l2 + l3)) * inv_vs[0];
+                    l0 = l1 = l2 = l3 = 0.0f;
                 }
-            };
-            auto hand_over = [&](int half) {
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
-            };
-            uint32_t pk[16];
-            chunk(0, pk);
-            tmem_st_32x32b_x16(s_addr, pk);
-            chunk(1, pk);
-            tmem_st_32x32b_x16(s_addr + 16, pk);
-            if (KV8) {
-                l_run += ((l0 + l1) + (l2 + l3)) * inv_vs[0];
-                l0 = l1 = l2 = l3 = 0.0f;
+                chunk(2, pk);
+                hand_over(0);
+                tmem_st_32x32b_x16(s_addr + 32, pk);
+                chunk(3, pk);
+                tmem_st_32x32b_x16(s_addr + 48, pk);
+                hand_over(1);
+                l_run += ((l0 + l1) + (l2 + l3)) * (KV8 ? inv_vs[1] : 1.0f);
             }
-            chunk(2, pk);
-            hand_over(0);
-            tmem_st_32x32b_x16(s_addr + 32, pk);
-            chunk(3, pk);
-            tmem_st_32x32b_x16(s_addr + 48, pk);
-            hand_over(1);
-            l_run += ((l0 + l1) + (l2 + l3)) * (KV8 ? inv_vs[1] : 1.0f);
-        }
-        if (t < n_tiles) {
-            if (ok && n_kv) ok = __all_sync(0xffffffffu, mbar_wait(o_done, 0, abort_word, a.status, H3B_ST_TIMEOUT_OTHER));
+            if (ok && n_kv) ok = wait(&ctl.o_done[t], mine_q & 1, H3B_ST_TIMEOUT_OTHER);
+            if (!ok) break;
+            c += n_kv;
+            mine += n_kv;
+            q += n_kv > 0;
+            mine_q += n_kv > 0;
             tc_fence_after();
             const bool seen = live && h3b_win_count(wr) > 0;
             if (p.split > 1) {
                 // this CTA's share of the row: sums as they are, with their maximum and denominator
-                const int slot = t * BM + q * 32 + lane;
                 float *part = reinterpret_cast<float *>(smem) + slot * PART_ROW;
 #pragma unroll 1
                 for (int ch = 0; ch < HD / 32; ch++) {
@@ -490,10 +687,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 ml[2 * BM + slot] = l_run;
             } else {
                 const float inv_l = 1.0f / l_run;
-                // Lane = row here; the rows of the warp are parked in (now free) tile memory and written out sixteen lanes
-                // per 256-byte head slice.
-                constexpr int STG_ROW = 256 + 16;
-                uint8_t *stg = smem + (size_t)(warp - SOFTMAX_WARP) * 32 * STG_ROW;
+                T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.row0 + qi) * a.o_rs + (long long)(it.kvh * a.group + hd) * a.o_hs;
                 bool odd = false;
 #pragma unroll 1
                 for (int ch = 0; ch < HD / 32; ch++) {
@@ -501,36 +695,35 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     tmem_ld_32x32b_x32(o_addr + ch * 32, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint32_t h[4];
+                    for (int i = 0; i < 32; i += 16) {
+                        uint32_t h[8];
 #pragma unroll
-                        for (int u = 0; u < 4; u++) {
+                        for (int u = 0; u < 8; u++) {
                             const float x = __uint_as_float(o[i + 2 * u]) * inv_l, y = __uint_as_float(o[i + 2 * u + 1]) * inv_l;
                             if (!KV8) odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
-                            h[u] = Elem<T>::pack(x, y);
+                            h[u] = seen ? Elem<T>::pack(x, y) : 0u;
                         }
-                        *reinterpret_cast<uint4 *>(stg + lane * STG_ROW + (ch * 32 + i) * 2) =
-                            seen ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(0u, 0u, 0u, 0u);
-                    }
-                }
-                __syncwarp();
-                const int sub = lane >> 4, chunk = lane & 15;
-#pragma unroll
-                for (int k2 = 0; k2 < 16; k2++) {
-                    const int rr = 2 * k2 + sub, row = r0 + t * BM + q * 32 + rr;
-                    if (ok && row < r_end) {
-                        const int qr = row / a.group;
-                        T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qr) * a.o_rs + (long long)(kvh * a.group + row - qr * a.group) * a.o_hs;
-                        *reinterpret_cast<uint4 *>(dst + chunk * 8) = *reinterpret_cast<const uint4 *>(stg + rr * STG_ROW + chunk * 16);
+                        if (live) {
+                            if (p.wide_stores) {
+                                store32(dst + ch * 32 + i, h);
+                            } else {
+                                *reinterpret_cast<uint4 *>(dst + ch * 32 + i) = make_uint4(h[0], h[1], h[2], h[3]);
+                                *reinterpret_cast<uint4 *>(dst + ch * 32 + i + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+                            }
+                        }
                     }
                 }
                 if (!KV8) {
-                    __syncwarp();
-                    uint32_t again = __ballot_sync(0xffffffffu, ok && seen && odd);
-                    while (again) {
-                        const int row = r0 + t * BM + q * 32 + (__ffs(again) - 1);
-                        again &= again - 1;
-                        attn_row_by_warp<T, KV8>(a, s, e, row / a.group, kvh * a.group + row % a.group, lane);
+                    uint32_t again = __ballot_sync(0xffffffffu, seen && odd);
+                    if (again) {
+                        SeqExt e;
+                        e.row0 = it.row0; e.nq = it.nq; e.n = it.n; e.pos0 = it.pos0;
+                        __syncwarp();                                    // the rows written above come first
+                        while (again) {
+                            const int l = __ffs(again) - 1;
+                            again &= again - 1;
+                            attn_row_by_warp<T, KV8>(a, it.s, e, __shfl_sync(0xffffffffu, qi, l), it.kvh * a.group + __shfl_sync(0xffffffffu, hd, l), lane);
+                        }
                     }
                 }
             }
@@ -541,46 +734,53 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         const int w4 = warp - WIDEN_WARP, sub = lane >> 3, piece = lane & 7;   // row within four, 16 codes of the row
         // 16 codes -> 32 bytes: pieces 2 * (piece & 3), + 1 of slab piece >> 2; lanes of the second slab write their second
         // piece first, so that the eight lanes of a row hit all banks
-        const int second = piece >> 2, c = 2 * (piece & 3);
-        auto widen = [&](uint8_t *tile, const uint8_t *codes, int key, bool unseen) {
-            uint4 raw[8];
+        const int second = piece >> 2, pc = 2 * (piece & 3);
+        TileItem it;
+        int c = 0;
+        for (int k = 0; ok && next_item(k, it); k++) {
+            int hi, lo, sn;
+            seen_by_any(it, hi, lo, sn);
+            for (int j = 0; j < it.n_kv && ok; j++, c++) {
+                const int st = c & 1, key = it.key(j);
+                const uint32_t ph = ((c >> 1) & 1) ^ 1;
+                const bool at_edge = edge(key, key + BN, hi, lo, sn);    // stale bytes behind the last token among them
 #pragma unroll
-            for (int i = 0; i < 8; i++) raw[i] = *reinterpret_cast<const uint4 *>(codes + (i * 16 + w4 * 4 + sub) * 128 + piece * 16);
-            if (unseen)
+                for (int w = 0; w < 4 && ok; w++) {                      // keys 0-63, 64-127, values 0-63, 64-127
+                    ok = wait(&ctl.c_full[w], c & 1, H3B_ST_TIMEOUT_FULL) &&
+                         (w & 1 || wait(w ? &ctl.v_empty[st] : &ctl.k_empty[st], ph, H3B_ST_TIMEOUT_EMPTY));
+                    if (!ok) break;
+                    const uint8_t *codes = sC + w * (CODES / 2);
+                    uint8_t *tile = (w >> 1 ? sV : sK) + st * TILE + second * SLAB + (w & 1) * (64 * 128);
+                    uint4 raw[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (hidden(key + i * 16 + w4 * 4 + sub)) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                    for (int i = 0; i < 4; i++) raw[i] = *reinterpret_cast<const uint4 *>(codes + (i * 16 + w4 * 4 + sub) * 128 + piece * 16);
+                    if (at_edge)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int row = i * 16 + w4 * 4 + sub;
-                const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                uint32_t h[8];
+                        for (int i = 0; i < 4; i++) {
+                            const int x = key + (w & 1) * 64 + i * 16 + w4 * 4 + sub;
+                            if (x > hi || (x < lo && x >= sn)) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl.c_empty[w]);         // the codes are in registers
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    h[2 * k] = widen2_e4m3((uint16_t)(v[k] & 0xffffu));
-                    h[2 * k + 1] = widen2_e4m3((uint16_t)(v[k] >> 16));
-                }
-                const uint4 x = make_uint4(h[0], h[1], h[2], h[3]), y = make_uint4(h[4], h[5], h[6], h[7]);
-                uint8_t *dst = tile + second * SLAB + row * 128;
-                *reinterpret_cast<uint4 *>(dst + (((c + second) ^ (row & 7)) << 4)) = second ? y : x;
-                *reinterpret_cast<uint4 *>(dst + (((c + 1 - second) ^ (row & 7)) << 4)) = second ? x : y;
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-        };
-        for (int j = 0; j < n_kv && ok; j++) {
-            const int st = j & 1, key = key_of(j);
-            const uint32_t ph = ((j >> 1) & 1) ^ 1;
-            const bool unseen = hidden(key + BN - 1) || hidden(key) || (key < row_a.lo && key + BN > row_z.s);
+                    for (int i = 0; i < 4; i++) {
+                        const int row = i * 16 + w4 * 4 + sub;
+                        const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                        uint32_t h[8];
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&c_full[w], j & 1, abort_word, a.status, H3B_ST_TIMEOUT_FULL) &&
-                                                 mbar_wait(w ? &v_empty[st] : &k_empty[st], ph, abort_word, a.status, H3B_ST_TIMEOUT_EMPTY));
-                if (!ok) break;
-                widen((w ? sV : sK) + st * TILE, sC + w * CODES, key, unseen);
-                if (lane == 0) {
-                    mbar_arrive(w ? &v_full[st] : &k_full[st]);
-                    mbar_arrive(&c_empty[w]);
+                        for (int u = 0; u < 4; u++) {
+                            h[2 * u] = widen2_e4m3((uint16_t)(v[u] & 0xffffu));
+                            h[2 * u + 1] = widen2_e4m3((uint16_t)(v[u] >> 16));
+                        }
+                        const uint4 x = make_uint4(h[0], h[1], h[2], h[3]), y = make_uint4(h[4], h[5], h[6], h[7]);
+                        *reinterpret_cast<uint4 *>(tile + row * 128 + (((pc + second) ^ (row & 7)) << 4)) = second ? y : x;
+                        *reinterpret_cast<uint4 *>(tile + row * 128 + (((pc + 1 - second) ^ (row & 7)) << 4)) = second ? x : y;
+                    }
+                    if (w & 1) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(w >> 1 ? &ctl.v_full[st] : &ctl.k_full[st]);
+                    }
                 }
             }
         }
@@ -594,18 +794,22 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     }
     if (p.split > 1) {
         // ---- the shares meet: a warp finishes a row, a lane four of its dimensions
+        const int *slot0 = ctl.item[0];                                  // the one item
+        const int kvh = slot0[0], s = slot0[1], r0 = slot0[2], rows = *abort_word ? 0 : slot0[3] - slot0[2];
+        SeqExt e;
+        e.row0 = slot0[4]; e.n = slot0[5]; e.pos0 = slot0[6]; e.nq = slot0[11];
         cluster_sync_all();
         const uint32_t base = smem_u32(smem);
-        const int rows = r_end - r0;
-        for (int r = rank * (C::THREADS / 32) + warp; r < rows; r += p.split * (C::THREADS / 32)) {
+        for (int r = rank * (C::THREADS / 32) + warp; r0 >= 0 && r < rows; r += p.split * (C::THREADS / 32)) {
+            const int slot = r < p.bm ? r : BM + r - p.bm;
             float m = -INFINITY, l = 0.0f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c = 0; c < p.split; c++) m = fmaxf(m, ld_cluster_f(mapa_shared(base, c) + (2 * BM * PART_ROW + r) * 4));
-            for (int c = 0; c < p.split; c++) {
-                const uint32_t peer = mapa_shared(base, c);
-                const float mc = ld_cluster_f(peer + (2 * BM * PART_ROW + r) * 4), lc = ld_cluster_f(peer + (2 * BM * PART_ROW + 2 * BM + r) * 4);
+            for (int i = 0; i < p.split; i++) m = fmaxf(m, ld_cluster_f(mapa_shared(base, i) + (2 * BM * PART_ROW + slot) * 4));
+            for (int i = 0; i < p.split; i++) {
+                const uint32_t peer = mapa_shared(base, i);
+                const float mc = ld_cluster_f(peer + (2 * BM * PART_ROW + slot) * 4), lc = ld_cluster_f(peer + (2 * BM * PART_ROW + 2 * BM + slot) * 4);
                 const float w = mc == -INFINITY ? 0.0f : ex2_approx(mc - m);
-                const float4 x = ld_cluster_f32x4(peer + (r * PART_ROW + lane * 4) * 4);
+                const float4 x = ld_cluster_f32x4(peer + (slot * PART_ROW + lane * 4) * 4);
                 l += lc != lc ? lc : w * lc;
                 v.x += w * x.x; v.y += w * x.y; v.z += w * x.z; v.w += w * x.w;
             }
@@ -650,18 +854,26 @@ int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t 
     TileParams p;
     memset(&p, 0, sizeof(p));
     p.a = a;
+    const CUtensorMapDataType dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int queries = wtile::BM / a.group;
+    p.bm = queries * a.group;
+    if (h3b_encode_tmap_3d(&p.map_q, dt, 2, a.q, 128, a.heads, a.rows, a.q_hs * 2, a.q_rs * 2, 64, a.group, queries, CU_TENSOR_MAP_SWIZZLE_128B))
+        return fail(error, error_size, "windowed attention: cuTensorMapEncodeTiled(Q) failed");
     if (!kv8 && a.lk) {
-        const CUtensorMapDataType dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
         if (h3b_encode_tmap_3d(&p.map_k, dt, 2, a.k, 128, a.kv_heads, a.lk, a.k_hs * 2, a.k_rs * 2, 64, 1, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
             h3b_encode_tmap_3d(&p.map_v, dt, 2, a.v, 128, a.kv_heads, a.lk, a.v_hs * 2, a.v_rs * 2, 64, 1, 128, CU_TENSOR_MAP_SWIZZLE_128B))
             return fail(error, error_size, "sdpa_window: cuTensorMapEncodeTiled failed");
     }
-    const size_t mtiles = ceil_div((size_t)a.max_rows * a.group, 2 * wtile::BM);
+    const size_t mtiles = ceil_div((size_t)a.max_rows, 2 * (size_t)queries);
     const size_t units = mtiles * a.kv_heads * a.n_seq;
-    const size_t tiles = std::max<size_t>(ceil_div(attn_window_keys(a.win, len, std::min<size_t>(a.max_rows, 2 * wtile::BM)), wtile::BN), 1);
+    const size_t tiles = std::max<size_t>(ceil_div(attn_window_keys(a.win, len, std::min<size_t>(a.max_rows, 2 * (size_t)queries)), wtile::BN), 1);
     p.split = units >= (size_t)cuda->sm_count ? 1 : (int)std::min(std::min<size_t>((size_t)cuda->sm_count / units, 8), std::max<size_t>(tiles / 2, 1));
     if (getenv("TILE_SPLIT")) p.split = atoi(getenv("TILE_SPLIT"));
-    const dim3 grid((unsigned)(mtiles * p.split), (unsigned)a.kv_heads, (unsigned)a.n_seq);
+    p.heads_first = getenv("TILE_HF") ? atoi(getenv("TILE_HF")) : 0;
+    if (p.split > 1 || mtiles > 65535) p.heads_first = 0;
+    p.wide_stores = ((uintptr_t)a.out % 32 == 0) && (a.o_rs | a.o_hs) % 16 == 0;
+    const dim3 grid = p.heads_first ? dim3((unsigned)a.kv_heads, (unsigned)mtiles, (unsigned)a.n_seq)
+                                    : dim3((unsigned)(mtiles * p.split), (unsigned)a.kv_heads, (unsigned)a.n_seq);
     if (kv8) return f16 ? launch_tile_t<__half, true>(cuda, p, grid, error, error_size) : launch_tile_t<__nv_bfloat16, true>(cuda, p, grid, error, error_size);
     return f16 ? launch_tile_t<__half, false>(cuda, p, grid, error, error_size) : launch_tile_t<__nv_bfloat16, false>(cuda, p, grid, error, error_size);
 }

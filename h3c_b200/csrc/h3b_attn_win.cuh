@@ -115,7 +115,7 @@ __device__ __forceinline__ float4 codes4(uint32_t w) {
 // One row and head by one warp, from the definition: lane l holds dimensions 4l..4l+3; a key costs one warp-wide sum.
 // Only visible keys are touched, so whatever masked places hold has no part in the result.
 template <typename T, bool KV8>
-__device__ __noinline__ void attn_row_by_warp(const WinArgs &a, int s, const SeqExt e, int row, int head, int lane) {
+__device__ __forceinline__ void attn_row_by_warp(const WinArgs &a, int s, const SeqExt e, int row, int head, int lane) {
     const int kvh = head / a.group;
     const h3b_win_row r = h3b_win_of(a.win, e.pos0 + row, e.n);
     const float4 q = load4(reinterpret_cast<const T *>(a.q) + (long long)(e.row0 + row) * a.q_rs + head * a.q_hs + lane * 4);
