@@ -71,10 +71,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t &r0, uint32_t &r1
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
 }
-// four E4M3 codes -> two pairs of f16 (exact)
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-}
 // transposes an 8x8 matrix of 16-bit values: lane (g, t) has row g, columns 2t, 2t + 1
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t r;
@@ -280,8 +276,8 @@ k_attn_few(const __grid_constant__ FewParams p) {
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             uint32_t a0, a1, a2, a3;
-                            widen4(w[u][0][k], a0, a2);
-                            widen4(w[u][1][k], a1, a3);
+                            widen4_e4m3(w[u][0][k], a0, a2);
+                            widen4_e4m3(w[u][1][k], a1, a3);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) mma16816<E>(sc[i + u][nt], a0, a1, a2, a3, qf[4 * h + k][nt][0], qf[4 * h + k][nt][1]);
                         }
@@ -403,10 +399,10 @@ k_attn_few(const __grid_constant__ FewParams p) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {      // dimensions 4j .. 4j + 3 of the lane's 16: rows g, g + 8 of products 2j, 2j + 1
                     uint32_t lo[4], hi[4];
-                    widen4(__byte_perm(w0[j], w1[j], 0x5140), lo[0], lo[1]);
-                    widen4(__byte_perm(w0[j], w1[j], 0x7362), lo[2], lo[3]);
-                    widen4(__byte_perm(w2[j], w3[j], 0x5140), hi[0], hi[1]);
-                    widen4(__byte_perm(w2[j], w3[j], 0x7362), hi[2], hi[3]);
+                    widen4_e4m3(__byte_perm(w0[j], w1[j], 0x5140), lo[0], lo[1]);
+                    widen4_e4m3(__byte_perm(w0[j], w1[j], 0x7362), lo[2], lo[3]);
+                    widen4_e4m3(__byte_perm(w2[j], w3[j], 0x5140), hi[0], hi[1]);
+                    widen4_e4m3(__byte_perm(w2[j], w3[j], 0x7362), hi[2], hi[3]);
 #pragma unroll
                     for (int b = 0; b < 2; b++)
 #pragma unroll

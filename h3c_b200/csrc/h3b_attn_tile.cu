@@ -80,11 +80,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ uint32_t widen2_e4m3(uint16_t w) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(w));
-    return r;
-}
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
@@ -122,8 +117,8 @@ __device__ __forceinline__ bool clc_answer(const uint32_t *answer, int &x, int &
 
 template <bool KV8> struct TileCfg {
     static constexpr int THREADS = KV8 ? 512 : 384;
-    // 8-bit: 512 threads start with 128 registers each, 80 + 2 * 184 + 64 = 4 * 128; 16-bit: 384 with 168, 88 + 2 * 208 = 3 * 168
-    static constexpr int REG_ISSUE = KV8 ? 80 : 88, REG_SOFTMAX = KV8 ? 184 : 208, REG_WIDEN = 64;
+    // 8-bit: 512 threads start with 128 registers each, 48 + 2 * 200 + 64 = 4 * 128; 16-bit: 384 with 168, 88 + 2 * 208 = 3 * 168
+    static constexpr int REG_ISSUE = KV8 ? 48 : 88, REG_SOFTMAX = KV8 ? 200 : 208, REG_WIDEN = 64;
     static constexpr int ITEM_READERS = KV8 ? 15 : 11;   // warps 0 to 2, softmax, widening
 };
 
@@ -136,8 +131,7 @@ struct TileItem {
     __device__ __forceinline__ int row_tiles(int bm) const { return r_end - r0 > bm ? 2 : 1; }
 };
 
-// EMU: bit q set = the q-th group of four probabilities of every 32 on the FMA pipe (ex2_emu2)
-template <typename T, bool KV8, uint32_t EMU>
+template <typename T, bool KV8>
 __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __grid_constant__ TileParams p) {
     using namespace wtile;
     using C = TileCfg<KV8>;
@@ -626,13 +620,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         fma2(x0, x1, __uint_as_float(sv[ch * 32 + i]), __uint_as_float(sv[ch * 32 + i + 1]), fh, cc);
                         fma2(x2, x3, __uint_as_float(sv[ch * 32 + i + 2]), __uint_as_float(sv[ch * 32 + i + 3]), fh, cc);
                         float p0, p1, p2, p3;
-                        if ((EMU >> (i >> 2)) & 1u) {
-                            ex2_emu2(p0, p1, x0, x1);
-                            ex2_emu2(p2, p3, x2, x3);
-                        } else {
-                            p0 = ex2_approx(x0); p1 = ex2_approx(x1); p2 = ex2_approx(x2); p3 = ex2_approx(x3);
-                        }
-                        add2(l0, l1, p0, p1);
+                        p0 = ex2_approx(x0); p1 = ex2_approx(x1); p2 = ex2_approx(x2); p3 = ex2_approx(x3);
+                    add2(l0, l1, p0, p1);
                         add2(l2, l3, p2, p3);
                         packed[i >> 1] = Elem<E>::pack(p0, p1);
                         packed[(i >> 1) + 1] = Elem<E>::pack(p2, p3);
@@ -731,10 +720,10 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     } else if (KV8) {
         // ---------------------------------------------------------------- widen the codes of a tile
         regs_dec<C::REG_WIDEN>();
-        const int w4 = warp - WIDEN_WARP, sub = lane >> 3, piece = lane & 7;   // row within four, 16 codes of the row
-        // 16 codes -> 32 bytes: pieces 2 * (piece & 3), + 1 of slab piece >> 2; lanes of the second slab write their second
-        // piece first, so that the eight lanes of a row hit all banks
-        const int second = piece >> 2, pc = 2 * (piece & 3);
+        // Sixteen lanes per row: 8 codes in, one 16-byte piece of the f16 row out; the rows of a lane are 8 apart, so that its
+        // place under the swizzle is the same in all of them.
+        const int row0 = (warp - WIDEN_WARP) * 2 + (lane >> 4), ch = lane & 15;
+        const uint32_t from = (uint32_t)(row0 * 128 + ch * 8), to = (uint32_t)((ch >> 3) * SLAB + row0 * 128 + (((ch & 7) ^ row0) << 4));
         TileItem it;
         int c = 0;
         for (int k = 0; ok && next_item(k, it); k++) {
@@ -744,37 +733,30 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 const int st = c & 1, key = it.key(j);
                 const uint32_t ph = ((c >> 1) & 1) ^ 1;
                 const bool at_edge = edge(key, key + BN, hi, lo, sn);    // stale bytes behind the last token among them
-#pragma unroll
+#pragma unroll 1                                                         // its code has to stay in the instruction caches beside the others'
                 for (int w = 0; w < 4 && ok; w++) {                      // keys 0-63, 64-127, values 0-63, 64-127
                     ok = wait(&ctl.c_full[w], c & 1, H3B_ST_TIMEOUT_FULL) &&
                          (w & 1 || wait(w ? &ctl.v_empty[st] : &ctl.k_empty[st], ph, H3B_ST_TIMEOUT_EMPTY));
                     if (!ok) break;
-                    const uint8_t *codes = sC + w * (CODES / 2);
-                    uint8_t *tile = (w >> 1 ? sV : sK) + st * TILE + second * SLAB + (w & 1) * (64 * 128);
-                    uint4 raw[4];
+                    const uint8_t *codes = sC + w * (CODES / 2) + from;
+                    uint8_t *tile = (w >> 1 ? sV : sK) + st * TILE + (w & 1) * (64 * 128) + to;
+                    uint2 raw[8];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) raw[i] = *reinterpret_cast<const uint4 *>(codes + (i * 16 + w4 * 4 + sub) * 128 + piece * 16);
+                    for (int i = 0; i < 8; i++) raw[i] = *reinterpret_cast<const uint2 *>(codes + i * (8 * 128));
                     if (at_edge)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int x = key + (w & 1) * 64 + i * 16 + w4 * 4 + sub;
-                            if (x > hi || (x < lo && x >= sn)) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                        for (int i = 0; i < 8; i++) {
+                            const int x = key + (w & 1) * 64 + i * 8 + row0;
+                            if (x > hi || (x < lo && x >= sn)) raw[i] = make_uint2(0u, 0u);
                         }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl.c_empty[w]);         // the codes are in registers
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int row = i * 16 + w4 * 4 + sub;
-                        const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                        uint32_t h[8];
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            h[2 * u] = widen2_e4m3((uint16_t)(v[u] & 0xffffu));
-                            h[2 * u + 1] = widen2_e4m3((uint16_t)(v[u] >> 16));
-                        }
-                        const uint4 x = make_uint4(h[0], h[1], h[2], h[3]), y = make_uint4(h[4], h[5], h[6], h[7]);
-                        *reinterpret_cast<uint4 *>(tile + row * 128 + (((pc + second) ^ (row & 7)) << 4)) = second ? y : x;
-                        *reinterpret_cast<uint4 *>(tile + row * 128 + (((pc + 1 - second) ^ (row & 7)) << 4)) = second ? x : y;
+                    for (int i = 0; i < 8; i++) {
+                        uint4 h;
+                        widen4_e4m3(raw[i].x, h.x, h.y);
+                        widen4_e4m3(raw[i].y, h.z, h.w);
+                        *reinterpret_cast<uint4 *>(tile + i * (8 * 128)) = h;
                     }
                     if (w & 1) {
                         fence_proxy_async_smem();
@@ -832,7 +814,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
 }
 
 template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const TileParams &p, dim3 grid, char *error, size_t error_size) {
-    void (*kernel)(const TileParams) = k_attn_tile<T, KV8, 0x11>;
+    void (*kernel)(const TileParams) = k_attn_tile<T, KV8>;
     H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wtile::smem_bytes<KV8>()), "attention smem attribute");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));

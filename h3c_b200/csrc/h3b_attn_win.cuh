@@ -112,6 +112,11 @@ __device__ __forceinline__ float4 codes4(uint32_t w) {
     return make_float4(a.x, a.y, b.x, b.y);
 }
 
+// four E4M3 codes -> two pairs of f16 (exact)
+__device__ __forceinline__ void widen4_e4m3(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+
 // One row and head by one warp, from the definition: lane l holds dimensions 4l..4l+3; a key costs one warp-wide sum.
 // Only visible keys are touched, so whatever masked places hold has no part in the result.
 template <typename T, bool KV8>
