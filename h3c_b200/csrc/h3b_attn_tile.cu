@@ -69,7 +69,8 @@ struct TileParams {
     CUtensorMap map_q;                                    // {d, head, row}, box {64, group, queries of a tile}
     CUtensorMap map_k, map_v;                             // 16-bit: {d, head, row}, box {64, 1, 128}
     int split;                                            // CTAs of a cluster, each with a range of the key tiles
-    int heads_first;                                      // grid x = K/V heads, y = row tiles (else the other way round)
+    int first, row_tiles;                                 // item of the grid's first CTA (cluster); row tiles of a sequence
+    int heads_first;                                      // items run over the K/V heads first, then over the row tiles (else the other way round)
     int wide_stores;                                      // rows of the output are 32-byte aligned
     int bm;                                               // rows of a row tile: whole queries, at most 128
 };
@@ -103,15 +104,15 @@ __device__ __forceinline__ void clc_ask(uint32_t *answer, uint64_t *bar) {
     asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
                  "r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ bool clc_answer(const uint32_t *answer, int &x, int &y, int &z) {
-    uint32_t got, cx, cy, cz;
+__device__ __forceinline__ bool clc_answer(const uint32_t *answer, int &x) {
+    uint32_t got, cx;
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tld.shared.b128 r, [%4];\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b32 y, z;\n\tld.shared.b128 r, [%2];\n\t"
         "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
-        : "=&r"(got), "=&r"(cx), "=&r"(cy), "=&r"(cz) : "r"(smem_u32(answer)) : "memory");
-    x = (int)cx; y = (int)cy; z = (int)cz;
+        "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, _}, r;\n\t}"
+        : "=&r"(got), "=&r"(cx) : "r"(smem_u32(answer)) : "memory");
+    x = (int)cx;
     return got != 0;
 }
 
@@ -437,14 +438,15 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     }
                     return true;
                 };
-                // what the CTA at (x, y, z) of the grid has to do; false: nothing
-                auto describe = [&](int x, int y, int z, TileItem &d) -> bool {
-                    const SeqExt e = seq_ext<KV8>(a, z);
+                // what CTA x of the grid has to do; false: nothing
+                auto describe = [&](int x, TileItem &d) -> bool {
+                    const int i = p.first + x / p.split;
+                    const int in_seq = a.kv_heads * p.row_tiles, j = i % in_seq;
+                    d.s = i / in_seq;
+                    d.kvh = p.heads_first ? j % a.kv_heads : j / p.row_tiles;
                     // late rows first: under a window that is open to the left they see the most
-                    const int row_tile = p.heads_first ? (int)gridDim.y - 1 - y : ((int)gridDim.x - 1 - x) / p.split;
-                    d.kvh = p.heads_first ? x : y;
-                    d.s = z;
-                    d.r0 = row_tile * (2 * p.bm);
+                    d.r0 = (p.row_tiles - 1 - (p.heads_first ? j / a.kv_heads : j % p.row_tiles)) * (2 * p.bm);
+                    const SeqExt e = seq_ext<KV8>(a, d.s);
                     const long long rows = (long long)e.nq * a.group;
                     if (d.r0 >= rows) return false;
                     d.r_end = (int)(rows < d.r0 + 2 * p.bm ? rows : d.r0 + 2 * p.bm);
@@ -456,12 +458,12 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     d.n_kv = max(min(d.t_first + share, w.count) - d.t_first, 0);
                     return true;
                 };
-                int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z, asked = 0;
+                int x = blockIdx.x, asked = 0;
                 bool more = p.split == 1;
                 // the next item with rows in `d`; r0 = -1: none
                 auto find = [&](bool own, TileItem &d) -> bool {
                     d.r0 = -1;
-                    if (own && describe(x, y, z, d)) return true;
+                    if (own && describe(x, d)) return true;
                     d.r0 = -1;
                     while (more) {
                         if (lane == 0) {
@@ -470,10 +472,10 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         }
                         if (!wait(&ctl.clc_full, asked & 1, H3B_ST_TIMEOUT_OTHER)) return false;
                         asked++;
-                        more = clc_answer(ctl.clc, x, y, z);
+                        more = clc_answer(ctl.clc, x);
                         fence_proxy_async_smem();                        // the next answer comes behind this reading
                         __syncwarp();
-                        if (more && describe(x, y, z, d)) return true;
+                        if (more && describe(x, d)) return true;
                         d.r0 = -1;
                     }
                     return true;
@@ -481,16 +483,13 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 int c = 0, raw[2] = {0, 0};
                 ok = find(true, it) && publish(0, it);
                 for (int k = 1; ok && it.r0 >= 0; k++) {
-                    TileItem nx;
-                    ok = find(false, nx) && publish(k, nx);
-                    if (!ok) break;
                     if (CONVERT) {
                         if (it.n_kv) ok = convert_q(it, q++);
                     } else if (!KV8) {
                         int hi, lo, sn;
                         seen_by_any(it, hi, lo, sn);
-                        for (int j = 0; j < it.n_kv && ok; j++, c++) {
-                            const int st = c & 1, key = it.key(j);
+                        for (int j = 0; j < it.n_kv && ok; j++) {
+                            const int st = (c + j) & 1, key = it.key(j);
                             if (!edge(key, it.n, hi, lo, sn)) continue;
                             ok = wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1, H3B_ST_TIMEOUT_FULL);
                             if (!ok) break;
@@ -506,7 +505,14 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                             if (lane == 0) mbar_arrive(&ctl.v_full[st]);
                         }
                     }
-                    it = nx;
+                    // The next item is asked for when the scores of the last tile but one are there, some 5 us before the end:
+                    // early enough for its first tiles, late enough that a CTA with a long item does not hold one back from
+                    // CTAs that are through (asking at the start gave some SMs four items and others one).  No tile of this
+                    // item uses that barrier again, so its phase cannot be missed.
+                    const int last = c + it.n_kv - 2;
+                    if (ok && it.n_kv >= 2) ok = wait(&ctl.k_empty[last & 1], (last >> 1) & 1, H3B_ST_TIMEOUT_EMPTY);
+                    c += it.n_kv;
+                    if (ok) ok = find(false, it) && publish(k, it);
                 }
             }
         }
@@ -813,7 +819,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     }
 }
 
-template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const TileParams &p, dim3 grid, char *error, size_t error_size) {
+template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const TileParams &p, size_t items, char *error, size_t error_size) {
     void (*kernel)(const TileParams) = k_attn_tile<T, KV8>;
     H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wtile::smem_bytes<KV8>()), "attention smem attribute");
     cudaLaunchConfig_t cfg;
@@ -821,7 +827,7 @@ template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const Ti
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)p.split; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3((unsigned)(items * p.split));
     cfg.blockDim = dim3(TileCfg<KV8>::THREADS);
     cfg.dynamicSmemBytes = wtile::smem_bytes<KV8>();
     cfg.stream = cuda->op_stream;
@@ -830,6 +836,18 @@ template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const Ti
     H3B_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, p), "k_attn_tile launch");
     cuda->launches++;
     return 1;
+}
+
+// Clusters of `n` of these CTAs (one per SM) that the chip holds at once: 74, 45, 33, 26, 22, 15, 15 for 2 .. 8 of them
+// on 148 SMs, because a cluster lies within one group of SMs.
+static size_t clusters_of(const h3_cuda *cuda, size_t n) {
+    return n < 3 ? cuda->sm_count / n : n < 7 ? (size_t)cuda->sm_count * 89 / 100 / n : (size_t)cuda->sm_count / 10 + 1;
+}
+// CTAs for each of `items` items that all run at once, at least two key tiles each
+static int split_of(const h3_cuda *cuda, size_t items, size_t tiles) {
+    size_t n = std::min<size_t>(std::max<size_t>(tiles / 2, 1), 8);
+    while (n > 1 && clusters_of(cuda, n) < items) n--;
+    return (int)n;
 }
 
 int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t len, char *error, size_t error_size) {
@@ -846,18 +864,35 @@ int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t 
             h3b_encode_tmap_3d(&p.map_v, dt, 2, a.v, 128, a.kv_heads, a.lk, a.v_hs * 2, a.v_rs * 2, 64, 1, 128, CU_TENSOR_MAP_SWIZZLE_128B))
             return fail(error, error_size, "sdpa_window: cuTensorMapEncodeTiled failed");
     }
-    const size_t mtiles = ceil_div((size_t)a.max_rows, 2 * (size_t)queries);
-    const size_t units = mtiles * a.kv_heads * a.n_seq;
+    const size_t sms = (size_t)cuda->sm_count, row_tiles = ceil_div((size_t)a.max_rows, 2 * (size_t)queries);
+    const size_t items = row_tiles * a.kv_heads * a.n_seq;
+    if (items > 0x7fffffffu / 8) return fail(error, error_size, "windowed attention: shape too large");
     const size_t tiles = std::max<size_t>(ceil_div(attn_window_keys(a.win, len, std::min<size_t>(a.max_rows, 2 * (size_t)queries)), wtile::BN), 1);
-    p.split = units >= (size_t)cuda->sm_count ? 1 : (int)std::min(std::min<size_t>((size_t)cuda->sm_count / units, 8), std::max<size_t>(tiles / 2, 1));
-    if (getenv("TILE_SPLIT")) p.split = atoi(getenv("TILE_SPLIT"));
-    p.heads_first = getenv("TILE_HF") ? atoi(getenv("TILE_HF")) : 0;
-    if (p.split > 1 || mtiles > 65535) p.heads_first = 0;
+    p.row_tiles = (int)row_tiles;
     p.wide_stores = ((uintptr_t)a.out % 32 == 0) && (a.o_rs | a.o_hs) % 16 == 0;
-    const dim3 grid = p.heads_first ? dim3((unsigned)a.kv_heads, (unsigned)mtiles, (unsigned)a.n_seq)
-                                    : dim3((unsigned)(mtiles * p.split), (unsigned)a.kv_heads, (unsigned)a.n_seq);
-    if (kv8) return f16 ? launch_tile_t<__half, true>(cuda, p, grid, error, error_size) : launch_tile_t<__nv_bfloat16, true>(cuda, p, grid, error, error_size);
-    return f16 ? launch_tile_t<__half, false>(cuda, p, grid, error, error_size) : launch_tile_t<__nv_bfloat16, false>(cuda, p, grid, error, error_size);
+    // Heads first puts the long items of all heads in front, which evens out the end (6,144-token frames 238 -> 208 us,
+    // ragged cache 176 -> 152); row tiles first lets neighbours share keys in L2, which matters once all keys together
+    // do not fit it (50,220-token video: 7.98 ms against 8.82).
+    p.heads_first = len * a.n_seq * a.kv_heads * (kv8 ? 256 : 512) <= (128u << 20);
+    int (*launch)(h3_cuda *, const TileParams &, size_t, char *, size_t);
+    if (kv8) launch = f16 ? launch_tile_t<__half, true> : launch_tile_t<__nv_bfloat16, true>;
+    else launch = f16 ? launch_tile_t<__half, false> : launch_tile_t<__nv_bfloat16, false>;
+    // Whole rounds of one item per SM run unsplit; what is left over, if it is less than half a round of one sequence's
+    // long items, has its keys split so that it fills the chip too (a frame of 1,620 queries over 50,220 cached tokens,
+    // 168 items: 1593 us unsplit, 1121 to 1249 split by 3 to 6 as a whole).
+    const size_t rest = items % sms, whole = items - rest;
+    const int n = rest ? split_of(cuda, rest, tiles) : 1;
+    if (whole && (n < 2 || whole > 4 * sms || a.n_seq > 1 || tiles < 32)) {
+        p.split = 1;
+        return launch(cuda, p, items, error, error_size);
+    }
+    if (whole) {
+        p.split = 1;
+        if (!launch(cuda, p, whole, error, error_size)) return 0;
+    }
+    p.first = (int)whole;
+    p.split = n;
+    return !rest || launch(cuda, p, rest, error, error_size);
 }
 
 }  // namespace h3b

@@ -38,7 +38,10 @@ static int fill(WinArgs &a, h3_cuda *cuda, const char *who, int dtype, const voi
 template <bool KV8> static int launch(h3_cuda *cuda, const WinArgs &a, int f16, size_t len, char *error, size_t error_size) {
     DeviceGuard guard(cuda);
     ProfScope prof(cuda, PROF_ATTN);
-    if ((size_t)a.max_rows * a.group <= 64) return launch_attn_few(cuda, a, f16, KV8, len, error, error_size);
+    // 16 rows are one pass of the few-row kernel over the keys.  Measured (us, few-row | tile kernel): 16 rows of 32 streams of
+    // 4,000 cached tokens and 8 heads 78 | 137, 24 rows 158 | 137; 16 rows over 30,000 tokens and 24 heads 66 | 102, 24 rows
+    // 84 | 101, 48 rows 124 | 101; 16-bit 64 | 84, 83 | 84, 97 | 84.
+    if ((size_t)a.max_rows * a.group <= 16) return launch_attn_few(cuda, a, f16, KV8, len, error, error_size);
     return launch_attn_tile(cuda, a, f16, KV8, len, error, error_size);
 }
 
