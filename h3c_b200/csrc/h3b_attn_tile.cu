@@ -54,6 +54,7 @@ struct Control {
     uint64_t c_full[4], c_empty[4] /* codes of 64 keys: [keys | values][half] */, item_full[2], item_empty[2], clc_full;
     uint32_t tmem_base;
     int abort_word;
+    int progress;                                         // tiles whose scores have been asked for
     alignas(16) uint32_t clc[4];
     alignas(16) int item[2][12];
     alignas(16) float4 scales[4];                         // of a tile: key scale of either half, log2 of the value scale of either half
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         }
         mbar_init(&ctl.clc_full, 1);
         ctl.abort_word = 0;
+        ctl.progress = 0;
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -346,6 +348,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         if (more) {
                             issue_s(t, nx);
                             if (t == n_tiles - 1 && lead) {
+                                *reinterpret_cast<volatile int *>(&ctl.progress) = c + j + 2;
                                 tc_commit(&ctl.k_empty[nx]);
                                 if (j + 2 == n_kv) tc_commit(&ctl.q_empty);   // the last scores of the item
                             }
@@ -505,12 +508,23 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                             if (lane == 0) mbar_arrive(&ctl.v_full[st]);
                         }
                     }
-                    // The next item is asked for when the scores of the last tile but one are there, some 5 us before the end:
+                    // The next item is asked for when the scores of the last tile but one have been, some 5 us before the end:
                     // early enough for its first tiles, late enough that a CTA with a long item does not hold one back from
-                    // CTAs that are through (asking at the start gave some SMs four items and others one).  No tile of this
-                    // item uses that barrier again, so its phase cannot be missed.
-                    const int last = c + it.n_kv - 2;
-                    if (ok && it.n_kv >= 2) ok = wait(&ctl.k_empty[last & 1], (last >> 1) & 1, H3B_ST_TIMEOUT_EMPTY);
+                    // CTAs that are through (asking at the start left some SMs with four items and others with one: 174 us
+                    // instead of 133 for the ragged cache).
+                    if (it.n_kv > 2) {
+                        const long long since = clock64();
+                        while (ok && *reinterpret_cast<volatile int *>(&ctl.progress) < c + it.n_kv - 1) {
+                            __nanosleep(100);
+                            if (*abort_word) ok = false;
+                            else if (clock64() - since > H3B_WAIT_CYCLES) {   // as long as any other wait
+                                *abort_word = H3B_ST_TIMEOUT_OTHER;
+                                if (a.status && lane == 0) atomicCAS(a.status, 0, H3B_ST_TIMEOUT_OTHER);
+                                ok = false;
+                            }
+                        }
+                        ok = __all_sync(0xffffffffu, ok) != 0;
+                    }
                     c += it.n_kv;
                     if (ok) ok = find(false, it) && publish(k, it);
                 }
