@@ -78,7 +78,7 @@ class KvCache8:
         for t in (k_scale, v_scale):
             if t.dtype != torch.float32 or not t.is_contiguous():
                 raise H3Error("KvCache8: scales must be contiguous float32")
-        if not (k.device == v.device == k_scale.device == v_scale.device):
+        if not (k.get_device() == v.get_device() == k_scale.get_device() == v_scale.get_device()):
             raise H3Error("KvCache8: the tensors are on different devices")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.c = _l.Kv8Cache(pages, tokens, heads, hd, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
@@ -94,12 +94,14 @@ class Cuda:
         self.h = load().h3_cuda_create(device_index, err, _l.ERR_LEN)
         if not self.h:
             raise H3Error(f"h3_cuda_create: {err.value.decode(errors='replace')}")
-        self.device = torch.device("cuda", device_index)
+        self.device, self._index = torch.device("cuda", device_index), device_index
+        self._raw_stream, self._int32 = torch._C._cuda_getCurrentRawStream, torch.int32
+        self._dt16 = {torch.bfloat16: BF16, torch.float16: F16}
         self.use_stream(torch.cuda.current_stream(self.device))
 
     def use_stream(self, stream):
         call("h3_cuda_set_op_stream", self.h, stream.cuda_stream)
-        self.stream = stream
+        self.stream, self._raw = stream, stream.cuda_stream
 
     def close(self):
         if self.h:
@@ -370,34 +372,37 @@ class Cuda:
 
     def _rows16(self, who, t):
         """(row stride, head stride) of a 16-bit [rows, heads, 128] view on this handle's device."""
-        if t.dim() != 3 or t.shape[2] != 128:
-            raise H3Error(f"{who}: tensors must be [rows, heads, 128], got {tuple(t.shape)}")
-        if t.device != self.device:
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != 128:
+            raise H3Error(f"{who}: tensors must be [rows, heads, 128], got {tuple(shape)}")
+        if t.get_device() != self._index:
             raise H3Error(f"{who}: a tensor is on {t.device}, the handle on {self.device}")
         rs, hs, es = t.stride()
         if es != 1:
             raise H3Error(f"{who}: the last dimension must be contiguous")
-        if t.shape[1] == 1:      # a dimension of one element has no stride of its own
+        if shape[1] == 1:        # a dimension of one element has no stride of its own
             hs = 128
-        if t.shape[0] <= 1:
-            rs = hs * t.shape[1]
+        if shape[0] <= 1:
+            rs = hs * shape[1]
         return rs, hs
+
+    def _on_current_stream(self):
+        return self._raw_stream(self._index) == self._raw
 
     def _out16(self, who, like, inputs, out):
         """The output [rows, heads * 128] and what keeps memory safe when the handle's stream is not the current one:
         new memory comes from the handle's stream, and the caller's tensors are not reused before it is through."""
         import torch
         rows, width = like.shape[0], like.shape[1] * 128
-        now = torch.cuda.current_stream(self.device)
-        if out is not None:
-            if out.shape != (rows, width) or out.dtype != like.dtype or out.device != self.device or (width and out.stride(1) != 1):
-                raise H3Error(f"{who}: out must be [{rows}, {width}] of {like.dtype} on {self.device} with contiguous rows")
-        if now.cuda_stream == self.stream.cuda_stream:
-            return torch.empty((rows, width), dtype=like.dtype, device=self.device) if out is None else out
+        if out is not None and (out.shape != (rows, width) or out.dtype != like.dtype or out.device != self.device or
+                                (width and out.stride(1) != 1)):
+            raise H3Error(f"{who}: out must be [{rows}, {width}] of {like.dtype} on {self.device} with contiguous rows")
+        if self._on_current_stream():
+            return like.new_empty((rows, width)) if out is None else out
         if out is None:
             with torch.cuda.stream(self.stream):
-                out = torch.empty((rows, width), dtype=like.dtype, device=self.device)
-            out.record_stream(now)
+                out = like.new_empty((rows, width))
+            out.record_stream(torch.cuda.current_stream(self.device))
         else:
             out.record_stream(self.stream)
         for t in inputs:
@@ -409,15 +414,16 @@ class Cuda:
         [lk, KV, 128] with H a multiple of KV, all bf16 or all f16 -> [lq, H*128].  Row i stands at p = q_pos + i, in the
         block (frame) that starts at b = p - p % block, and sees key j when j <= b + block - 1 + right and
         (j >= b - left or j < sinks); a negative left or right does not bound that side."""
-        import torch
         (qr, qh), (kr, kh), (vr, vh) = self._rows16("sdpa_window", q), self._rows16("sdpa_window", k), self._rows16("sdpa_window", v)
-        if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype or v.shape != k.shape:
+        dt = self._dt16.get(q.dtype)
+        if dt is None or k.dtype is not q.dtype or v.dtype is not q.dtype or v.shape != k.shape:
             raise H3Error("sdpa_window: q, k, v must all be bf16 or all f16, and v shaped like k")
-        heads, hd = q.shape[1], q.shape[2]
+        lq, heads, hd = q.shape
+        lk, kv_heads, _ = k.shape
         out = self._out16("sdpa_window", q, (q, k, v), out)
-        call("h3b_sdpa_window_dev", self.h, _dt(q), q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, q.shape[0],
-             k.shape[0], heads, k.shape[1], hd, hd ** -0.5 if scale is None else float(scale), q_pos, left, right, sinks, block,
-             out.data_ptr(), out.stride(0) if out.shape[0] > 1 else heads * hd, hd)
+        call("h3b_sdpa_window_dev", self.h, dt, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, lq, lk, heads,
+             kv_heads, hd, hd ** -0.5 if scale is None else scale, q_pos, left, right, sinks, block, out.data_ptr(),
+             out.stride(0) if lq > 1 else heads * hd, hd)
         return out
 
     # ---- paged key/value cache in 8 bits
@@ -432,46 +438,46 @@ class Cuda:
         return KvCache8(k, v, ks, vs)
 
     def _batch(self, who, cache, cu_rows, ext, table):
-        import torch
-        if cache.k.device != self.device:
+        """Checks the sequence tables; (sequences, pages per sequence)."""
+        if cache.k.get_device() != self._index:
             raise H3Error(f"{who}: the cache is on {cache.k.device}, the handle on {self.device}")
-        n = ext.shape[0]
         for t in (cu_rows, ext, table):
-            if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+            if t.dtype is not self._int32 or t.get_device() != self._index or not t.is_contiguous():
                 raise H3Error(f"{who}: cu_rows, lengths and page table must be contiguous int32 on {self.device}")
-        if ext.dim() != 1 or cu_rows.shape != (n + 1,) or table.dim() != 2 or table.shape[0] != n:
+        shape, n = table.shape, len(ext)
+        if ext.dim() != 1 or cu_rows.dim() != 1 or len(cu_rows) != n + 1 or len(shape) != 2 or shape[0] != n:
             raise H3Error(f"{who}: cu_rows [n + 1], lengths [n] and page table [n, pages per sequence] do not fit together")
-        return n
+        return n, shape[1]
 
     def kv8_append(self, cache: KvCache8, k, v, cu_rows, start, table, *, max_rows):
         """Rows cu_rows[s] .. cu_rows[s+1]-1 of k / v [rows, KV, 128] (bf16 or f16) go behind the first start[s] tokens of
         sequence s, whose pages are table[s] (h3b_kv8_append_dev).  max_rows bounds the rows of any one sequence."""
-        import torch
         (kr, kh), (vr, vh) = self._rows16("kv8_append", k), self._rows16("kv8_append", v)
-        if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype or v.shape != k.shape or k.shape[1] != cache.k.shape[1]:
+        dt, shape = self._dt16.get(k.dtype), k.shape
+        if dt is None or v.dtype is not k.dtype or v.shape != shape or shape[1] != cache.c.kv_heads:
             raise H3Error("kv8_append: k and v must be [rows, kv_heads, 128], both bf16 or both f16")
-        n = self._batch("kv8_append", cache, cu_rows, start, table)
-        if torch.cuda.current_stream(self.device).cuda_stream != self.stream.cuda_stream:
+        n, width = self._batch("kv8_append", cache, cu_rows, start, table)
+        if not self._on_current_stream():
             for t in (k, v, cu_rows, start, table, cache.k, cache.v, cache.k_scale, cache.v_scale):
                 t.record_stream(self.stream)
-        call("h3b_kv8_append_dev", self.h, cache.c, _dt(k), k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, k.shape[0], cu_rows.data_ptr(),
-             start.data_ptr(), table.data_ptr(), table.shape[1], n, max_rows)
+        call("h3b_kv8_append_dev", self.h, cache.c, dt, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, shape[0], cu_rows.data_ptr(),
+             start.data_ptr(), table.data_ptr(), width, n, max_rows)
 
     def kv8_sdpa(self, cache: KvCache8, q, cu_rows, lens, table, *, max_rows, max_len, left=-1, right=0, sinks=0, block=1, scale=None,
                  out=None):
         """Attention of q rows [rows, H, 128] (bf16 or f16) over the cache (h3b_kv8_sdpa_dev) -> [rows, H*128].  Sequence s
         has lens[s] tokens in the pages table[s]; its rows cu_rows[s] .. cu_rows[s+1]-1 are the last ones of them.  Windows
         as in sdpa_window (the default is causal).  max_rows bounds the rows of any one sequence, max_len estimates lens."""
-        import torch
         qr, qh = self._rows16("kv8_sdpa", q)
-        if q.dtype not in (torch.bfloat16, torch.float16):
+        dt = self._dt16.get(q.dtype)
+        if dt is None:
             raise H3Error("kv8_sdpa: q must be bf16 or f16")
-        n = self._batch("kv8_sdpa", cache, cu_rows, lens, table)
-        heads, hd = q.shape[1], q.shape[2]
+        n, width = self._batch("kv8_sdpa", cache, cu_rows, lens, table)
+        rows, heads, hd = q.shape
         out = self._out16("kv8_sdpa", q, (q, cu_rows, lens, table, cache.k, cache.v, cache.k_scale, cache.v_scale), out)
-        call("h3b_kv8_sdpa_dev", self.h, cache.c, _dt(q), q.data_ptr(), qr, qh, q.shape[0], cu_rows.data_ptr(), lens.data_ptr(),
-             table.data_ptr(), table.shape[1], n, max_rows, max_len, heads, hd ** -0.5 if scale is None else float(scale), left, right,
-             sinks, block, out.data_ptr(), out.stride(0) if out.shape[0] > 1 else heads * hd, hd)
+        call("h3b_kv8_sdpa_dev", self.h, cache.c, dt, q.data_ptr(), qr, qh, rows, cu_rows.data_ptr(), lens.data_ptr(),
+             table.data_ptr(), width, n, max_rows, max_len, heads, hd ** -0.5 if scale is None else scale, left, right, sinks, block,
+             out.data_ptr(), out.stride(0) if rows > 1 else heads * hd, hd)
         return out
 
     def sdpa_f16_dev(self, q, k, v, scale=None):

@@ -531,7 +531,8 @@ static FewPlan few_plan(const h3_cuda *cuda, size_t units, size_t tiles) {
 template <typename T, bool KV8, bool WIDE> static int launch_few_t(h3_cuda *cuda, const FewParams &p, dim3 grid, int nt, char *error, size_t error_size) {
     void (*kernel)(const FewParams) = nt == 1 ? k_attn_few<T, KV8, 1, WIDE> : k_attn_few<T, KV8, 2, WIDE>;
     using C = few::Cfg<KV8, WIDE>;
-    H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM_BYTES), "attention smem attribute");
+    static std::atomic<uint64_t> done[2];
+    if (!smem_once(cuda, done[nt - 1], (const void *)kernel, C::SMEM_BYTES, "attention smem attribute", error, error_size)) return 0;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attr;

@@ -835,7 +835,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
 
 template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const TileParams &p, size_t items, char *error, size_t error_size) {
     void (*kernel)(const TileParams) = k_attn_tile<T, KV8>;
-    H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wtile::smem_bytes<KV8>()), "attention smem attribute");
+    static std::atomic<uint64_t> done;
+    if (!smem_once(cuda, done, (const void *)kernel, wtile::smem_bytes<KV8>(), "attention smem attribute", error, error_size)) return 0;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attr;

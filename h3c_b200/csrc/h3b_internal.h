@@ -1,6 +1,8 @@
 // Internal declarations shared by the translation units of libh3_b200.so.
 #pragma once
 
+#include <atomic>
+
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
@@ -95,6 +97,16 @@ struct DeviceGuard {
         if (before >= 0) cudaSetDevice(before);
     }
 };
+
+// Dynamic shared memory of a kernel, set once per device (`done`: the kernel's own mask of devices).
+static inline int smem_once(const h3_cuda *c, std::atomic<uint64_t> &done, const void *kernel, size_t bytes, const char *what, char *error,
+                            size_t error_size) {
+    const uint64_t bit = 1ull << (c->device & 63);
+    if (c->device < 64 && (done.load(std::memory_order_relaxed) & bit)) return 1;
+    H3B_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 1;
+}
 
 static inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
 static inline size_t dtype_bytes(int dt) { return dt == H3B_F32 || dt == H3B_I32 ? 4 : 2; }

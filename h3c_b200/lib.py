@@ -7,6 +7,7 @@ library has not been built; there is no fallback.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -316,6 +317,7 @@ _SIGS = {
 }
 
 _lib = None
+_tls = threading.local()   # the message buffer of a host thread
 
 
 def load() -> C.CDLL:
@@ -351,7 +353,10 @@ def ptr(t) -> int | None:
 def call(name: str, *args):
     """Calls an entry point that ends in (error, error_size) and returns 1/0; raises H3Error on 0."""
     lib = load()
-    err = C.create_string_buffer(ERR_LEN)
+    err = getattr(_tls, "err", None)
+    if err is None:
+        err = _tls.err = C.create_string_buffer(ERR_LEN)
+    err[0] = 0
     rc = getattr(lib, name)(*args, err, ERR_LEN)
     if rc != 1:
         raise H3Error(f"{name}: {err.value.decode(errors='replace') or 'failed'}")
