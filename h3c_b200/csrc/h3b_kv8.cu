@@ -10,9 +10,9 @@
 // A block into which a non-finite value is written gets a NaN scale and zero codes: attention over it gives NaN for
 // the rows that see it and nothing else, like the value itself would.
 //
-// h3b_kv8_append_dev: one CTA per (64-token block of the sequence that receives rows, K/V head); 16 lanes hold a row of
-// 128, every thread keeps its four 16-byte pieces of K and of V in registers between the maximum and the conversion:
-// one read, one write, no second pass.
+// h3b_kv8_append_dev: one CTA per (64-token block of the sequence that receives rows, K/V head, K or V); 16 lanes hold a
+// row of 128, every thread keeps its eight 16-byte pieces in registers between the maximum and the conversion: one read,
+// one write, no second pass.
 #include "h3b_attn_win.cuh"
 
 namespace h3b {
@@ -22,7 +22,7 @@ int kv8_cache_ok(const h3b_kv8_cache *c, const char *who, char *error, size_t er
     if (c->head_dim != 128) return fail(error, error_size, "%s: head_dim %zu unsupported (128 only)", who, c->head_dim);
     if (!c->page_tokens || c->page_tokens % KV8_BLOCK || c->page_tokens > 65536)
         return fail(error, error_size, "%s: page_tokens %zu is not a multiple of %d up to 65536", who, c->page_tokens, KV8_BLOCK);
-    if (!c->kv_heads || c->kv_heads > 65535) return fail(error, error_size, "%s: %zu K/V heads", who, c->kv_heads);
+    if (!c->kv_heads || c->kv_heads > 32767) return fail(error, error_size, "%s: %zu K/V heads", who, c->kv_heads);
     if (!c->pages || c->pages >= 0x7fffffffu / c->kv_heads / c->page_tokens)
         return fail(error, error_size, "%s: a pool of %zu pages is not supported (pages * kv_heads * page_tokens < 2^31)", who, c->pages);
     if (!c->d_k || !c->d_v || !c->d_k_scale || !c->d_v_scale) return fail(error, error_size, "%s: NULL cache tensor", who);
@@ -61,9 +61,9 @@ __device__ __forceinline__ float kv8_scale(uint32_t abs_bits) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-template <typename T> __global__ void __launch_bounds__(256) k_kv8_append(const __grid_constant__ AppendArgs a) {
-    __shared__ uint32_t red[2][8];
-    const int s = blockIdx.z, kvh = blockIdx.y, tid = threadIdx.x;
+template <typename T> __global__ void __launch_bounds__(128) k_kv8_append(const __grid_constant__ AppendArgs a) {
+    __shared__ uint32_t red[4];
+    const int s = blockIdx.z, kvh = blockIdx.y >> 1, w = blockIdx.y & 1, tid = threadIdx.x;
     const int r0 = a.cu[s], r1 = a.cu[s + 1], start = a.start[s], nr = r1 - r0;
     if (r0 < 0 || r1 < r0 || r1 > a.rows || nr > a.max_rows || start < 0 ||
         (long long)start + nr > a.table_stride * a.page_blocks * KV8_BLOCK) {
@@ -74,81 +74,64 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv8_append(const 
     const int t0 = blk * KV8_BLOCK;                              // its first token
     const int from = max(start - t0, 0), to = min(start + nr - t0, KV8_BLOCK);   // tokens [from, to) of it are new
     if (from >= to) return;
+    const int sub = tid >> 4, c = tid & 15;                      // row of a pass, 16-byte piece of the row
+    const T *src = reinterpret_cast<const T *>(a.x[w]) + (long long)(r0 + t0 - start) * a.rs[w] + kvh * a.hs[w] + c * 8;
+    uint4 raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int t = i * 8 + sub;
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (t >= from && t < to) raw[i] = __ldg(reinterpret_cast<const uint4 *>(src + t * a.rs[w]));
+    }
+    // the page is looked up while the rows are on their way
     const int pg = blk / a.page_blocks, page = a.table[s * a.table_stride + pg];
     if (page < 0 || page >= a.pages) {
         if (tid == 0 && a.status) atomicCAS(a.status, 0, H3B_ST_EXTENT);
         return;
     }
     const long long bi = ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
-    const int sub = tid >> 4, c = tid & 15;                      // row of a pass, 16-byte piece of the row
-    uint4 raw[2][4];
-    uint32_t top[2] = {0u, 0u};
+    const float before = from > 0 ? a.scales[w][bi] : 0.0f;      // tokens in front of the new ones keep it at least
+    uint32_t top = 0u;
 #pragma unroll
-    for (int w = 0; w < 2; w++)
+    for (int i = 0; i < 8; i++) top = max(top, abs_max8<T>(raw[i]));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((tid & 31) == 0) red[tid >> 5] = top;
+    __syncthreads();                                             // (and every thread has read the old scale)
+    const uint32_t bits = widen_abs<T>(max(max(red[0], red[1]), max(red[2], red[3])));
+    float scale = bits >= 0x7f800000u ? __int_as_float(0x7fffffff) : kv8_scale(bits);
+    if (from > 0 && !(before <= scale)) scale = before != before ? before : (scale != scale ? scale : before);
+    if (tid == 0) a.scales[w][bi] = scale;
+    const bool dead = scale != scale;
+    const float inv = dead ? 0.0f : 1.0f / scale;
+    uint8_t *dst = a.codes[w] + bi * (KV8_BLOCK * 128) + c * 8;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = i * 16 + sub;
-            raw[w][i] = make_uint4(0u, 0u, 0u, 0u);
-            if (t >= from && t < to)
-                raw[w][i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x[w]) +
-                                                                  (long long)(r0 + t0 + t - start) * a.rs[w] + kvh * a.hs[w]) + c);
-        }
+    for (int i = 0; i < 8; i++) {
+        const int t = i * 8 + sub;
+        if (t >= from && t < to) {
+            const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            uint32_t h[4];
 #pragma unroll
-    for (int w = 0; w < 2; w++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) top[w] = max(top[w], abs_max8<T>(raw[w][i]));
-        top[w] = __reduce_max_sync(0xffffffffu, top[w]);
-        if ((tid & 31) == 0) red[w][tid >> 5] = top[w];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 2; w++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) top[w] = max(top[w], red[w][i]);
-        const uint32_t bits = widen_abs<T>(top[w]);
-        const float before = from > 0 ? a.scales[w][bi] : 0.0f;  // tokens in front of the new ones keep it at least
-        float scale = bits >= 0x7f800000u ? __int_as_float(0x7fffffff) : kv8_scale(bits);
-        if (from > 0 && !(before <= scale)) scale = before != before ? before : (scale != scale ? scale : before);
-        __syncthreads();                                         // every thread has read the old scale
-        if (tid == 0) a.scales[w][bi] = scale;
-        const bool dead = scale != scale;
-        const float inv = dead ? 0.0f : 1.0f / scale;
-        uint8_t *dst = a.codes[w] + bi * (KV8_BLOCK * 128);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = i * 16 + sub;
-            if (t >= from && t < to) {
-                const uint32_t v[4] = {raw[w][i].x, raw[w][i].y, raw[w][i].z, raw[w][i].w};
-                uint32_t packed[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    uint32_t out = 0;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t two = v[2 * j + h];
-                        float2 f;
-                        if (Elem<T>::FMT == 1) f = make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
-                        else f = __half22float2(*reinterpret_cast<const __half2 *>(&two));
-                        f.x *= inv;
-                        f.y *= inv;
-                        out |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * h);
-                    }
-                    packed[j] = dead ? 0u : out;
-                }
-                *reinterpret_cast<uint2 *>(dst + t * 128 + c * 8) = make_uint2(packed[0], packed[1]);
-            } else if (t < from && scale != before) {            // codes that are there, under the raised scale
-                uint2 old = *reinterpret_cast<const uint2 *>(dst + t * 128 + c * 8);
-                const float f = before * inv;
-                uint32_t words[2] = {old.x, old.y};
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float4 x = codes4(words[j]);
-                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x.x * f, x.y * f), __NV_SATFINITE, __NV_E4M3);
-                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x.z * f, x.w * f), __NV_SATFINITE, __NV_E4M3);
-                    words[j] = dead ? 0u : lo | hi << 16;
-                }
-                *reinterpret_cast<uint2 *>(dst + t * 128 + c * 8) = make_uint2(words[0], words[1]);
+            for (int j = 0; j < 4; j++) {
+                float2 f;
+                if (Elem<T>::FMT == 1) f = make_float2(__uint_as_float(v[j] << 16), __uint_as_float(v[j] & 0xffff0000u));
+                else f = __half22float2(*reinterpret_cast<const __half2 *>(&v[j]));
+                f.x *= inv;
+                f.y *= inv;
+                h[j] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
             }
+            *reinterpret_cast<uint2 *>(dst + t * 128) = dead ? make_uint2(0u, 0u) : make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+        } else if (t < from && scale != before) {                // codes that are there, under the raised scale
+            uint2 old = *reinterpret_cast<const uint2 *>(dst + t * 128);
+            const float f = before * inv;
+            uint32_t words[2] = {old.x, old.y};
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float4 x = codes4(words[j]);
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x.x * f, x.y * f), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x.z * f, x.w * f), __NV_SATFINITE, __NV_E4M3);
+                words[j] = dead ? 0u : lo | hi << 16;
+            }
+            *reinterpret_cast<uint2 *>(dst + t * 128) = make_uint2(words[0], words[1]);
         }
     }
 }
@@ -187,11 +170,11 @@ int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, con
     a.page_blocks = (int)(cache->page_tokens / KV8_BLOCK);
     a.status = cuda->d_status;
     // max_rows rows that start anywhere in a block reach this many blocks
-    const dim3 grid((unsigned)ceil_div(max_rows + KV8_BLOCK - 1, KV8_BLOCK), (unsigned)cache->kv_heads, (unsigned)n_seq);
+    const dim3 grid((unsigned)ceil_div(max_rows + KV8_BLOCK - 1, KV8_BLOCK), (unsigned)(2 * cache->kv_heads), (unsigned)n_seq);
     DeviceGuard guard(cuda);
     ProfScope prof(cuda, PROF_OTHER);
-    if (dtype == H3B_F16) k_kv8_append<__half><<<grid, 256, 0, cuda->op_stream>>>(a);
-    else k_kv8_append<__nv_bfloat16><<<grid, 256, 0, cuda->op_stream>>>(a);
+    if (dtype == H3B_F16) k_kv8_append<__half><<<grid, 128, 0, cuda->op_stream>>>(a);
+    else k_kv8_append<__nv_bfloat16><<<grid, 128, 0, cuda->op_stream>>>(a);
     cuda->launches++;
     H3B_CUDA_OK(cudaGetLastError(), "k_kv8_append launch");
     return 1;
