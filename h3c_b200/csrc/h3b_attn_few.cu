@@ -33,7 +33,9 @@ template <bool KV8, bool WIDE> struct Cfg {
     static constexpr int U = KV8 ? 64 : 32;         // keys of a tile: 8 KiB of keys, 8 KiB of values
     static constexpr int WARPS = WIDE ? 12 : 4, CTAS = WIDE ? 1 : 3, THREADS = WARPS * 32;
     static constexpr int HALF = U * 128 * (KV8 ? 1 : 2), STAGE = 2 * HALF;         // keys | values
-    static_assert(STAGE >= 16 * 128 * 4, "a warp parks its 16 x 128 sums in its stage at the end");
+    // a warp parks its sums in its stage at the end; pitch and order of a row such that its lanes meet all banks
+    static constexpr int PITCH = KV8 ? 136 : 132;
+    static_assert(STAGE >= 16 * PITCH * 4, "16 parked rows");
     // stages of the warps | partial results of the CTA (16 rows x 128 f32, m, l) | m, l of the warps | barriers
     static constexpr size_t SMEM_BYTES = 1024 + (size_t)WARPS * STAGE + 16 * 128 * 4 + 2 * 16 * 4 + WARPS * 16 * 8 + WARPS * 16 + 64;
 };
@@ -131,7 +133,7 @@ k_attn_few(const __grid_constant__ FewParams p) {
     // ---- copies: lane 0 issues, all lanes together look up 32 tiles at a time
     int look_base = 0;
     int my_row = 0;                                // 8-bit: first row of the tile's codes, -1: page outside the pool
-    float my_ks = 1.0f, my_vs = 1.0f;
+    float my_ks = 1.0f, my_lvs = 0.0f, my_ivs = 1.0f;   // key scale, log2 and inverse of the value scale
     auto look_up = [&](int it0) {
         look_base = it0;
         if (KV8) {
@@ -141,12 +143,14 @@ k_attn_few(const __grid_constant__ FewParams p) {
                 const long long bi = kv8_block_index(a, s, tile * U / KV8_BLOCK, kvh);
                 my_row = bi < 0 ? -1 : (int)(bi * KV8_BLOCK) + tile * U % KV8_BLOCK;
                 my_ks = bi < 0 ? 1.0f : __ldg(a.ks + bi);
-                my_vs = bi < 0 ? 1.0f : __ldg(a.vs + bi);
+                const float vs = bi < 0 ? 1.0f : __ldg(a.vs + bi);
+                my_lvs = log2f(vs);
+                my_ivs = 1.0f / vs;
             }
         }
     };
     int next_row = 0;                              // of the tile whose keys were asked for last
-    float next_ks = 1.0f, next_vs = 1.0f;
+    float next_ks = 1.0f, next_lvs = 0.0f, next_ivs = 1.0f;
     auto copy = [&](int it, int row, int which) {                                  // which: 0 keys, 1 values
         if (lane == 0) {
             uint8_t *dst = stage + which * HALF;
@@ -166,7 +170,8 @@ k_attn_few(const __grid_constant__ FewParams p) {
         if (KV8) {
             next_row = __shfl_sync(0xffffffffu, my_row, it - look_base);
             next_ks = __shfl_sync(0xffffffffu, my_ks, it - look_base);
-            next_vs = __shfl_sync(0xffffffffu, my_vs, it - look_base);
+            next_lvs = __shfl_sync(0xffffffffu, my_lvs, it - look_base);
+            next_ivs = __shfl_sync(0xffffffffu, my_ivs, it - look_base);
         }
         copy(it, next_row, 0);
     };
@@ -247,7 +252,7 @@ k_attn_few(const __grid_constant__ FewParams p) {
 
     for (int it = 0; it < n_it; it++) {
         const int k0 = h3b_win_tile(tiles, first + it * WARPS) * U;
-        const float ks = next_ks, vs = next_vs;
+        const float ks = next_ks, lvs = next_lvs, ivs = next_ivs;
         const bool absent = KV8 && next_row < 0;
         ok = __all_sync(0xffffffffu, mbar_wait(&bar[0], it & 1, abort_word, a.status, H3B_ST_TIMEOUT_FULL));
         if (!ok) break;
@@ -299,31 +304,31 @@ k_attn_few(const __grid_constant__ FewParams p) {
         if (it + 1 < n_it) fetch_keys(it + 1);
 
         // exponents: score * scale (+ log2 of the value scale), masked ones -inf; probabilities
-        const float lvs = KV8 ? log2f(vs) : 0.0f, ivs = KV8 ? 1.0f / vs : 1.0f;
         const bool masked = !h3b_win_full(row_a, row_z, k0, U) || absent;
         uint32_t pf[MT][NT][2];                                                     // P^T as operand: keys 2t.. and 2t + 8..
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             bool grow = false;
-            float top[2];
+            float top[2], f[2], off[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float f = KV8 ? row_scale[nt][j] * ks : row_scale[nt][j];
-                h3b_win_row wr;
-                if (masked) wr = h3b_win_of(a.win, e.pos0 + min(r_first + nt * 8 + 2 * t + j, r_end - 1) / a.group, e.n);
+                if (masked) {
+                    const h3b_win_row wr = h3b_win_of(a.win, e.pos0 + min(r_first + nt * 8 + 2 * t + j, r_end - 1) / a.group, e.n);
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++)
+                            if (!h3b_win_sees(wr, k0 + i * 16 + r * 8 + (KV8 ? swap_g : g)) || absent) sc[i][nt][2 * r + j] = -INFINITY;
+                }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        float x = KV8 ? fmaf(sc[i][nt][2 * r + j], f, lvs) : sc[i][nt][2 * r + j] * f;
-                        if (masked) {
-                            const int key = k0 + i * 16 + r * 8 + (KV8 ? swap_g : g);
-                            if (!h3b_win_sees(wr, key) || absent) x = -INFINITY;
-                        }
-                        sc[i][nt][2 * r + j] = x;
-                        mx = fmaxf(mx, x);
-                    }
+                for (int i = 0; i < MT; i++) mx = fmaxf(mx, fmaxf(sc[i][nt][j], sc[i][nt][2 + j]));
+                // factors are positive: the largest score has the largest exponent
+                f[j] = KV8 ? row_scale[nt][j] * ks : row_scale[nt][j];
+                off[j] = lvs;
+                // a lane that sees nothing of the tile: its scales (perhaps NaN) have no part
+                if (KV8 && mx == -INFINITY) f[j] = 1.0f, off[j] = 0.0f;
+                mx = KV8 ? fmaf(mx, f[j], off[j]) : mx * f[j];
                 top[j] = mx;
                 grow |= mx > m_run[nt][j] + 8.0f || (m_run[nt][j] == -INFINITY && mx > -INFINITY);
             }
@@ -347,13 +352,13 @@ k_attn_few(const __grid_constant__ FewParams p) {
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float m_use = m_run[nt][j] == -INFINITY ? 0.0f : m_run[nt][j];
+                const float m_use = m_run[nt][j] == -INFINITY ? 0.0f : m_run[nt][j], c = (KV8 ? off[j] : 0.0f) - m_use;
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
-                        const float x = ex2_approx(sc[i][nt][2 * r + j] - m_use);
+                        const float x = ex2_approx(fmaf(sc[i][nt][2 * r + j], f[j], c));
                         sc[i][nt][2 * r + j] = x;
                         sum += x;
                     }
@@ -448,16 +453,16 @@ k_attn_few(const __grid_constant__ FewParams p) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 if (KV8) {
-                    *reinterpret_cast<float2 *>(&mine[r * 128 + swap_g * 16 + 2 * i]) = make_float2(o[i][nt][j], o[i][nt][2 + j]);
+                    *reinterpret_cast<float2 *>(&mine[r * C::PITCH + i * 16 + swap_g * 2]) = make_float2(o[i][nt][j], o[i][nt][2 + j]);   // d = 16 swap_g + 2 i, + 1
                 } else {
-                    mine[r * 128 + i * 16 + g] = o[i][nt][j];
-                    mine[r * 128 + i * 16 + g + 8] = o[i][nt][2 + j];
+                    mine[r * C::PITCH + i * 16 + g] = o[i][nt][j];
+                    mine[r * C::PITCH + i * 16 + g + 8] = o[i][nt][2 + j];
                 }
             }
         }
     __syncthreads();
     for (int i = threadIdx.x; i < R * 128; i += C::THREADS) {
-        const int r = i >> 7;
+        const int r = i >> 7, dim = i & 127, at = r * C::PITCH + (KV8 ? ((dim & 14) << 3) + (dim >> 4 << 1) + (dim & 1) : dim);
         float m = -INFINITY, l = 0.0f, v = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; w++) m = fmaxf(m, warp_ml[(w * 16 + r) * 2]);
@@ -467,7 +472,7 @@ k_attn_few(const __grid_constant__ FewParams p) {
             const float c = mw == -INFINITY ? 0.0f : ex2_approx(mw - m);
             // a warp whose l is NaN saw something undefined: it counts even if it has no maximum
             l += lw != lw ? lw : c * lw;
-            v += c * reinterpret_cast<const float *>(smem + w * STAGE)[i];
+            v += c * reinterpret_cast<const float *>(smem + w * STAGE)[at];
         }
         acc[i] = v;
         if ((i & 127) == 0) {
