@@ -122,6 +122,10 @@ k_attn_few(const __grid_constant__ FewParams p) {
 
     uint8_t *stage = smem + warp * STAGE;
     uint64_t *bar = bars + warp * 2;
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&p.map_k);
+        tma_prefetch_desc(&p.map_v);
+    }
     if (lane == 0) {
         mbar_init(&bar[0], 1);
         mbar_init(&bar[1], 1);

@@ -190,6 +190,11 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     tc_fence_after();
     const uint32_t tmem_base = ctl.tmem_base;
 
+    if (threadIdx.x == 32) tma_prefetch_desc(&p.map_q);
+    if (!KV8 && threadIdx.x == 0) {
+        tma_prefetch_desc(&p.map_k);
+        tma_prefetch_desc(&p.map_v);
+    }
     // every wait: the whole warp together, bounded
     auto wait = [&](uint64_t *b, uint32_t parity, int code) -> bool {
         return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, a.status, code)) != 0;
@@ -558,6 +563,12 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 const int key = it.key(j);
                 ok = wait(&ctl.s_full[t], (mine + j) & 1, H3B_ST_TIMEOUT_TMEM_FULL);
                 if (!ok) break;
+                float4 scl;
+                float2 inv;
+                if (KV8) {
+                    scl = ctl.scales[(c + j) & 3];
+                    inv = ctl.inv_scales[(c + j) & 3];
+                }
                 if (CONVERT && j == 0) row_scale *= __uint_as_float((uint32_t)(127 - ctl.q_shift[q & 1][slot]) << 23);
                 tc_fence_after();
                 uint32_t sv[BN];
@@ -573,6 +584,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         const uint32_t from = lo <= 0 ? 0xffffffffu : lo > 31 ? 0u : 0xffffffffu << lo;
                         const uint32_t sink = sn <= 0 ? 0u : sn > 31 ? 0xffffffffu : (1u << sn) - 1u;
                         const uint32_t see = upto & (from | sink);
+                        if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;
 #pragma unroll
                         for (int i = 0; i < 32; i++)
                             if (!(see >> i & 1u)) sv[ch * 32 + i] = 0xff800000u;
@@ -592,8 +604,6 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 float f[2] = {row_scale, row_scale}, off[2] = {0.0f, 0.0f}, inv_vs[2] = {1.0f, 1.0f};
                 float mx;
                 if (KV8) {
-                    const float4 scl = ctl.scales[(c + j) & 3];
-                    const float2 inv = ctl.inv_scales[(c + j) & 3];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         f[h] = row_scale * (h ? scl.y : scl.x);
