@@ -119,6 +119,25 @@ def test_window_over_long_keys(cuda, lq, lk, w, dtype):
     check_window(cuda, q, k, v, q_pos=lk - lq, **w)
 
 
+@pytest.mark.parametrize("lq, lk, heads, kv, w", [
+    (6144, 6144, 24, 24, dict(left=2048, right=0, sinks=1024, block=1024)),     # several items for every SM
+    (1531, 7919, 56, 8, dict(left=1000, right=77, sinks=5)),                     # 126-row tiles, a last round that is partly empty
+    (1620, 9000, 24, 24, dict(left=-1, right=0, block=1620)),                    # whole rounds and a rest whose keys are split
+    (1500, 9000, 3, 1, dict(left=-1, right=0)), (700, 300, 126, 14, dict(left=3, right=3))])
+def test_window_full_size_sampled(cuda, lq, lk, heads, kv, w):
+    g = gen(lq)
+    q, k, v = normal(g, lq, heads, 128, dtype=BF), normal(g, lk, kv, 128, dtype=BF), normal(g, lk, kv, 128, dtype=BF)
+    got = cuda.sdpa_window(q, k, v, q_pos=max(0, lk - lq), **w).view(lq, heads, 128)
+    cuda.check()
+    rows = torch.unique(torch.cat([torch.arange(0, lq, 97, device="cuda"), torch.arange(max(0, lq - 130), lq, 3, device="cuda"),
+                                   torch.arange(0, min(lq, 260), 5, device="cuda")]))
+    seen = mask(rows.cpu().numpy() + max(0, lk - lq), lk, w["left"], w["right"], w.get("sinks", 0), w.get("block", 1))
+    for h in sorted({0, heads // 2, heads - 1}):
+        kv_h = h // (heads // kv)
+        want, a = attend(q[rows, h:h + 1], k[:, kv_h:kv_h + 1], v[:, kv_h:kv_h + 1], seen, 128 ** -0.5)
+        close(got[rows, h], want, a, float(v.float().abs().max()), BF)
+
+
 def test_window_without_bounds_is_the_frameworks_attention(cuda):
     g = gen(3)
     q, k, v = (normal(g, n, 4, 128, dtype=BF) for n in (500, 700, 700))
@@ -464,6 +483,33 @@ def test_cache_attention_of_evicted_pages_and_stale_memory(cuda):
         got = cuda.kv8_sdpa(cache, q, i32(cu), i32([1000, 210]), i32(bad), max_rows=rows, max_len=1000, left=100, sinks=70)
         cuda.check()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows, lens, heads, kv, w", [
+    ([1620], [9000], 24, 24, dict(block=1620)), ([700, 1, 333, 701, 64, 2, 500, 90, 17], [9000, 1000, 333, 8000, 64, 5000, 700, 3000, 2000], 24, 6, dict(left=2047, sinks=64)),
+    ([1] * 64, [100 + 117 * i for i in range(64)], 28, 4, dict()), ([300] * 20, [300 + 50 * i for i in range(20)], 12, 4, dict(left=500))])
+def test_cache_full_size_sampled(cuda, rows, lens, heads, kv, w):
+    rng, g = np.random.default_rng(sum(lens)), gen(sum(lens))
+    pool = sum(-(-n // 64) for n in lens) + 1
+    cache = cuda.kv8_cache(pool, 64, kv)
+    table = pages_of(rng, lens, 64, pool)
+    cu_k = np.concatenate([[0], np.cumsum(lens)])
+    k, v = normal(g, int(cu_k[-1]), kv, 128, dtype=BF), normal(g, int(cu_k[-1]), kv, 128, dtype=BF)
+    cuda.kv8_append(cache, k, v, i32(cu_k), i32([0] * len(lens)), i32(table), max_rows=max(lens))
+    model = Model(cache)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    q = normal(g, int(cu[-1]), heads, 128, dtype=BF)
+    got = cuda.kv8_sdpa(cache, q, i32(cu), i32(lens), i32(table), max_rows=max(rows), max_len=max(lens), **w).view(-1, heads, 128)
+    cuda.check()
+    full = dict(left=-1, right=0, sinks=0, block=1) | w
+    for s, n in enumerate(lens):
+        kk, vv = model.values(s, n, table)
+        pick = torch.unique(torch.cat([torch.arange(0, rows[s], 61, device="cuda"), torch.arange(max(0, rows[s] - 3), rows[s], device="cuda")]))
+        seen = mask(n - rows[s] + pick.cpu().numpy(), n, **full)
+        for h in {s % heads, heads - 1}:
+            kv_h = h // (heads // kv)
+            want, a = attend(q[cu[s]:cu[s + 1]][pick, h:h + 1], kk[:, kv_h:kv_h + 1], vv[:, kv_h:kv_h + 1], seen, 128 ** -0.5)
+            close(got[cu[s]:cu[s + 1]][pick, h], want, a, float(vv.abs().max()), BF, HF)
 
 
 def test_cache_sequences_that_share_pages(cuda):
