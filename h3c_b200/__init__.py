@@ -64,24 +64,28 @@ class KvCache8:
     (or uint8) and f32 scales [pages, kv_heads, page_tokens // 64], value = code * scale.  The tensors stay the
     caller's; `Cuda.kv8_cache` makes new ones.  A page list is an int32 row of page numbers, one per page_tokens."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "c")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "kv_heads", "device_index", "packed")
 
     def __init__(self, k, v, k_scale, v_scale):
-        import torch
-        pages, heads, tokens, hd = shape = k.shape
-        blocks = (pages, heads, tokens // 64)
-        if v.shape != shape or k_scale.shape != blocks or v_scale.shape != blocks:
-            raise H3Error("KvCache8: codes must be [pages, kv_heads, page_tokens, 128], scales [pages, kv_heads, page_tokens // 64]")
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape:
+            raise H3Error("KvCache8: k and v must be [pages, kv_heads, page_tokens, 128]")
+        pages, heads, tokens, hd = shape
+        scales = k_scale.shape
+        if scales != (pages, heads, tokens // 64) or v_scale.shape != scales:
+            raise H3Error("KvCache8: scales must be [pages, kv_heads, page_tokens // 64]")
+        where = k.get_device()
         for t in (k, v):
-            if t.dtype not in (torch.float8_e4m3fn, torch.uint8) or not t.is_contiguous():
+            if str(t.dtype) not in ("torch.float8_e4m3fn", "torch.uint8") or not t.is_contiguous():
                 raise H3Error("KvCache8: codes must be contiguous float8_e4m3fn or uint8")
         for t in (k_scale, v_scale):
-            if t.dtype != torch.float32 or not t.is_contiguous():
+            if str(t.dtype) != "torch.float32" or not t.is_contiguous():
                 raise H3Error("KvCache8: scales must be contiguous float32")
-        if not (k.get_device() == v.get_device() == k_scale.get_device() == v_scale.get_device()):
+        if v.get_device() != where or k_scale.get_device() != where or v_scale.get_device() != where:
             raise H3Error("KvCache8: the tensors are on different devices")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.c = _l.Kv8Cache(pages, tokens, heads, hd, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self.kv_heads, self.device_index = heads, where
+        self.packed = _l.KV8_CACHE.pack(pages, tokens, heads, hd, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
 
 
 class Cuda:
@@ -421,9 +425,10 @@ class Cuda:
         lq, heads, hd = q.shape
         lk, kv_heads, _ = k.shape
         out = self._out16("sdpa_window", q, (q, k, v), out)
-        call("h3b_sdpa_window_dev", self.h, dt, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, lq, lk, heads,
-             kv_heads, hd, hd ** -0.5 if scale is None else scale, q_pos, left, right, sinks, block, out.data_ptr(),
-             out.stride(0) if lq > 1 else heads * hd, hd)
+        call("h3b_sdpa_window_dev", self.h, _l.SDPA_WINDOW_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qr, qh, kr, kh, vr, vh,
+            out.stride(0) if lq > 1 else heads * hd, hd, lq, lk, heads, kv_heads, hd, q_pos, left, right, sinks, block,
+            hd ** -0.5 if scale is None else scale, dt))
         return out
 
     # ---- paged key/value cache in 8 bits
@@ -439,7 +444,7 @@ class Cuda:
 
     def _batch(self, who, cache, cu_rows, ext, table):
         """Checks the sequence tables; (sequences, pages per sequence)."""
-        if cache.k.get_device() != self._index:
+        if cache.device_index != self._index:
             raise H3Error(f"{who}: the cache is on {cache.k.device}, the handle on {self.device}")
         for t in (cu_rows, ext, table):
             if t.dtype is not self._int32 or t.get_device() != self._index or not t.is_contiguous():
@@ -454,14 +459,15 @@ class Cuda:
         sequence s, whose pages are table[s] (h3b_kv8_append_dev).  max_rows bounds the rows of any one sequence."""
         (kr, kh), (vr, vh) = self._rows16("kv8_append", k), self._rows16("kv8_append", v)
         dt, shape = self._dt16.get(k.dtype), k.shape
-        if dt is None or v.dtype is not k.dtype or v.shape != shape or shape[1] != cache.c.kv_heads:
+        if dt is None or v.dtype is not k.dtype or v.shape != shape or shape[1] != cache.kv_heads:
             raise H3Error("kv8_append: k and v must be [rows, kv_heads, 128], both bf16 or both f16")
         n, width = self._batch("kv8_append", cache, cu_rows, start, table)
         if not self._on_current_stream():
             for t in (k, v, cu_rows, start, table, cache.k, cache.v, cache.k_scale, cache.v_scale):
                 t.record_stream(self.stream)
-        call("h3b_kv8_append_dev", self.h, cache.c, dt, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, shape[0], cu_rows.data_ptr(),
-             start.data_ptr(), table.data_ptr(), width, n, max_rows)
+        call("h3b_kv8_append_dev", self.h, cache.packed, _l.KV8_APPEND_ARGS.pack(
+            k.data_ptr(), v.data_ptr(), cu_rows.data_ptr(), start.data_ptr(), table.data_ptr(), kr, kh, vr, vh, shape[0], width, n,
+            max_rows, dt))
 
     def kv8_sdpa(self, cache: KvCache8, q, cu_rows, lens, table, *, max_rows, max_len, left=-1, right=0, sinks=0, block=1, scale=None,
                  out=None):
@@ -475,9 +481,10 @@ class Cuda:
         n, width = self._batch("kv8_sdpa", cache, cu_rows, lens, table)
         rows, heads, hd = q.shape
         out = self._out16("kv8_sdpa", q, (q, cu_rows, lens, table, cache.k, cache.v, cache.k_scale, cache.v_scale), out)
-        call("h3b_kv8_sdpa_dev", self.h, cache.c, dt, q.data_ptr(), qr, qh, rows, cu_rows.data_ptr(), lens.data_ptr(),
-             table.data_ptr(), width, n, max_rows, max_len, heads, hd ** -0.5 if scale is None else scale, left, right, sinks, block,
-             out.data_ptr(), out.stride(0) if rows > 1 else heads * hd, hd)
+        call("h3b_kv8_sdpa_dev", self.h, cache.packed, _l.KV8_SDPA_ARGS.pack(
+            q.data_ptr(), out.data_ptr(), cu_rows.data_ptr(), lens.data_ptr(), table.data_ptr(), qr, qh,
+            out.stride(0) if rows > 1 else heads * hd, hd, rows, heads, width, n, max_rows, max_len, left, right, sinks, block,
+            hd ** -0.5 if scale is None else scale, dt))
         return out
 
     def sdpa_f16_dev(self, q, k, v, scale=None):

@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         fma2(x2, x3, __uint_as_float(sv[ch * 32 + i + 2]), __uint_as_float(sv[ch * 32 + i + 3]), fh, cc);
                         float p0, p1, p2, p3;
                         p0 = ex2_approx(x0); p1 = ex2_approx(x1); p2 = ex2_approx(x2); p3 = ex2_approx(x3);
-                    add2(l0, l1, p0, p1);
+                        add2(l0, l1, p0, p1);
                         add2(l2, l3, p2, p3);
                         packed[i >> 1] = Elem<E>::pack(p0, p1);
                         packed[(i >> 1) + 1] = Elem<E>::pack(p2, p3);

@@ -64,49 +64,47 @@ int h3b_window_tiles(size_t keys, int64_t pos0, size_t rows, int64_t left, int64
     return 1;
 }
 
-int h3b_sdpa_window_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row_stride, size_t q_head_stride, const void *d_k,
-                        size_t k_row_stride, size_t k_head_stride, const void *d_v, size_t v_row_stride, size_t v_head_stride,
-                        size_t lq, size_t lk, size_t heads, size_t kv_heads, size_t head_dim, float scale, int64_t q_pos,
-                        int64_t left, int64_t right, int64_t sinks, int64_t block, void *d_out, size_t o_row_stride,
-                        size_t o_head_stride, char *error, size_t error_size) {
+int h3b_sdpa_window_dev(h3_cuda *cuda, const h3b_sdpa_window_args *x, char *error, size_t error_size) {
     WinArgs a;
-    if (!fill(a, cuda, "sdpa_window", dtype, d_q, q_row_stride, q_head_stride, lq, heads, kv_heads, head_dim, scale, left, right,
-              sinks, block, d_out, o_row_stride, o_head_stride, error, error_size))
+    if (!x) return fail(error, error_size, "sdpa_window: NULL arguments");
+    if (!fill(a, cuda, "sdpa_window", x->dtype, x->d_q, x->q_row_stride, x->q_head_stride, x->lq, x->heads, x->kv_heads, x->head_dim,
+              x->scale, x->left, x->right, x->sinks, x->block, x->d_out, x->o_row_stride, x->o_head_stride, error, error_size))
         return 0;
-    if (lk >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "sdpa_window: shape too large");
-    if (q_pos < 0 || q_pos + (int64_t)lq > H3B_WIN_MAX) return fail(error, error_size, "sdpa_window: q_pos out of range");
-    if (lk && (!d_k || !d_v)) return fail(error, error_size, "sdpa_window: NULL tensor");
-    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) % 8 || ((uintptr_t)d_k & 15) || ((uintptr_t)d_v & 15))
+    const size_t strides = x->k_row_stride | x->k_head_stride | x->v_row_stride | x->v_head_stride;
+    if (x->lk >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "sdpa_window: shape too large");
+    if (x->q_pos < 0 || x->q_pos > H3B_WIN_MAX - (int64_t)x->lq) return fail(error, error_size, "sdpa_window: q_pos out of range");
+    if (x->lk && (!x->d_k || !x->d_v)) return fail(error, error_size, "sdpa_window: NULL tensor");
+    if (strides % 8 || ((uintptr_t)x->d_k & 15) || ((uintptr_t)x->d_v & 15))
         return fail(error, error_size, "sdpa_window: pointers must be 16-byte aligned and strides multiples of 8 elements");
-    if (!k_row_stride || !k_head_stride || !v_row_stride || !v_head_stride)
+    if (!x->k_row_stride || !x->k_head_stride || !x->v_row_stride || !x->v_head_stride)
         return fail(error, error_size, "sdpa_window: row and head strides must be given");
-    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) >> 39) return fail(error, error_size, "sdpa_window: stride too large");
-    if (!lq) return 1;
-    a.k = d_k; a.v = d_v;
-    a.k_rs = (long long)k_row_stride; a.k_hs = (long long)k_head_stride;
-    a.v_rs = (long long)v_row_stride; a.v_hs = (long long)v_head_stride;
-    a.lk = (int)lk; a.q_pos = (int)q_pos; a.max_rows = (int)lq; a.n_seq = 1;
-    return launch<false>(cuda, a, dtype == H3B_F16, lk, error, error_size);
+    if (strides >> 39) return fail(error, error_size, "sdpa_window: stride too large");
+    if (!x->lq) return 1;
+    a.k = x->d_k; a.v = x->d_v;
+    a.k_rs = (long long)x->k_row_stride; a.k_hs = (long long)x->k_head_stride;
+    a.v_rs = (long long)x->v_row_stride; a.v_hs = (long long)x->v_head_stride;
+    a.lk = (int)x->lk; a.q_pos = (int)x->q_pos; a.max_rows = (int)x->lq; a.n_seq = 1;
+    return launch<false>(cuda, a, x->dtype == H3B_F16, x->lk, error, error_size);
 }
 
-int h3b_kv8_sdpa_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const void *d_q, size_t q_row_stride,
-                     size_t q_head_stride, size_t rows, const int32_t *d_cu_rows, const int32_t *d_len, const int32_t *d_table,
-                     size_t table_stride, size_t n_seq, size_t max_rows, size_t max_len, size_t heads, float scale, int64_t left,
-                     int64_t right, int64_t sinks, int64_t block, void *d_out, size_t o_row_stride, size_t o_head_stride,
-                     char *error, size_t error_size) {
+int h3b_kv8_sdpa_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_sdpa_args *x, char *error, size_t error_size) {
     WinArgs a;
+    if (!x) return fail(error, error_size, "kv8_sdpa: NULL arguments");
     if (!kv8_cache_ok(cache, "kv8_sdpa", error, error_size)) return 0;
-    if (!fill(a, cuda, "kv8_sdpa", dtype, d_q, q_row_stride, q_head_stride, rows, heads, cache->kv_heads, cache->head_dim, scale,
-              left, right, sinks, block, d_out, o_row_stride, o_head_stride, error, error_size))
+    if (!fill(a, cuda, "kv8_sdpa", x->dtype, x->d_q, x->q_row_stride, x->q_head_stride, x->rows, x->heads, cache->kv_heads,
+              cache->head_dim, x->scale, x->left, x->right, x->sinks, x->block, x->d_out, x->o_row_stride, x->o_head_stride, error,
+              error_size))
         return 0;
-    if (!kv8_batch_ok(cache, "kv8_sdpa", rows, d_cu_rows, d_len, d_table, table_stride, n_seq, max_rows, error, error_size)) return 0;
-    if (max_len >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "kv8_sdpa: max_len out of range");
-    if (!rows || !n_seq || !max_rows) return 1;
+    if (!kv8_batch_ok(cache, "kv8_sdpa", x->rows, x->d_cu_rows, x->d_len, x->d_table, x->table_stride, x->n_seq, x->max_rows, error,
+                      error_size))
+        return 0;
+    if (x->max_len >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "kv8_sdpa: max_len out of range");
+    if (!x->rows || !x->n_seq || !x->max_rows) return 1;
     a.kc = cache->d_k; a.vc = cache->d_v; a.ks = cache->d_k_scale; a.vs = cache->d_v_scale;
-    a.cu = d_cu_rows; a.len = d_len; a.table = d_table; a.table_stride = (long long)table_stride;
+    a.cu = x->d_cu_rows; a.len = x->d_len; a.table = x->d_table; a.table_stride = (long long)x->table_stride;
     a.pages = (int)cache->pages; a.page_blocks = (int)(cache->page_tokens / KV8_BLOCK);
-    a.max_rows = (int)max_rows; a.n_seq = (int)n_seq;
-    return launch<true>(cuda, a, dtype == H3B_F16, max_len, error, error_size);
+    a.max_rows = (int)x->max_rows; a.n_seq = (int)x->n_seq;
+    return launch<true>(cuda, a, x->dtype == H3B_F16, x->max_len, error, error_size);
 }
 
 }  // extern "C"

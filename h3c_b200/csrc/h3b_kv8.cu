@@ -142,38 +142,39 @@ using namespace h3b;
 
 extern "C" {
 
-int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const void *d_k, size_t k_row_stride,
-                       size_t k_head_stride, const void *d_v, size_t v_row_stride, size_t v_head_stride, size_t rows,
-                       const int32_t *d_cu_rows, const int32_t *d_start, const int32_t *d_table, size_t table_stride, size_t n_seq,
-                       size_t max_rows, char *error, size_t error_size) {
+int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_append_args *x, char *error, size_t error_size) {
+    if (!x) return fail(error, error_size, "kv8_append: NULL arguments");
     if (!kv8_cache_ok(cache, "kv8_append", error, error_size)) return 0;
+    const size_t strides = x->k_row_stride | x->k_head_stride | x->v_row_stride | x->v_head_stride, max_rows = x->max_rows;
     if (!cuda) return fail(error, error_size, "kv8_append: NULL handle");
-    if (dtype != H3B_BF16 && dtype != H3B_F16) return fail(error, error_size, "kv8_append: dtype must be bf16 or f16");
-    if (rows >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "kv8_append: shape too large");
-    if (rows && (!d_k || !d_v)) return fail(error, error_size, "kv8_append: NULL tensor");
-    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) % 8 || ((uintptr_t)d_k & 15) || ((uintptr_t)d_v & 15))
+    if (x->dtype != H3B_BF16 && x->dtype != H3B_F16) return fail(error, error_size, "kv8_append: dtype must be bf16 or f16");
+    if (x->rows >= (size_t)H3B_WIN_MAX) return fail(error, error_size, "kv8_append: shape too large");
+    if (x->rows && (!x->d_k || !x->d_v)) return fail(error, error_size, "kv8_append: NULL tensor");
+    if (strides % 8 || ((uintptr_t)x->d_k & 15) || ((uintptr_t)x->d_v & 15))
         return fail(error, error_size, "kv8_append: pointers must be 16-byte aligned and strides multiples of 8 elements");
-    if (!k_row_stride || !k_head_stride || !v_row_stride || !v_head_stride)
+    if (!x->k_row_stride || !x->k_head_stride || !x->v_row_stride || !x->v_head_stride)
         return fail(error, error_size, "kv8_append: row and head strides must be given");
-    if ((k_row_stride | k_head_stride | v_row_stride | v_head_stride) >> 39) return fail(error, error_size, "kv8_append: stride too large");
-    if (!kv8_batch_ok(cache, "kv8_append", rows, d_cu_rows, d_start, d_table, table_stride, n_seq, max_rows, error, error_size)) return 0;
-    if (!rows || !n_seq || !max_rows) return 1;
+    if (strides >> 39) return fail(error, error_size, "kv8_append: stride too large");
+    if (!kv8_batch_ok(cache, "kv8_append", x->rows, x->d_cu_rows, x->d_start, x->d_table, x->table_stride, x->n_seq, max_rows, error,
+                      error_size))
+        return 0;
+    if (!x->rows || !x->n_seq || !max_rows) return 1;
     AppendArgs a;
     memset(&a, 0, sizeof(a));
-    a.x[0] = d_k; a.x[1] = d_v;
-    a.rs[0] = (long long)k_row_stride; a.rs[1] = (long long)v_row_stride;
-    a.hs[0] = (long long)k_head_stride; a.hs[1] = (long long)v_head_stride;
+    a.x[0] = x->d_k; a.x[1] = x->d_v;
+    a.rs[0] = (long long)x->k_row_stride; a.rs[1] = (long long)x->v_row_stride;
+    a.hs[0] = (long long)x->k_head_stride; a.hs[1] = (long long)x->v_head_stride;
     a.codes[0] = cache->d_k; a.codes[1] = cache->d_v;
     a.scales[0] = cache->d_k_scale; a.scales[1] = cache->d_v_scale;
-    a.cu = d_cu_rows; a.start = d_start; a.table = d_table; a.table_stride = (long long)table_stride;
-    a.rows = (int)rows; a.max_rows = (int)max_rows; a.kv_heads = (int)cache->kv_heads; a.pages = (int)cache->pages;
+    a.cu = x->d_cu_rows; a.start = x->d_start; a.table = x->d_table; a.table_stride = (long long)x->table_stride;
+    a.rows = (int)x->rows; a.max_rows = (int)max_rows; a.kv_heads = (int)cache->kv_heads; a.pages = (int)cache->pages;
     a.page_blocks = (int)(cache->page_tokens / KV8_BLOCK);
     a.status = cuda->d_status;
     // max_rows rows that start anywhere in a block reach this many blocks
-    const dim3 grid((unsigned)ceil_div(max_rows + KV8_BLOCK - 1, KV8_BLOCK), (unsigned)(2 * cache->kv_heads), (unsigned)n_seq);
+    const dim3 grid((unsigned)ceil_div(max_rows + KV8_BLOCK - 1, KV8_BLOCK), (unsigned)(2 * cache->kv_heads), (unsigned)x->n_seq);
     DeviceGuard guard(cuda);
     ProfScope prof(cuda, PROF_OTHER);
-    if (dtype == H3B_F16) k_kv8_append<__half><<<grid, 128, 0, cuda->op_stream>>>(a);
+    if (x->dtype == H3B_F16) k_kv8_append<__half><<<grid, 128, 0, cuda->op_stream>>>(a);
     else k_kv8_append<__nv_bfloat16><<<grid, 128, 0, cuda->op_stream>>>(a);
     cuda->launches++;
     H3B_CUDA_OK(cudaGetLastError(), "k_kv8_append launch");

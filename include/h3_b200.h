@@ -484,11 +484,16 @@ int h3b_sdpa_strided_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row
  * A negative left or right does not bound that side (-1, -1, 0, 1: full attention; -1, 0, 0, 1: causal).  A row that
  * sees no key is zero.  What masked keys hold (NaN, infinities) has no part in the result.  lq = 0 does nothing; out
  * must not overlap the inputs; nothing is allocated, so the call can be captured. */
-int h3b_sdpa_window_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row_stride, size_t q_head_stride, const void *d_k,
-                        size_t k_row_stride, size_t k_head_stride, const void *d_v, size_t v_row_stride, size_t v_head_stride,
-                        size_t lq, size_t lk, size_t heads, size_t kv_heads, size_t head_dim, float scale, int64_t q_pos,
-                        int64_t left, int64_t right, int64_t sinks, int64_t block, void *d_out, size_t o_row_stride,
-                        size_t o_head_stride, char *error, size_t error_size);
+typedef struct {
+    const void *d_q, *d_k, *d_v;
+    void *d_out;
+    size_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride, o_row_stride, o_head_stride;
+    size_t lq, lk, heads, kv_heads, head_dim;
+    int64_t q_pos, left, right, sinks, block;
+    float scale; /* of the scores */
+    int dtype;
+} h3b_sdpa_window_args;
+int h3b_sdpa_window_dev(h3_cuda *cuda, const h3b_sdpa_window_args *args, char *error, size_t error_size);
 /* Host arithmetic of the two windowed operators: the key tiles (of `unit` keys) that rows at pos0 .. pos0 + rows - 1
  * of a sequence of `keys` keys visit: `sink_tiles` tiles from 0 on, then tiles from `from` on, `count` in all. */
 int h3b_window_tiles(size_t keys, int64_t pos0, size_t rows, int64_t left, int64_t right, int64_t sinks, int64_t block,
@@ -508,24 +513,36 @@ typedef struct {
     uint8_t *d_k, *d_v;
     float *d_k_scale, *d_v_scale;
 } h3b_kv8_cache;
-/* Puts k / v rows [rows, kv_heads, 128] (bf16 or f16) behind the first start[s] tokens of each sequence.  The scale of
+/* Puts k / v rows [rows, kv_heads, 128] (bf16 or f16) behind the first d_start[s] tokens of each sequence.  The scale of
  * 64 tokens is the smallest power of two 2^e, e >= -64, with absmax <= 448 * 2^e; a block that already holds tokens in
  * front of the new ones keeps its scale or raises it (their codes are then moved to the raised one).  Tokens of the
  * block behind the new ones are left as they are.  A non-finite value makes its block's scale NaN (codes zero) until
  * the block is started again.  No two sequences of one call may write to the same page. */
-int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const void *d_k, size_t k_row_stride,
-                       size_t k_head_stride, const void *d_v, size_t v_row_stride, size_t v_head_stride, size_t rows,
-                       const int32_t *d_cu_rows, const int32_t *d_start, const int32_t *d_table, size_t table_stride, size_t n_seq,
-                       size_t max_rows, char *error, size_t error_size);
-/* Attention of q rows [rows, heads, 128] over the cache: sequence s has len[s] tokens and its rows are the last ones of
- * them (row i of nq at position len[s] - nq + i); windows as in h3b_sdpa_window_dev.  Rows of out that belong to no
- * sequence are left as they are.  max_len (a bound on len[], or an estimate: results do not depend on it) only guides
+typedef struct {
+    const void *d_k, *d_v;
+    const int32_t *d_cu_rows, *d_start, *d_table;
+    size_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    size_t rows, table_stride, n_seq, max_rows;
+    int dtype;
+} h3b_kv8_append_args;
+int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_append_args *args, char *error,
+                       size_t error_size);
+/* Attention of q rows [rows, heads, 128] over the cache: sequence s has d_len[s] tokens and its rows are the last ones of
+ * them (row i of nq at position d_len[s] - nq + i); windows as in h3b_sdpa_window_dev.  Rows of out that belong to no
+ * sequence are left as they are.  max_len (a bound on d_len[], or an estimate: its rows' values do not depend on it beyond rounding) only guides
  * how the work is split. */
-int h3b_kv8_sdpa_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, int dtype, const void *d_q, size_t q_row_stride,
-                     size_t q_head_stride, size_t rows, const int32_t *d_cu_rows, const int32_t *d_len, const int32_t *d_table,
-                     size_t table_stride, size_t n_seq, size_t max_rows, size_t max_len, size_t heads, float scale, int64_t left,
-                     int64_t right, int64_t sinks, int64_t block, void *d_out, size_t o_row_stride, size_t o_head_stride,
-                     char *error, size_t error_size);
+typedef struct {
+    const void *d_q;
+    void *d_out;
+    const int32_t *d_cu_rows, *d_len, *d_table;
+    size_t q_row_stride, q_head_stride, o_row_stride, o_head_stride;
+    size_t rows, heads, table_stride, n_seq, max_rows, max_len;
+    int64_t left, right, sinks, block;
+    float scale;
+    int dtype;
+} h3b_kv8_sdpa_args;
+int h3b_kv8_sdpa_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_sdpa_args *args, char *error,
+                     size_t error_size);
 
 /* Addition: the same attention over this rank's heads/ulysses heads of the gathered sequence
  * (scatter->q, ->k, ->v, lq = lk = seq_real), each output row stored into scatter->peer_att of the

@@ -3,11 +3,14 @@ through its host entry point against the definition, and the refusals of the ent
 before the handle is used, so a zeroed block of memory stands in for one)."""
 import ctypes as C
 import itertools
+from pathlib import Path
 
 import pytest
 
 import h3c_b200
 from h3c_b200 import lib as l
+
+ROOT = Path(__file__).resolve().parent.parent
 
 
 def sees(j, p, n, left, right, sinks, block):
@@ -59,12 +62,20 @@ def refused(name, *args):
     return err.value.decode()
 
 
+def block(layout, fields):
+    return layout.pack(*(0 if v is None else v for v in fields.values()))
+
+
 def fake_handle():
     return C.cast(C.create_string_buffer(8192), C.c_void_p)
 
 
-WINDOW = dict(dtype=l.BF16, q=A, qr=1024, qh=128, k=A, kr=1024, kh=128, v=A, vr=1024, vh=128, lq=4, lk=9, heads=8, kv=8, hd=128,
-              scale=0.1, q_pos=0, left=-1, right=0, sinks=0, block=1, out=A, orow=1024, oh=128)
+WINDOW = dict(q=A, k=A, v=A, out=A, qr=1024, qh=128, kr=1024, kh=128, vr=1024, vh=128, orow=1024, oh=128, lq=4, lk=9, heads=8, kv=8,
+              hd=128, q_pos=0, left=-1, right=0, sinks=0, block=1, scale=0.1, dtype=l.BF16)
+
+
+def window(**change):
+    return block(l.SDPA_WINDOW_ARGS, WINDOW | change)
 
 
 @pytest.mark.parametrize("change, says", [
@@ -78,66 +89,90 @@ WINDOW = dict(dtype=l.BF16, q=A, qr=1024, qh=128, k=A, kr=1024, kh=128, v=A, vr=
     (dict(kr=0), "strides must be given"), (dict(qh=0), "strides must be given"), (dict(vr=1 << 40), "stride too large"),
     (dict(q_pos=-1), "q_pos"), (dict(q_pos=1 << 29), "q_pos"), (dict(lq=1 << 29), "too large"), (dict(lk=1 << 29), "too large")])
 def test_window_refusals(change, says):
-    assert says in refused("h3b_sdpa_window_dev", fake_handle(), *(WINDOW | change).values())
+    assert says in refused("h3b_sdpa_window_dev", fake_handle(), window(**change))
 
 
 def test_null_handles_are_refused():
-    assert "NULL handle" in refused("h3b_sdpa_window_dev", None, *WINDOW.values())
-    c = cache()
-    assert "NULL handle" in refused("h3b_kv8_append_dev", None, c, *APPEND.values())
-    assert "NULL handle" in refused("h3b_kv8_sdpa_dev", None, c, *CACHE.values())
+    assert "NULL handle" in refused("h3b_sdpa_window_dev", None, window())
+    assert "NULL handle" in refused("h3b_kv8_append_dev", None, cache(), append())
+    assert "NULL handle" in refused("h3b_kv8_sdpa_dev", None, cache(), attention())
+    assert "NULL arguments" in refused("h3b_sdpa_window_dev", fake_handle(), None)
+    assert "NULL arguments" in refused("h3b_kv8_append_dev", fake_handle(), cache(), None)
+    assert "NULL arguments" in refused("h3b_kv8_sdpa_dev", fake_handle(), cache(), None)
+    assert "NULL cache" in refused("h3b_kv8_append_dev", fake_handle(), None, append())
+    assert "NULL cache" in refused("h3b_kv8_sdpa_dev", fake_handle(), None, attention())
 
 
 def cache(**change):
-    f = dict(pages=10, page_tokens=128, kv_heads=4, head_dim=128, d_k=A, d_v=A, d_k_scale=A, d_v_scale=A) | change
-    return l.Kv8Cache(**f)
+    return block(l.KV8_CACHE, dict(pages=10, page_tokens=128, kv_heads=4, head_dim=128, d_k=A, d_v=A, d_k_scale=A, d_v_scale=A) | change)
 
 
-APPEND = dict(dtype=l.BF16, k=A, kr=512, kh=128, v=A, vr=512, vh=128, rows=5, cu=A, start=A, table=A, stride=3, n_seq=2, max_rows=5)
-CACHE = dict(dtype=l.F16, q=A, qr=1024, qh=128, rows=6, cu=A, len=A, table=A, stride=3, n_seq=2, max_rows=5, max_len=99, heads=8,
-             scale=0.1, left=-1, right=0, sinks=0, block=1, out=A, orow=1024, oh=128)
+APPEND = dict(k=A, v=A, cu=A, start=A, table=A, kr=512, kh=128, vr=512, vh=128, rows=5, stride=3, n_seq=2, max_rows=5, dtype=l.BF16)
+CACHE = dict(q=A, out=A, cu=A, len=A, table=A, qr=1024, qh=128, orow=1024, oh=128, rows=6, heads=8, stride=3, n_seq=2, max_rows=5,
+             max_len=99, left=-1, right=0, sinks=0, block=1, scale=0.1, dtype=l.F16)
+
+
+def append(**change):
+    return block(l.KV8_APPEND_ARGS, APPEND | change)
+
+
+def attention(**change):
+    return block(l.KV8_SDPA_ARGS, CACHE | change)
+
+
 BAD_CACHE = [(dict(head_dim=64), "head_dim"), (dict(page_tokens=0), "page_tokens"), (dict(page_tokens=96), "page_tokens"),
              (dict(page_tokens=1 << 17), "page_tokens"), (dict(kv_heads=0), "K/V heads"), (dict(pages=0), "pages"),
              (dict(pages=1 << 24), "pages"), (dict(d_k=None), "NULL cache"), (dict(d_v_scale=None), "NULL cache"),
              (dict(d_v=A + 8), "aligned"), (dict(d_k_scale=A + 2), "aligned")]
 BAD_BATCH = [(dict(cu=None), "NULL sequence table"), (dict(table=None), "NULL sequence table"), (dict(table=A + 1), "4-byte"),
              (dict(stride=0), "table_stride"), (dict(stride=1 << 23), "table_stride"), (dict(n_seq=65536), "sequences"),
-             (dict(max_rows=7), "max_rows"), (dict(dtype=l.F32), "bf16 or f16")]
+             (dict(max_rows=7), "max_rows"), (dict(max_rows=-1), "max_rows"), (dict(rows=-1), "large"), (dict(n_seq=-1), "sequences"), (dict(dtype=l.F32), "bf16 or f16")]
 
 
 @pytest.mark.parametrize("change, says", BAD_CACHE)
 def test_cache_layout_refusals(change, says):
-    assert says in refused("h3b_kv8_append_dev", fake_handle(), cache(**change), *APPEND.values())
-    assert says in refused("h3b_kv8_sdpa_dev", fake_handle(), cache(**change), *CACHE.values())
+    assert says in refused("h3b_kv8_append_dev", fake_handle(), cache(**change), append())
+    assert says in refused("h3b_kv8_sdpa_dev", fake_handle(), cache(**change), attention())
 
 
 @pytest.mark.parametrize("change, says", BAD_BATCH)
 def test_batch_refusals(change, says):
-    named = {k: ("start" if k == "len" else k) for k in APPEND}
-    assert says in refused("h3b_kv8_append_dev", fake_handle(), cache(), *(APPEND | {named.get(k, k): v for k, v in change.items()}).values())
-    assert says in refused("h3b_kv8_sdpa_dev", fake_handle(), cache(), *(CACHE | change).values())
+    assert says in refused("h3b_kv8_append_dev", fake_handle(), cache(), append(**change))
+    assert says in refused("h3b_kv8_sdpa_dev", fake_handle(), cache(), attention(**change))
 
 
 @pytest.mark.parametrize("change, says", [(dict(k=None), "NULL tensor"), (dict(v=A + 8), "16-byte"), (dict(kr=4), "multiples of 8"),
                                           (dict(vh=0), "strides must be given"), (dict(kr=1 << 40), "stride too large")])
 def test_append_refusals(change, says):
-    assert says in refused("h3b_kv8_append_dev", fake_handle(), cache(), *(APPEND | change).values())
+    assert says in refused("h3b_kv8_append_dev", fake_handle(), cache(), append(**change))
 
 
 @pytest.mark.parametrize("change, says", [(dict(heads=6), "6 heads over 4"), (dict(q=None), "NULL tensor"), (dict(out=A + 8), "16-byte"),
                                           (dict(qr=4), "multiples of 8"), (dict(oh=0), "strides must be given"), (dict(sinks=-2), "sinks"),
                                           (dict(block=0), "block"), (dict(scale=-1.0), "scale"), (dict(max_len=1 << 29), "max_len")])
 def test_cache_attention_refusals(change, says):
-    assert says in refused("h3b_kv8_sdpa_dev", fake_handle(), cache(), *(CACHE | change).values())
+    assert says in refused("h3b_kv8_sdpa_dev", fake_handle(), cache(), attention(**change))
 
 
 def test_calls_without_work_return_before_the_device():
     lib, err = h3c_b200.load(), C.create_string_buffer(512)
-    assert lib.h3b_sdpa_window_dev(fake_handle(), *(WINDOW | dict(lq=0, q=None, out=None)).values(), err, 512) == 1
-    assert lib.h3b_kv8_append_dev(fake_handle(), cache(), *(APPEND | dict(n_seq=0, cu=None, start=None, table=None)).values(), err, 512) == 1
-    assert lib.h3b_kv8_append_dev(fake_handle(), cache(), *(APPEND | dict(rows=0, max_rows=0, k=None, v=None)).values(), err, 512) == 1
-    assert lib.h3b_kv8_sdpa_dev(fake_handle(), cache(), *(CACHE | dict(rows=0, max_rows=0, q=None, out=None)).values(), err, 512) == 1
-    assert lib.h3b_kv8_sdpa_dev(fake_handle(), cache(), *(CACHE | dict(n_seq=0)).values(), err, 512) == 1
+    assert lib.h3b_sdpa_window_dev(fake_handle(), window(lq=0, q=None, out=None), err, 512) == 1
+    assert lib.h3b_kv8_append_dev(fake_handle(), cache(), append(n_seq=0, cu=None, start=None, table=None), err, 512) == 1
+    assert lib.h3b_kv8_append_dev(fake_handle(), cache(), append(rows=0, max_rows=0, k=None, v=None), err, 512) == 1
+    assert lib.h3b_kv8_sdpa_dev(fake_handle(), cache(), attention(rows=0, max_rows=0, q=None, out=None), err, 512) == 1
+    assert lib.h3b_kv8_sdpa_dev(fake_handle(), cache(), attention(n_seq=0), err, 512) == 1
+
+
+def test_argument_blocks_have_the_size_of_the_header_structs(tmp_path):
+    import subprocess
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "h3_b200.h"\nint main(void) { printf("%zu %zu %zu %zu", sizeof(h3b_sdpa_window_args), '
+                   'sizeof(h3b_kv8_cache), sizeof(h3b_kv8_append_args), sizeof(h3b_kv8_sdpa_args)); return 0; }\n')
+    subprocess.run(["gcc", "-I" + str(ROOT / "include"), str(src), "-o", str(tmp_path / "sizes")], check=True)
+    got = subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout.split()
+    # a block may leave out the padding behind its last field
+    want = [-(-b.size // 8) * 8 for b in (l.SDPA_WINDOW_ARGS, l.KV8_CACHE, l.KV8_APPEND_ARGS, l.KV8_SDPA_ARGS)]
+    assert [int(x) for x in got] == want
 
 
 def test_cache_object_checks_its_tensors():
