@@ -137,7 +137,7 @@ k_attn_few(const __grid_constant__ FewParams p) {
     // ---- copies: lane 0 issues, all lanes together look up 32 tiles at a time
     int look_base = 0;
     int my_row = 0;                                // 8-bit: first row of the tile's codes, -1: page outside the pool
-    float my_ks = 1.0f, my_lvs = 0.0f, my_ivs = 1.0f;   // key scale, log2 and inverse of the value scale
+    float my_ks = 1.0f, my_vs = 1.0f, my_lvs = 0.0f, my_ivs = 1.0f;   // its scales; log2 and inverse of the value scale
     auto look_up = [&](int it0) {
         look_base = it0;
         if (KV8) {
@@ -147,9 +147,7 @@ k_attn_few(const __grid_constant__ FewParams p) {
                 const long long bi = kv8_block_index(a, s, tile * U / KV8_BLOCK, kvh);
                 my_row = bi < 0 ? -1 : (int)(bi * KV8_BLOCK) + tile * U % KV8_BLOCK;
                 my_ks = bi < 0 ? 1.0f : __ldg(a.ks + bi);
-                const float vs = bi < 0 ? 1.0f : __ldg(a.vs + bi);
-                my_lvs = log2f(vs);
-                my_ivs = 1.0f / vs;
+                my_vs = bi < 0 ? 1.0f : __ldg(a.vs + bi);
             }
         }
     };
@@ -169,20 +167,35 @@ k_attn_few(const __grid_constant__ FewParams p) {
             }
         }
     };
-    auto fetch_keys = [&](int it) {                // page and scales of tile `it` (warp-uniform), then its keys
-        if (it - look_base >= 32) look_up(it);
+    auto logs = [&]() {
         if (KV8) {
-            next_row = __shfl_sync(0xffffffffu, my_row, it - look_base);
-            next_ks = __shfl_sync(0xffffffffu, my_ks, it - look_base);
-            next_lvs = __shfl_sync(0xffffffffu, my_lvs, it - look_base);
-            next_ivs = __shfl_sync(0xffffffffu, my_ivs, it - look_base);
+            my_lvs = log2f(my_vs);
+            my_ivs = 1.0f / my_vs;
         }
+    };
+    auto take_scales = [&](int src) {
+        if (KV8) {
+            next_ks = __shfl_sync(0xffffffffu, my_ks, src);
+            next_lvs = __shfl_sync(0xffffffffu, my_lvs, src);
+            next_ivs = __shfl_sync(0xffffffffu, my_ivs, src);
+        }
+    };
+    auto fetch_keys = [&](int it) {                // page and scales of tile `it` (warp-uniform), then its keys
+        if (it - look_base >= 32) {
+            look_up(it);
+            logs();
+        }
+        if (KV8) next_row = __shfl_sync(0xffffffffu, my_row, it - look_base);
+        take_scales(it - look_base);
         copy(it, next_row, 0);
     };
-    if (n_it) {
+    if (n_it) {                                    // the first copies do not wait for the scales
         look_up(0);
-        fetch_keys(0);
+        if (KV8) next_row = __shfl_sync(0xffffffffu, my_row, 0);
+        copy(0, next_row, 0);
         copy(0, next_row, 1);
+        logs();
+        take_scales(0);
     }
 
     // ---- Q as the other operand: lane (g, t) has row g of every 8.  16-bit keys: the product's own order of d.  8-bit:
@@ -492,15 +505,25 @@ k_attn_few(const __grid_constant__ FewParams p) {
         const int qi = (r_first + r) / a.group, hd = (r_first + r) - qi * a.group;
         bool odd = false;
         if (d < 128) {
-            float m = -INFINITY, l = 0.0f, v = 0.0f;
-            for (int c = 0; c < p.split; c++) m = fmaxf(m, ld_cluster_f32(mapa_shared(acc_addr, c) + (16 * 128 + r) * 4));
-            for (int c = 0; c < p.split; c++) {
+            float mc[8], lc[8], vc[8], m = -INFINITY, l = 0.0f, v = 0.0f;            // at most 8 CTAs, all loads under way at once
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+                if (c >= p.split) break;
                 const uint32_t base = mapa_shared(acc_addr, c);
-                const float mc = ld_cluster_f32(base + (16 * 128 + r) * 4), lc = ld_cluster_f32(base + (16 * 128 + 16 + r) * 4);
-                const float w = mc == -INFINITY ? 0.0f : ex2_approx(mc - m);
-                l += lc != lc ? lc : w * lc;
-                v += w * ld_cluster_f32(base + (r * 128 + d) * 4);
+                mc[c] = ld_cluster_f32(base + (16 * 128 + r) * 4);
+                lc[c] = ld_cluster_f32(base + (16 * 128 + 16 + r) * 4);
+                vc[c] = ld_cluster_f32(base + (r * 128 + d) * 4);
             }
+#pragma unroll
+            for (int c = 0; c < 8; c++)
+                if (c < p.split) m = fmaxf(m, mc[c]);
+#pragma unroll
+            for (int c = 0; c < 8; c++)
+                if (c < p.split) {
+                    const float w = mc[c] == -INFINITY ? 0.0f : ex2_approx(mc[c] - m);
+                    l += lc[c] != lc[c] ? lc[c] : w * lc[c];
+                    v += w * vc[c];
+                }
             const float res = h3b_win_count(h3b_win_of(a.win, e.pos0 + qi, e.n)) ? v * (1.0f / l) : 0.0f;
             T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qi) * a.o_rs + (long long)(kvh * a.group + hd) * a.o_hs;
             reinterpret_cast<unsigned short *>(dst)[d] = (unsigned short)(Elem<T>::pack(res, res) & 0xffffu);
