@@ -347,7 +347,7 @@ k_attn_few(const __grid_constant__ FewParams p) {
                 if (KV8 && mx == -INFINITY) f[j] = 1.0f, off[j] = 0.0f;
                 mx = KV8 ? fmaf(mx, f[j], off[j]) : mx * f[j];
                 top[j] = mx;
-                grow |= mx > m_run[nt][j] + 8.0f || (m_run[nt][j] == -INFINITY && mx > -INFINITY);
+                grow |= mx > m_run[nt][j] + 8.0f;                                   // also at the first visible key: m_run = -inf
             }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll

@@ -297,6 +297,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             // ------------------------------------------------------------ MMA issuer
             // The whole warp walks the loop, converged; one lane, elected once, issues every tcgen05 instruction.  The
             // stage barriers of the next iteration are polled behind an issued block, while the queue drains.
+            // Its waits are not voted on: a lane that gives up alone leaves the loop alone, and nothing in it is collective.
+            auto poll = [&](uint64_t *b, uint32_t parity, int code) -> bool { return mbar_wait(b, parity, abort_word, a.status, code); };
             const bool lead = elect_one();
             constexpr uint32_t idesc_s = umma_idesc(1, Elem<E>::FMT, Elem<E>::FMT, BM, BN, 0, 0);
             constexpr uint32_t idesc_o = umma_idesc(1, Elem<E>::FMT, Elem<E>::FMT, BM, HD, 0, 1);
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             for (int k = 0; ok && next_item(k, it); k++) {
                 const int n_kv = it.n_kv, n_tiles = it.row_tiles(p.bm);
                 if (!n_kv) continue;
-                ok = wait(&ctl.q_full, q & 1, H3B_ST_TIMEOUT_OTHER) && wait(&ctl.k_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL);
+                ok = poll(&ctl.q_full, q & 1, H3B_ST_TIMEOUT_OTHER) && poll(&ctl.k_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL);
                 if (!ok) break;
                 tc_fence_after();
                 for (int t = 0; t < n_tiles; t++) issue_s(t, c & 1);
@@ -334,18 +336,18 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     tc_commit(&ctl.k_empty[c & 1]);
                     if (n_kv == 1) tc_commit(&ctl.q_empty);
                 }
-                ok = wait(&ctl.v_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL) &&
-                     (n_kv < 2 || wait(&ctl.k_full[(c + 1) & 1], ((c + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL));
+                ok = poll(&ctl.v_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL) &&
+                     (n_kv < 2 || poll(&ctl.k_full[(c + 1) & 1], ((c + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL));
                 auto step = [&](int j, auto stage_c) {
                     constexpr int st = decltype(stage_c)::value, nx = st ^ 1;
                     const bool more = j + 1 < n_kv;
                     for (int t = 0; t < n_tiles && ok; t++) {
                         const uint32_t ph = (uint32_t)((t ? pc[1] : pc[0]) + j) & 1;
-                        ok = wait(&ctl.p_full[2 * t], ph, H3B_ST_TIMEOUT_OTHER);
+                        ok = poll(&ctl.p_full[2 * t], ph, H3B_ST_TIMEOUT_OTHER);
                         if (!ok) break;
                         tc_fence_after();
                         issue_pv(t, st, 0, j == 0);
-                        ok = wait(&ctl.p_full[2 * t + 1], ph, H3B_ST_TIMEOUT_OTHER);
+                        ok = poll(&ctl.p_full[2 * t + 1], ph, H3B_ST_TIMEOUT_OTHER);
                         if (!ok) break;
                         tc_fence_after();
                         issue_pv(t, st, 1, false);
@@ -360,8 +362,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         }
                     }
                     if (ok && more) {
-                        ok = wait(&ctl.v_full[nx], ((c + j + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
-                        if (ok && j + 2 < n_kv) ok = wait(&ctl.k_full[st], ((c + j + 2) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
+                        ok = poll(&ctl.v_full[nx], ((c + j + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
+                        if (ok && j + 2 < n_kv) ok = poll(&ctl.k_full[st], ((c + j + 2) >> 1) & 1, H3B_ST_TIMEOUT_FULL);
                         tc_fence_after();
                     }
                 };
@@ -561,6 +563,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             float m_run = -INFINITY, l_run = 0.0f, row_scale = a.scale_log2;
             for (int j = 0; j < n_kv; j++) {
                 const int key = it.key(j);
+                const bool whole = h3b_win_full(wa, wz, key, BN);        // no mask; decided before the scores are waited for
                 ok = wait(&ctl.s_full[t], (mine + j) & 1, H3B_ST_TIMEOUT_TMEM_FULL);
                 if (!ok) break;
                 float4 scl;
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
 #pragma unroll
                 for (int ch = 0; ch < BN / 32; ch++) tmem_ld_32x32b_x32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[ch * 32]));
                 tmem_ld_wait();
-                if (!h3b_win_full(wa, wz, key, BN)) {
+                if (!whole) {
 #pragma unroll
                     for (int ch = 0; ch < BN / 32; ch++) {
                         // bits of the 32 keys that the row sees
@@ -619,11 +622,11 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 }
                 if (mx != mx) l_run = mx;                                // undefined, and so is the row from here on
                 const float m_new = fmaxf(m_run, mx);
-                const bool grow = m_new > m_run + 8.0f || (m_run == -INFINITY && m_new > -INFINITY);
+                const bool grow = m_new > m_run + 8.0f;                  // also at the first visible key: m_run = -inf
                 if (__any_sync(0xffffffffu, grow)) {
                     float alpha = 1.0f;
                     if (grow) {
-                        alpha = m_run == -INFINITY ? 0.0f : ex2_approx(m_run - m_new);
+                        alpha = ex2_approx(m_run - m_new);
                         m_run = m_new;
                         l_run *= alpha;
                     }
