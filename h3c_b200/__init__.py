@@ -83,9 +83,13 @@ class KvCache8:
                 raise H3Error("KvCache8: scales must be contiguous float32")
         if v.get_device() != where or k_scale.get_device() != where or v_scale.get_device() != where:
             raise H3Error("KvCache8: the tensors are on different devices")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.kv_heads, self.device_index = heads, where
-        self.packed = _l.KV8_CACHE.pack(pages, tokens, heads, hd, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        packed = _l.KV8_CACHE.pack(pages, tokens, heads, hd, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        for name, value in zip(self.__slots__, (k, v, k_scale, v_scale, heads, where, packed)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):   # the packed description holds the addresses of these very tensors
+        if value is not getattr(self, name, None):   # `cache.k_scale *= 2` works in place and sets it to itself
+            raise AttributeError("a KvCache8 keeps its tensors: make another one")
 
 
 class Cuda:

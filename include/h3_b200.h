@@ -502,12 +502,12 @@ int h3b_window_tiles(size_t keys, int64_t pos0, size_t rows, int64_t left, int64
 /* Addition: a paged key/value cache held in 8 bits.  The caller owns the memory (16-byte aligned codes):
  *   d_k, d_v              E4M3 codes [pages][kv_heads][page_tokens][128]
  *   d_k_scale, d_v_scale  f32        [pages][kv_heads][page_tokens / 64], one scale per 64 tokens and head
- * value = code * scale; page_tokens is a multiple of 64; pages * kv_heads * page_tokens < 2^31.  The pages of sequence
+ * value = code * scale, scales positive (or NaN, see below); page_tokens is a multiple of 64; pages * kv_heads * page_tokens < 2^31.  The pages of sequence
  * s are table[s * table_stride ...], its token t lies in page t / page_tokens of that list; pages that no call needs
  * (behind the length, or wholly outside the window) may hold any index.  A sequence's rows are rows cu_rows[s] ..
  * cu_rows[s + 1] - 1 of the 16-bit tensors.  These tables are int32 on the device, so that a captured call follows
  * them; max_rows bounds the rows of any one sequence.  A sequence whose rows, length or page indices lie outside the
- * arrays is skipped or read as masked, and h3b_cuda_check reports it. */
+ * arrays is not followed there, its output is invalid, and h3b_cuda_check reports it. */
 typedef struct {
     size_t pages, page_tokens, kv_heads, head_dim;
     uint8_t *d_k, *d_v;
@@ -517,7 +517,7 @@ typedef struct {
  * 64 tokens is the smallest power of two 2^e, e >= -64, with absmax <= 448 * 2^e; a block that already holds tokens in
  * front of the new ones keeps its scale or raises it (their codes are then moved to the raised one).  Tokens of the
  * block behind the new ones are left as they are.  A non-finite value makes its block's scale NaN (codes zero) until
- * the block is started again.  No two sequences of one call may write to the same page. */
+ * the block is started again.  No page may be written for two sequences, or twice for one, in one call. */
 typedef struct {
     const void *d_k, *d_v;
     const int32_t *d_cu_rows, *d_start, *d_table;

@@ -87,6 +87,7 @@ def window(**change):
     (dict(q=A + 8), "16-byte"), (dict(k=A + 2), "16-byte"), (dict(v=A + 4), "16-byte"), (dict(out=A + 8), "16-byte"),
     (dict(qr=1028), "multiples of 8"), (dict(kh=129), "multiples of 8"), (dict(vr=4), "multiples of 8"), (dict(oh=2), "multiples of 8"),
     (dict(kr=0), "strides must be given"), (dict(qh=0), "strides must be given"), (dict(vr=1 << 40), "stride too large"),
+    (dict(oh=64), "overlap"), (dict(orow=120), "overlap"), (dict(lq=1 << 28, heads=128, kv=8), "too large"),
     (dict(q_pos=-1), "q_pos"), (dict(q_pos=1 << 29), "q_pos"), (dict(lq=1 << 29), "too large"), (dict(lk=1 << 29), "too large")])
 def test_window_refusals(change, says):
     assert says in refused("h3b_sdpa_window_dev", fake_handle(), window(**change))
@@ -180,7 +181,10 @@ def test_cache_object_checks_its_tensors():
     k = torch.zeros(3, 2, 128, 128, dtype=torch.uint8)
     s = torch.zeros(3, 2, 2)
     h3c_b200.KvCache8(k, k.clone(), s, s.clone())
-    h3c_b200.KvCache8(k.view(torch.float8_e4m3fn), k, s, s)
+    c = h3c_b200.KvCache8(k.view(torch.float8_e4m3fn), k, s, s)
+    assert c.kv_heads == 2 and l.KV8_CACHE.unpack(c.packed) == (3, 128, 2, 128, k.data_ptr(), k.data_ptr(), s.data_ptr(), s.data_ptr())
+    with pytest.raises(AttributeError):
+        c.k = k
     for bad in ((k[:2], k, s, s), (k, k, s[..., :1], s), (k.float(), k, s, s), (k, k, s.double(), s),
                 (k.transpose(1, 2), k.transpose(1, 2), s, s), (k, k, s.expand(3, 2, 2)[:, :, :1], s)):
         with pytest.raises(h3c_b200.H3Error):

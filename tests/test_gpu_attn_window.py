@@ -211,9 +211,10 @@ def test_window_strides_orders_and_views(cuda):
         check_window(cuda, *wide, **w)
         every = [normal(g, 2 * n, h, 128, dtype=BF)[::2] for h, n in ((6, lq), (2, 400), (2, 400))]
         check_window(cuda, *every, **w)
-        room = torch.full((lq + 5, 6 * 128 + 64), 3.0, dtype=BF, device="cuda")            # out inside something larger
-        check_window(cuda, q, k, v, got=cuda.sdpa_window(q, k, v, out=room[:lq, :768], **w), **w)
-        assert (room[lq:] == 3).all() and (room[:, 768:] == 3).all()
+        for first, wide in ((0, 6 * 128 + 64), (8, 6 * 128 + 24)):                          # out inside something larger, 16-byte aligned
+            room = torch.full((lq + 5, wide), 3.0, dtype=BF, device="cuda")
+            check_window(cuda, q, k, v, got=cuda.sdpa_window(q, k, v, out=room[:lq, first:first + 768], **w), **w)
+            assert (room[lq:] == 3).all() and (room[:, :first] == 3).all() and (room[:, first + 768:] == 3).all()
 
 
 @pytest.mark.parametrize("lq", [1, 150])
@@ -647,6 +648,42 @@ def test_captured_decode_loop_follows_the_tables(cuda, rows):
                 model.same_as(cache)
                 check_cache(cuda, cache, table.cpu().numpy(), model, q, cu.tolist(), [(i + 1) * rows] * n, got=out, left=300, sinks=4)
                 check_window(cuda, q, k, v, got=near, left=10, right=0)
+    finally:
+        torch.cuda.synchronize()
+        cuda.use_stream(torch.cuda.current_stream())
+
+
+def test_two_graphs_replayed_at_once(cuda):
+    """Nothing is shared between two captured calls but the handle: their replays may overlap."""
+    g = gen(17)
+    rng = np.random.default_rng(17)
+    cache, table, _ = filled(cuda, rng, g, [3000], 64, 4, BF, spread=False)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    table, lens = i32(table), i32([3000])
+    graphs, outs, wants = [], [], []
+    try:
+        for s, rows in zip(side, (3, 300)):
+            q = normal(g, rows, 8, 128, dtype=BF)
+            k, v = normal(g, 2000, 8, 128, dtype=BF), normal(g, 2000, 8, 128, dtype=BF)
+            cu = i32([0, rows])
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                cuda.use_stream(s)
+                step = lambda: (cuda.kv8_sdpa(cache, q, cu, lens, table, max_rows=rows, max_len=3000, left=1500),  # noqa: E731
+                                cuda.sdpa_window(q, k, v, left=900, right=0, q_pos=2000 - rows, sinks=3))
+                wants.append([o.clone() for o in step()])
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=s):
+                    outs.append(step())
+                graphs.append((graph, q, k, v, cu))
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for s, (graph, *_) in zip(side, graphs):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(outs, wants):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
     finally:
         torch.cuda.synchronize()
         cuda.use_stream(torch.cuda.current_stream())
