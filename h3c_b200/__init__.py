@@ -67,25 +67,25 @@ class KvCache8:
     __slots__ = ("k", "v", "k_scale", "v_scale", "kv_heads", "device_index", "packed")
 
     def __init__(self, k, v, k_scale, v_scale):
-        shape = k.shape
+        import torch
+        shape, scales = k.shape, k_scale.shape
         if len(shape) != 4 or v.shape != shape:
             raise H3Error("KvCache8: k and v must be [pages, kv_heads, page_tokens, 128]")
         pages, heads, tokens, hd = shape
-        scales = k_scale.shape
         if scales != (pages, heads, tokens // 64) or v_scale.shape != scales:
             raise H3Error("KvCache8: scales must be [pages, kv_heads, page_tokens // 64]")
-        where = k.get_device()
-        for t in (k, v):
-            if str(t.dtype) not in ("torch.float8_e4m3fn", "torch.uint8") or not t.is_contiguous():
-                raise H3Error("KvCache8: codes must be contiguous float8_e4m3fn or uint8")
-        for t in (k_scale, v_scale):
-            if str(t.dtype) != "torch.float32" or not t.is_contiguous():
-                raise H3Error("KvCache8: scales must be contiguous float32")
+        where, codes, f32 = k.get_device(), (torch.float8_e4m3fn, torch.uint8), torch.float32
+        if k.dtype not in codes or v.dtype not in codes or not k.is_contiguous() or not v.is_contiguous():
+            raise H3Error("KvCache8: codes must be contiguous float8_e4m3fn or uint8")
+        if k_scale.dtype is not f32 or v_scale.dtype is not f32 or not k_scale.is_contiguous() or not v_scale.is_contiguous():
+            raise H3Error("KvCache8: scales must be contiguous float32")
         if v.get_device() != where or k_scale.get_device() != where or v_scale.get_device() != where:
             raise H3Error("KvCache8: the tensors are on different devices")
-        packed = _l.KV8_CACHE.pack(pages, tokens, heads, hd, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
-        for name, value in zip(self.__slots__, (k, v, k_scale, v_scale, heads, where, packed)):
-            object.__setattr__(self, name, value)
+        keep = object.__setattr__
+        keep(self, "k", k), keep(self, "v", v), keep(self, "k_scale", k_scale), keep(self, "v_scale", v_scale)
+        keep(self, "kv_heads", heads), keep(self, "device_index", where)
+        keep(self, "packed", _l.KV8_CACHE.pack(pages, tokens, heads, hd, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
+                                               v_scale.data_ptr()))
 
     def __setattr__(self, name, value):   # the packed description holds the addresses of these very tensors
         if value is not getattr(self, name, None):   # `cache.k_scale *= 2` works in place and sets it to itself
