@@ -210,29 +210,20 @@ k_attn_few(const __grid_constant__ FewParams p) {
         const T *src = reinterpret_cast<const T *>(a.q) + (long long)(e.row0 + qi) * a.q_rs + (long long)(kvh * a.group + hd) * a.q_hs;
         float rs = a.scale_log2;
         if (KV8) {
-            uint32_t w[16];
+            uint32_t w[16], pair = 0u;
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 uint4 x = make_uint4(0u, 0u, 0u, 0u);
                 if (live) x = __ldg(reinterpret_cast<const uint4 *>(src + (c >> 1) * 64 + t * 16 + (c & 1) * 8));
                 w[4 * c] = x.x; w[4 * c + 1] = x.y; w[4 * c + 2] = x.z; w[4 * c + 3] = x.w;
+                pair = __vmaxu2(pair, abs_max8_pair(x));
             }
-            float top = 0.0f;
-            bool odd = false;                      // not finite: as it is, so that it reaches the result
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float f = fabsf(to_f<T>(w[i], j));
-                    odd |= !(f < INFINITY);
-                    top = fmaxf(top, f);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            odd = __shfl_xor_sync(0xffffffffu, (int)odd, 1) | odd;
-            odd = __shfl_xor_sync(0xffffffffu, (int)odd, 2) | odd;
-            int sh = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
-            sh = odd || top == 0.0f ? 0 : max(min(sh, 120), -120);
+            uint32_t top = max(pair & 0xffffu, pair >> 16);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const uint32_t bits = widen_abs<T>(top);
+            int sh = 14 - ((int)(bits >> 23) - 127);
+            sh = bits >= 0x7f800000u || bits == 0u ? 0 : max(min(sh, 120), -120);   // not finite: as it is, so that it reaches the result
             const float up = __uint_as_float((uint32_t)(127 + sh) << 23), down = __uint_as_float((uint32_t)(127 - sh) << 23);
             rs *= down;
 #pragma unroll

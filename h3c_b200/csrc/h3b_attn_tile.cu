@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         const int r = r0 + sub;
                         uint4 *at = reinterpret_cast<uint4 *>(base + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
                         const uint4 w = *at;
-                        uint32_t top = abs_max8<T>(w);
+                        uint32_t top = abs_max8(w);
 #pragma unroll
                         for (int y = 1; y < 16; y <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, y));
                         const uint32_t bits = widen_abs<T>(top);

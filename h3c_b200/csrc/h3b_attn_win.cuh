@@ -74,16 +74,14 @@ __device__ __forceinline__ long long kv8_block_index(const WinArgs &a, int s, in
     return ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
 }
 
-// largest magnitude of eight 16-bit floats as their bit pattern: magnitudes order like integers, NaN above infinity
-template <typename T> __device__ __forceinline__ uint32_t abs_max8(const uint4 &w) {
-    uint32_t m = 0;
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t t = v[i] & 0x7fff7fffu;
-        m = max(m, max(t & 0xffffu, t >> 16));
-    }
-    return m;
+// Largest magnitude of eight 16-bit floats, as two 16-bit patterns side by side: magnitudes order like integers, NaN above
+// infinity.
+__device__ __forceinline__ uint32_t abs_max8_pair(const uint4 &w) {
+    return __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+}
+__device__ __forceinline__ uint32_t abs_max8(const uint4 &w) {
+    const uint32_t m = abs_max8_pair(w);
+    return max(m & 0xffffu, m >> 16);
 }
 // such a pattern as that of an f32
 template <typename T> __device__ __forceinline__ uint32_t widen_abs(uint32_t h) {

@@ -93,7 +93,8 @@ template <typename T> __global__ void __launch_bounds__(128) k_kv8_append(const 
     const float before = from > 0 ? a.scales[w][bi] : 0.0f;      // tokens in front of the new ones keep it at least
     uint32_t top = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, abs_max8<T>(raw[i]));
+    for (int i = 0; i < 8; i++) top = __vmaxu2(top, abs_max8_pair(raw[i]));
+    top = max(top & 0xffffu, top >> 16);
     top = __reduce_max_sync(0xffffffffu, top);
     if ((tid & 31) == 0) red[tid >> 5] = top;
     __syncthreads();                                             // (and every thread has read the old scale)
