@@ -4,8 +4,8 @@
 // A work item is (two row tiles A and B of one K/V head, range of keys).  A row is a (query, head) pair of the K/V head's
 // group, queries outermost: shared heads fill tiles with few queries, and K and V are read once for all heads of the
 // group.  A tile holds as many whole queries as fit 128 rows (126 rows for groups of 3, 6, 7), so that one TMA box of
-// {64 dimensions, group, queries} brings half of its Q.  The key tiles (128 keys) that an item visits are the tiles of the sinks and of the union of its
-// rows' windows (h3b_window.h); only a tile that some row does not see wholly pays for a mask.
+// {64 dimensions, group, queries} brings half of its Q.  The key tiles (128 keys) that an item visits are the tiles of the
+// sinks and of the union of its rows' windows (h3b_window.h); only a tile that some row does not see wholly pays for a mask.
 // A CTA stays on its SM and takes item after item (cluster launch control hands it the CTAs that have not started yet,
 // in grid order, so the chip balances itself), and the roles run ahead into the next item: its Q, K and V arrive while
 // the last softmax and the stores of the current one are under way.  With one item per CTA, a window of 256 keys took
@@ -33,6 +33,21 @@
 //
 // Few items and many keys: the keys are split over the CTAs of a cluster (one item each), whose partial results meet in
 // shared memory.
+//
+// Measured (B200; TFLOP/s of visible pairs): frames of the 6,144-token step (24 heads, three frames and the first) 191-198 us
+// = 1170-1210, 226 us in a long run at the 1000 W limit; 50,220-token video (eight frames back and the first) 7.5-7.8 ms =
+// 1100-1130, at the limit all the time; full attention over 6,144 tokens 367-380 us against 355-360 of k_attn, which needs
+// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 76-83 us = 570-625; a frame of
+// 1,620 queries over 50,220 cached tokens 0.99-1.03 ms = 970-1010; prompts and tokens of 9 sequences, windows of 2,048 and
+// 64 sinks 127-136 us.  Per key tile of both row tiles: 3,230 cycles (16-bit), 3,780 (8-bit, where the widened tiles are
+// written and the codes read beside the operands in shared memory), 2,048 of them products: the chain scores -> softmax ->
+// P V -> next scores of a row tile bounds it, as in k_attn.  A tile with masks takes about 1,000 cycles more.
+// Measured and rejected:
+//   - warps of their own that divide and store finished rows: 16-bit the same within 1 %, 8-bit (the widening warps) 10 % slower;
+//   - row tiles of the last, partly empty round as items of their own: 76.2 against 77.3 us (56 heads over 8);
+//   - a share of the exponentials on the FMA pipe (ex2_emu2): 1 to 4 % slower here;
+//   - a widening loop unrolled over its four quarters: 8-bit 25 % slower (instruction cache);
+//   - claiming the next item at the start of the current one: 174 against 133 us (ragged cache).
 #include <algorithm>
 #include <type_traits>
 
