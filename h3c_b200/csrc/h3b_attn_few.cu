@@ -24,12 +24,12 @@
 //   one token for each of 64 streams of up to 16,384 tokens, 56 heads over 8: 178 us = 6.6 TB/s, what a copy reaches.  With
 //   the rows as the products' 16 rows it was 464 us, with twelve warps and shorter tiles 210: half of every product was
 //   padding and a warp alone issues one instruction in four cycles.
-//   five drafted tokens for 12 streams, 24 heads over 8 (15 rows), windows of 8,192: 46 us = 3.8 TB/s; twice the products
-//   and exponentials per key, issue-bound (about 1,000 instructions per 64 keys and warp, 33 % of the issue slots of three
-//   warps per scheduler, two thirds of their time waiting for the result before).
-//   one stream of 2,313 tokens and 24 heads: 8.4 us, one of no tokens at all 4.1: launch, look-ups one behind the other
-//   (extents, page, copy) and the meeting of warps and CTAs.  One token over 4,160 of 16,384 16-bit keys, 24 heads: 12.6 us.
-//   Widening on the integer pipe (four instructions for two codes instead of one conversion): 10 % slower.
+//   five drafted tokens for 12 streams, 24 heads over 8 (15 rows), windows of 8,192: 46-47 us = 3.8 TB/s; twice the
+//   products and exponentials per key.  Bound by latency: no unit is half busy (DRAM 48 %, issue 33 %, tensor 27 %), and of
+//   7.6 cycles that a warp takes per instruction 2.1 are fixed latency, 1.3 loads and 1.0 barriers.
+//   one stream of 24 heads: 8.2-8.4 us over 2,313 tokens, 6.8 over 640, 5.4 over 64, 3.6 over none: launch, look-ups one
+//   behind the other (extents, page, copy) and the meeting of warps and CTAs.  One token over 4,160 of 16,384 16-bit keys,
+//   24 heads: 12.6 us.
 #include <algorithm>
 #include <type_traits>
 

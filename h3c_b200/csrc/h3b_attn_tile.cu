@@ -35,19 +35,20 @@
 // shared memory.
 //
 // Measured (B200; TFLOP/s of visible pairs): frames of the 6,144-token step (24 heads, three frames and the first) 191-198 us
-// = 1170-1210, 226 us in a long run at the 1000 W limit; 50,220-token video (eight frames back and the first) 7.5-7.8 ms =
-// 1100-1130, at the limit all the time; full attention over 6,144 tokens 367-380 us against 355-360 of k_attn, which needs
-// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 76-83 us = 570-625; a frame of
+// = 1170-1210, 226-239 us in a long run at the 1000 W limit; 50,220-token video (eight frames back and the first) 7.5-7.8 ms =
+// 1100-1130, at the limit all the time; full attention over 6,144 tokens 379-381 us against 360 of k_attn, which needs
+// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 76-108 us = 440-625 (differs from
+// machine to machine and between runs, for a reason not found); a frame of
 // 1,620 queries over 50,220 cached tokens 0.99-1.03 ms = 970-1010; prompts and tokens of 9 sequences, windows of 2,048 and
 // 64 sinks 127-136 us.  Per key tile of both row tiles: 3,230 cycles (16-bit), 3,780 (8-bit, where the widened tiles are
 // written and the codes read beside the operands in shared memory), 2,048 of them products: the chain scores -> softmax ->
-// P V -> next scores of a row tile bounds it, as in k_attn.  A tile with masks takes about 1,000 cycles more.
+// P V -> next scores of a row tile bounds it, as in k_attn.
 // Measured and rejected:
 //   - warps of their own that divide and store finished rows: 16-bit the same within 1 %, 8-bit (the widening warps) 10 % slower;
-//   - row tiles of the last, partly empty round as items of their own: 76.2 against 77.3 us (56 heads over 8);
-//   - a share of the exponentials on the FMA pipe (ex2_emu2): 1 to 4 % slower here;
-//   - a widening loop unrolled over its four quarters: 8-bit 25 % slower (instruction cache);
-//   - claiming the next item at the start of the current one: 174 against 133 us (ragged cache).
+//   - row tiles of the last, partly empty round as items of their own: 76.2 against 77.3 us (56 heads over 8), less than that case varies;
+//   - a share of the exponentials on the FMA pipe (ex2_emu2): of eight, one 1 to 1.5 % slower, three 6 to 9, four 7 to 12;
+//   - a widening loop unrolled over its four quarters: 2,115 against 1,713 us (a frame over 50,220 cached tokens; instruction cache);
+//   - claiming the next item at the start of the current one: 175 against 133 us (ragged cache).
 #include <algorithm>
 #include <type_traits>
 
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     }
                     // The next item is asked for when the scores of the last tile but one have been, some 5 us before the end:
                     // early enough for its first tiles, late enough that a CTA with a long item does not hold one back from
-                    // CTAs that are through (asking at the start left some SMs with four items and others with one: 174 us
+                    // CTAs that are through (asking at the start left some SMs with four items and others with one: 175 us
                     // instead of 133 for the ragged cache).
                     if (it.n_kv > 2) {
                         const long long since = clock64();
@@ -913,9 +914,10 @@ int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t 
     const size_t tiles = std::max<size_t>(ceil_div(attn_window_keys(a.win, len, std::min<size_t>(a.max_rows, 2 * (size_t)queries)), wtile::BN), 1);
     p.row_tiles = (int)row_tiles;
     p.wide_stores = ((uintptr_t)a.out % 32 == 0) && (a.o_rs | a.o_hs) % 16 == 0;
-    // Heads first puts the long items of all heads in front, which evens out the end (6,144-token frames 238 -> 208 us,
-    // ragged cache 176 -> 152); row tiles first lets neighbours share keys in L2, which matters once all keys together
-    // do not fit it (50,220-token video: 7.98 ms against 8.82).
+    // Heads first puts the long items of all heads in front, which evens out the end; row tiles first lets neighbours share
+    // keys in L2, which matters once all keys together do not fit it.  Measured (us, heads first | row tiles first): frames of
+    // the 6,144-token step 196 | 209, ragged cache 127 | 131, 50,220-token video 8,500 | 7,650; against the rule only 56 heads
+    // over 8 with 1,078-key windows, 108 | 96, whose items are all of one length.
     p.heads_first = len * a.n_seq * a.kv_heads * (kv8 ? 256 : 512) <= (128u << 20);
     int (*launch)(h3_cuda *, const TileParams &, size_t, char *, size_t);
     if (kv8) launch = f16 ? launch_tile_t<__half, true> : launch_tile_t<__nv_bfloat16, true>;
