@@ -37,8 +37,8 @@
 // Measured (B200; TFLOP/s of visible pairs): frames of the 6,144-token step (24 heads, three frames and the first) 191-198 us
 // = 1170-1210, 226-239 us in a long run at the 1000 W limit; 50,220-token video (eight frames back and the first) 7.5-7.8 ms =
 // 1100-1130, at the limit all the time; full attention over 6,144 tokens 379-381 us against 360 of k_attn, which needs
-// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 76-108 us = 440-625 (differs from
-// machine to machine and between runs, for a reason not found); a frame of
+// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 75 us = 630 at 1,965 MHz,
+// 93-95 right after work that had run into the power limit; a frame of
 // 1,620 queries over 50,220 cached tokens 0.99-1.03 ms = 970-1010; prompts and tokens of 9 sequences, windows of 2,048 and
 // 64 sinks 127-136 us.  Per key tile of both row tiles: 3,230 cycles (16-bit), 3,780 (8-bit, where the widened tiles are
 // written and the codes read beside the operands in shared memory), 2,048 of them products: the chain scores -> softmax ->
@@ -46,7 +46,7 @@
 // Measured and rejected:
 //   - warps of their own that divide and store finished rows: 16-bit the same within 1 %, 8-bit (the widening warps) 10 % slower;
 //   - row tiles of the last, partly empty round as items of their own: 76.2 against 77.3 us (56 heads over 8), less than that case varies;
-//   - a share of the exponentials on the FMA pipe (ex2_emu2): of eight, one 1 to 1.5 % slower, three 6 to 9, four 7 to 12;
+//   - a share of the exponentials on the FMA pipe (ex2_emu2): of eight, one 0.7 to 1.5 % slower, three 6 to 9, four 7 to 12;
 //   - a widening loop unrolled over its four quarters: 2,115 against 1,713 us (a frame over 50,220 cached tokens; instruction cache);
 //   - claiming the next item at the start of the current one: 175 against 133 us (ragged cache).
 #include <algorithm>
@@ -916,8 +916,8 @@ int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t 
     p.wide_stores = ((uintptr_t)a.out % 32 == 0) && (a.o_rs | a.o_hs) % 16 == 0;
     // Heads first puts the long items of all heads in front, which evens out the end; row tiles first lets neighbours share
     // keys in L2, which matters once all keys together do not fit it.  Measured (us, heads first | row tiles first): frames of
-    // the 6,144-token step 196 | 209, ragged cache 127 | 131, 50,220-token video 8,500 | 7,650; against the rule only 56 heads
-    // over 8 with 1,078-key windows, 108 | 96, whose items are all of one length.
+    // the 6,144-token step 198 | 210, ragged cache 126 | 131, 56 heads over 8 with 1,078-key windows 75.3 | 76.5; the other
+    // way a frame over 50,220 cached tokens 1,006-1,016 | 985-1,001 and the 50,220-token video 8,525 | 7,650.
     p.heads_first = len * a.n_seq * a.kv_heads * (kv8 ? 256 : 512) <= (128u << 20);
     int (*launch)(h3_cuda *, const TileParams &, size_t, char *, size_t);
     if (kv8) launch = f16 ? launch_tile_t<__half, true> : launch_tile_t<__nv_bfloat16, true>;
