@@ -25,8 +25,11 @@ static int fill(WinArgs &a, h3_cuda *cuda, const char *who, int dtype, const voi
         return fail(error, error_size, "%s: pointers must be 16-byte aligned and strides multiples of 8 elements", who);
     if (!q_rs || !q_hs || !o_rs || !o_hs) return fail(error, error_size, "%s: row and head strides must be given", who);
     if ((q_rs | q_hs | o_rs | o_hs) >> 39) return fail(error, error_size, "%s: stride too large", who);
-    if ((rows > 1 && o_rs < 128) || (heads > 1 && o_hs < 128)) return fail(error, error_size, "%s: rows or heads of the output overlap", who);
     if (rows * (heads / kv_heads) > 0x7fffff00u) return fail(error, error_size, "%s: shape too large", who);
+    // rows of heads or heads of rows, packed or not; divided, because the products may pass 64 bits
+    const bool rows_fit = rows < 2 || o_rs >= 128, heads_fit = heads < 2 || o_hs >= 128;
+    const bool nested = rows < 2 || heads < 2 || (rows_fit && heads_fit && ((o_rs - 128) / o_hs >= heads - 1 || (o_hs - 128) / o_rs >= rows - 1));
+    if (!rows_fit || !heads_fit || !nested) return fail(error, error_size, "%s: rows or heads of the output overlap", who);
     memset(&a, 0, sizeof(a));
     a.q = q; a.out = out;
     a.q_rs = (long long)q_rs; a.q_hs = (long long)q_hs; a.o_rs = (long long)o_rs; a.o_hs = (long long)o_hs;

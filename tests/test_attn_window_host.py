@@ -189,3 +189,25 @@ def test_cache_object_checks_its_tensors():
                 (k.transpose(1, 2), k.transpose(1, 2), s, s), (k, k, s.expand(3, 2, 2)[:, :, :1], s)):
         with pytest.raises(h3c_b200.H3Error):
             h3c_b200.KvCache8(*bad)
+
+
+@pytest.mark.parametrize("rows, heads, orow, oh, overlaps", [
+    (4, 8, 128, 128, True),      # row 1 of head 0 is row 0 of head 1
+    (4, 8, 1016, 128, True),     # rows a piece shorter than their heads
+    (4, 8, 128, 504, True),      # heads a piece shorter than their rows
+    (4, 8, 512, 384, True),
+    (1 << 28, 8, (1 << 39) - 8, 128, False), (1 << 28, 8, 128, (1 << 35) - 8, True),   # products past 64 bits and past 32
+    (4, 8, 1024, 128, False), (4, 8, 2048, 256, False),     # rows of heads, packed and not
+    (4, 8, 128, 512, False), (4, 8, 136, 536, False),       # heads of rows
+    (1, 8, 8, 128, False), (4, 1, 128, 8, False)])          # a stride that nothing uses
+def test_outputs_whose_rows_or_heads_overlap_are_refused(rows, heads, orow, oh, overlaps):
+    """Both entry points share the check; another refusal stands behind it, so that nothing is launched (for the largest
+    counts another one stands before it: 2^28 rows of 8 heads are 2^31 rows of one K/V head)."""
+    large = rows * heads > 0x7fffff00
+    says = refused("h3b_sdpa_window_dev", fake_handle(), window(lq=rows, heads=heads, kv=1, orow=orow, oh=oh, q_pos=-1))
+    assert ("too large" if large else "overlap" if overlaps else "q_pos") in says
+    says = refused("h3b_sdpa_window_dev", fake_handle(), window(lq=rows, heads=heads, kv=heads, orow=orow, oh=oh, q_pos=-1))
+    assert ("overlap" if overlaps else "q_pos") in says
+    says = refused("h3b_kv8_sdpa_dev", fake_handle(), cache(kv_heads=heads),
+                   attention(rows=rows, heads=heads, orow=orow, oh=oh, max_rows=1, max_len=1 << 29))
+    assert ("overlap" if overlaps else "max_len") in says
