@@ -547,6 +547,34 @@ def test_cache_lengths_shorter_than_the_rows_and_max_len_as_a_guess(cuda):
         assert not none.any()
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_long_sums_do_not_drift(cuda, bits):
+    """Positive values, so that nothing cancels, of one page again and again: the weights of one page.  The bound: P in f16
+    and the rounding of the output half a step each; products cut to 2^-25 of the sum, and the sum to 2^-23 of itself per 16
+    keys, over the 32,768 keys of one accumulator; 2^-14 for scores and exponentials."""
+    page, reps = 16384, 256 if bits == 8 else 16
+    g, heads = gen(12), 32
+    cache = cuda.kv8_cache(1, page, 1)
+    cache.k_scale.fill_(1)
+    cache.v_scale.fill_(1)
+    cache.k.copy_(torch.randn(1, 1, page, 128, device="cuda", generator=g).to(torch.float8_e4m3fn))
+    cache.v.copy_((1 + torch.rand(1, 1, page, 128, device="cuda", generator=g)).to(torch.float8_e4m3fn))
+    k, v = cache.k[0, 0].double(), cache.v[0, 0].double()
+    if bits == 8:                                              # one CTA: 4 million tokens
+        q = (0.5 * torch.randn(8, heads, 128, device="cuda", generator=g)).to(HF)
+        table = torch.zeros(1, reps, dtype=torch.int32, device="cuda")
+        got = cuda.kv8_sdpa(cache, q, i32([0, 8]), i32([page * reps]), table, max_rows=8, max_len=1, right=-1)
+    else:                                                      # as many items as fill the chip: 262,144 keys each
+        q = (0.5 * torch.randn(1280, heads, 128, device="cuda", generator=g)).to(HF)
+        kk, vv = (x.to(HF).repeat(reps, 1)[:, None].contiguous() for x in (cache.k[0, 0], cache.v[0, 0]))
+        got = cuda.sdpa_window(q, kk, vv)
+    cuda.check()
+    some = slice(0, q.shape[0] * heads, max(1, q.shape[0] // 8))
+    want = torch.softmax(q.reshape(-1, 128)[some].double() @ k.T * 128 ** -0.5, -1) @ v
+    worst = float((got.view(-1, 128)[some].double() / want - 1).abs().max())
+    assert worst <= 2 * 2.0 ** -11 + 32768 * (2.0 ** -25 + 2.0 ** -27) + 2.0 ** -14, worst
+
+
 def test_bad_extents_and_pages_are_reported_and_touch_nothing(cuda):
     import h3c_b200
     rng, g = np.random.default_rng(10), gen(10)
