@@ -216,9 +216,33 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     auto wait = [&](uint64_t *b, uint32_t parity, int code) -> bool {
         return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, a.status, code)) != 0;
     };
+    // A wait that may last as long as an item, which has no bound of its own (one of 2^29 keys takes 8 s): its limit runs
+    // from the last tile whose scores were asked for, so that it bounds a tile and not the item.  Only where that can be:
+    // in every role it cost the 8-bit kernel 1,063 against 1,034 us (a frame over 50,220 cached tokens), here 1,023 against
+    // 994 and 1,037 against 1,013 on two machines; no other case measured pays more than 0.2 %.
+    auto wait_item = [&](auto done, int code) -> bool {
+        volatile int *progress = &ctl.progress;
+        long long since = clock64();
+        int seen = *progress;
+        bool fine = true;
+        for (uint32_t spins = 1; fine && !done(); spins++) {
+            if (*abort_word) fine = false;
+            else if ((spins & 0xff) == 0) {
+                const int now = *progress;
+                if (now != seen) {
+                    seen = now;
+                    since = clock64();
+                } else if (clock64() - since > H3B_WAIT_CYCLES) {
+                    *abort_word = code;
+                    if (a.status) atomicCAS(a.status, 0, code);
+                    fine = false;
+                }
+            }
+        }
+        return __all_sync(0xffffffffu, fine) != 0;
+    };
     // the k-th item of this CTA; false: no more (or a wait gave up)
-    auto next_item = [&](int k, TileItem &it) -> bool {
-        if (!wait(&ctl.item_full[k & 1], (k >> 1) & 1, H3B_ST_TIMEOUT_OTHER)) return false;
+    auto take_item = [&](int k, TileItem &it) -> bool {
         const int4 *src = reinterpret_cast<const int4 *>(ctl.item[k & 1]);
         const int4 x = src[0], y = src[1], z = src[2];
         it.kvh = x.x; it.s = x.y; it.r0 = x.z; it.r_end = x.w;
@@ -227,6 +251,11 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.item_empty[k & 1]);
         return it.r0 >= 0;
+    };
+    auto next_item = [&](int k, TileItem &it) -> bool { return wait(&ctl.item_full[k & 1], (k >> 1) & 1, H3B_ST_TIMEOUT_OTHER) && take_item(k, it); };
+    // for those that have nothing to do, or are through, long before the item ends
+    auto next_item_early = [&](int k, TileItem &it) -> bool {
+        return wait_item([&] { return mbar_try_wait(&ctl.item_full[k & 1], (k >> 1) & 1); }, H3B_ST_TIMEOUT_OTHER) && take_item(k, it);
     };
     // no row of the item sees key j: j > hi or s <= j < lo
     auto seen_by_any = [&](const TileItem &it, int &hi, int &lo, int &sn) {
@@ -314,7 +343,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             // ------------------------------------------------------------ MMA issuer
             // The whole warp walks the loop, converged; one lane, elected once, issues every tcgen05 instruction.  The
             // stage barriers of the next iteration are polled behind an issued block, while the queue drains.
-            // Its waits are not voted on: a lane that gives up alone leaves the loop alone, and nothing in it is collective.
+            // Its waits are not voted on: nothing within an item is collective, and a lane that gives up alone meets the others
+            // at the end of the item (theirs end too, since a wait that cannot be met looks at abort_word).
             auto poll = [&](uint64_t *b, uint32_t parity, int code) -> bool { return mbar_wait(b, parity, abort_word, a.status, code); };
             const bool lead = elect_one();
             constexpr uint32_t idesc_s = umma_idesc(1, Elem<E>::FMT, Elem<E>::FMT, BM, BN, 0, 0);
@@ -346,14 +376,13 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 const int n_kv = it.n_kv, n_tiles = it.row_tiles(p.bm);
                 if (!n_kv) continue;
                 ok = poll(&ctl.q_full, q & 1, H3B_ST_TIMEOUT_OTHER) && poll(&ctl.k_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL);
-                if (!ok) break;
                 tc_fence_after();
-                for (int t = 0; t < n_tiles; t++) issue_s(t, c & 1);
-                if (lead) {
+                for (int t = 0; t < n_tiles && ok; t++) issue_s(t, c & 1);
+                if (ok && lead) {
                     tc_commit(&ctl.k_empty[c & 1]);
                     if (n_kv == 1) tc_commit(&ctl.q_empty);
                 }
-                ok = poll(&ctl.v_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL) &&
+                ok = ok && poll(&ctl.v_full[c & 1], (c >> 1) & 1, H3B_ST_TIMEOUT_FULL) &&
                      (n_kv < 2 || poll(&ctl.k_full[(c + 1) & 1], ((c + 1) >> 1) & 1, H3B_ST_TIMEOUT_FULL));
                 auto step = [&](int j, auto stage_c) {
                     constexpr int st = decltype(stage_c)::value, nx = st ^ 1;
@@ -394,6 +423,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 q++;
                 pc[0] += n_kv;
                 if (n_tiles == 2) pc[1] += n_kv;
+                ok = __all_sync(0xffffffffu, ok) != 0;                   // here the lanes meet again
             }
         } else {
             // ------------------------------------------------------------ Q, items, value rows that nobody sees
@@ -447,7 +477,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             };
             int q = 0;
             if (warp == 2) {
-                for (int k = 0; ok && next_item(k, it); k++)
+                for (int k = 0; ok && next_item_early(k, it); k++)
                     if (it.n_kv) {
                         ok = load_q(it, q) && (!CONVERT || convert_q(it, q));
                         q++;
@@ -518,7 +548,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         for (int j = 0; j < it.n_kv && ok; j++) {
                             const int st = (c + j) & 1, key = it.key(j);
                             if (!edge(key, it.n, hi, lo, sn)) continue;
-                            ok = wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1, H3B_ST_TIMEOUT_FULL);
+                            // tiles that need no cleaning lie in between
+                            ok = wait_item([&] { return mbar_try_wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1); }, H3B_ST_TIMEOUT_FULL);
                             if (!ok) break;
                             if (st) raw[1]++;
                             else raw[0]++;
@@ -537,17 +568,12 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     // CTAs that are through (asking at the start left some SMs with four items and others with one: 175 us
                     // instead of 133 for the ragged cache).
                     if (it.n_kv > 2) {
-                        const long long since = clock64();
-                        while (ok && *reinterpret_cast<volatile int *>(&ctl.progress) < c + it.n_kv - 1) {
+                        const int until = c + it.n_kv - 1;
+                        ok = ok && wait_item([&] {
+                            if (*reinterpret_cast<volatile int *>(&ctl.progress) >= until) return true;
                             __nanosleep(100);
-                            if (*abort_word) ok = false;
-                            else if (clock64() - since > H3B_WAIT_CYCLES) {   // as long as any other wait
-                                *abort_word = H3B_ST_TIMEOUT_OTHER;
-                                if (a.status && lane == 0) atomicCAS(a.status, 0, H3B_ST_TIMEOUT_OTHER);
-                                ok = false;
-                            }
-                        }
-                        ok = __all_sync(0xffffffffu, ok) != 0;
+                            return false;
+                        }, H3B_ST_TIMEOUT_OTHER);
                     }
                     c += it.n_kv;
                     if (ok) ok = find(false, it) && publish(k, it);
@@ -563,7 +589,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         const uint32_t s_addr = tmem_base + lane_base + S_COL + 128u * t, o_addr = tmem_base + lane_base + O_COL + 128u * t;
         TileItem it;
         int c = 0, mine = 0, q = 0, mine_q = 0;                          // tiles and items with keys so far, and those of this row tile
-        for (int k = 0; ok && next_item(k, it); k++) {
+        for (int k = 0; ok && next_item_early(k, it); k++) {
             const int n_kv = it.n_kv;
             if (t >= it.row_tiles(p.bm)) {
                 c += n_kv;
@@ -942,7 +968,8 @@ int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t 
     }
     const size_t sms = (size_t)cuda->sm_count, row_tiles = ceil_div((size_t)a.max_rows, 2 * (size_t)queries);
     const size_t items = row_tiles * a.kv_heads * a.n_seq;
-    if (items > 0x7fffffffu / 8) return fail(error, error_size, "windowed attention: shape too large");
+    // (so many that passing over those without rows stays within the limit of a wait)
+    if (items > (1u << 26)) return fail(error, error_size, "windowed attention: shape too large");
     const size_t tiles = std::max<size_t>(ceil_div(attn_window_keys(a.win, len, std::min<size_t>(a.max_rows, 2 * (size_t)queries)), wtile::BN), 1);
     p.row_tiles = (int)row_tiles;
     p.wide_stores = ((uintptr_t)a.out % 32 == 0) && (a.o_rs | a.o_hs) % 16 == 0;

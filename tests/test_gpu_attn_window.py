@@ -575,6 +575,25 @@ def test_long_sums_do_not_drift(cuda, bits):
     assert worst <= 2 * 2.0 ** -11 + 32768 * (2.0 ** -25 + 2.0 ** -27) + 2.0 ** -14, worst
 
 
+def test_an_item_that_runs_longer_than_a_wait_may(cuda):
+    """200 million tokens of one sequence (one page, listed again and again) that a small max_len leaves to one CTA: some
+    1.6 million key tiles, about 3 s, while a wait gives up after 4e9 cycles, some 2 s, without any progress.  Keys of zero
+    make every probability 1, so that a row's sums are its keys times a power of two: exact in one accumulator (32,768 keys)
+    and, as multiples of 32,768 (64) below 2^39 (2^30), in what adds them up, but for the last tile, where one rounding of
+    2^-24 is less than half a step of the output."""
+    n, page, rows, heads = 200_000_000, 65536, 8, 32
+    cache = cuda.kv8_cache(1, page, 1)
+    values = 2.0 ** (torch.arange(128, device="cuda") % 5 - 3) * (1 - 2 * (torch.arange(128, device="cuda") % 2))
+    cache.k_scale.fill_(1)
+    cache.v_scale.fill_(1)
+    cache.v.copy_(values.expand(1, 1, page, 128).to(torch.float8_e4m3fn))
+    table = torch.zeros(1, -(-n // page), dtype=torch.int32, device="cuda")
+    q = normal(gen(3), rows, heads, 128, dtype=BF)
+    out = cuda.kv8_sdpa(cache, q, i32([0, rows]), i32([n]), table, max_rows=rows, max_len=1)
+    cuda.check()
+    assert torch.equal(out.float().view(rows, heads, 128), values.float().expand(rows, heads, 128))
+
+
 def test_bad_extents_and_pages_are_reported_and_touch_nothing(cuda):
     import h3c_b200
     rng, g = np.random.default_rng(10), gen(10)
