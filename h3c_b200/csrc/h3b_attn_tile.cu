@@ -875,6 +875,10 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         }
     }
 
+    // A wait gave up: copies and products that are under way (microseconds) still write to this CTA's memory.  Whoever saw it
+    // waits 1 ms before the others are let out.
+    if (*abort_word)
+        for (const long long since = clock64(); clock64() - since < 2000000;) __nanosleep(1000);
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
