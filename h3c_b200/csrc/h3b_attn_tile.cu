@@ -34,13 +34,13 @@
 // Few items and many keys: the keys are split over the CTAs of a cluster (one item each), whose partial results meet in
 // shared memory.
 //
-// Measured (B200; TFLOP/s of visible pairs): frames of the 6,144-token step (24 heads, three frames and the first) 191-198 us
-// = 1170-1210, 226-239 us in a long run at the 1000 W limit; 50,220-token video (eight frames back and the first) 7.5-7.8 ms =
-// 1100-1130, at the limit all the time; full attention over 6,144 tokens 379-381 us against 360 of k_attn, which needs
-// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 75 us = 630 at 1,965 MHz,
+// Measured (B200; TFLOP/s of visible pairs): frames of the 6,144-token step (24 heads, three frames and the first) 195-199 us
+// = 1165-1190, 226-239 us in a long run at the 1000 W limit; 50,220-token video (eight frames back and the first) 7.6-7.8 ms =
+// 1100-1125, at the limit all the time; full attention over 6,144 tokens 379-381 us against 360 of k_attn, which needs
+// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 76-77 us = 620 at 1,965 MHz,
 // 93-95 right after work that had run into the power limit; a frame of
-// 1,620 queries over 50,220 cached tokens 0.99-1.03 ms = 970-1010; prompts and tokens of 9 sequences, windows of 2,048 and
-// 64 sinks 127-136 us.  Per key tile of both row tiles: 3,230 cycles (16-bit), 3,780 (8-bit, where the widened tiles are
+// 1,620 queries over 50,220 cached tokens 1.02-1.04 ms = 960-980; prompts and tokens of 9 sequences, windows of 2,048 and
+// 64 sinks 131-132 us.  Per key tile of both row tiles, before the sums were folded (below): 3,230 cycles (16-bit), 3,780 (8-bit, where the widened tiles are
 // written and the codes read beside the operands in shared memory), 2,048 of them products: the chain scores -> softmax ->
 // P V -> next scores of a row tile bounds it, as in k_attn.
 // Measured and rejected:

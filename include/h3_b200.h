@@ -483,7 +483,7 @@ int h3b_sdpa_strided_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row
  *     j <= b + block - 1 + right  and  (j >= b - left  or  j < sinks).
  * A negative left or right does not bound that side (-1, -1, 0, 1: full attention; -1, 0, 0, 1: causal).  A row that
  * sees no key is zero.  What masked keys hold (NaN, infinities) has no part in the result.  lq = 0 does nothing; out
- * must not overlap the inputs; nothing is allocated, so the call can be captured. */
+ * must not overlap the inputs or itself; nothing is allocated, so the call can be captured. */
 typedef struct {
     const void *d_q, *d_k, *d_v;
     void *d_out;
@@ -502,8 +502,8 @@ int h3b_window_tiles(size_t keys, int64_t pos0, size_t rows, int64_t left, int64
 /* Addition: a paged key/value cache held in 8 bits.  The caller owns the memory (16-byte aligned codes):
  *   d_k, d_v              E4M3 codes [pages][kv_heads][page_tokens][128]
  *   d_k_scale, d_v_scale  f32        [pages][kv_heads][page_tokens / 64], one scale per 64 tokens and head
- * value = code * scale, scales positive (or NaN, see below); page_tokens is a multiple of 64; pages * kv_heads * page_tokens < 2^31.  The pages of sequence
- * s are table[s * table_stride ...], its token t lies in page t / page_tokens of that list; pages that no call needs
+ * value = code * scale, scales positive (or NaN, see below); page_tokens is a multiple of 64; pages * kv_heads *
+ * page_tokens < 2^31.  The pages of sequence s are table[s * table_stride ...], its token t lies in page t / page_tokens of that list; pages that no call needs
  * (behind the length, or wholly outside the window) may hold any index.  A sequence's rows are rows cu_rows[s] ..
  * cu_rows[s + 1] - 1 of the 16-bit tensors.  These tables are int32 on the device, so that a captured call follows
  * them; max_rows bounds the rows of any one sequence.  A sequence whose rows, length or page indices lie outside the
@@ -515,7 +515,8 @@ typedef struct {
 } h3b_kv8_cache;
 /* Puts k / v rows [rows, kv_heads, 128] (bf16 or f16) behind the first d_start[s] tokens of each sequence.  The scale of
  * 64 tokens is the smallest power of two 2^e, e >= -64, with absmax <= 448 * 2^e; a block that already holds tokens in
- * front of the new ones keeps its scale or raises it (their codes are then moved to the raised one).  Tokens of the
+ * front of the new ones keeps its scale or raises it (their codes are then moved to the raised one; a scale does not come
+ * down again when d_start goes back, over drafted tokens that were not taken, say).  Tokens of the
  * block behind the new ones are left as they are.  A non-finite value makes its block's scale NaN (codes zero) until
  * the block is started again.  No page may be written for two sequences, or twice for one, in one call. */
 typedef struct {
@@ -529,8 +530,10 @@ int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_
                        size_t error_size);
 /* Attention of q rows [rows, heads, 128] over the cache: sequence s has d_len[s] tokens and its rows are the last ones of
  * them (row i of nq at position d_len[s] - nq + i); windows as in h3b_sdpa_window_dev.  Rows of out that belong to no
- * sequence are left as they are.  max_len (a bound on d_len[], or an estimate: its rows' values do not depend on it beyond rounding) only guides
- * how the work is split. */
+ * sequence are left as they are.  max_len (a bound on d_len[], or an estimate) only guides how the work is split, and so
+ * the order of the sums.  With up to 16 rows per K/V head, sums of values that do not cancel come out low by 5e-4 at a
+ * million visible tokens where the keys are not split (2e-3 at four million); split over the chip, by a true max_len
+ * and few sequences, 4e-5 (2e-4; 1e-3 at 16 million).  With more rows it is 1.5e-4 at any length. */
 typedef struct {
     const void *d_q;
     void *d_out;
