@@ -37,10 +37,10 @@
 // Measured (B200; TFLOP/s of visible pairs): frames of the 6,144-token step (24 heads, three frames and the first) 195-199 us
 // = 1165-1190, 226-239 us in a long run at the 1000 W limit; 50,220-token video (eight frames back and the first) 7.6-7.8 ms =
 // 1100-1125, at the limit all the time; full attention over 6,144 tokens 379-381 us against 360 of k_attn, which needs
-// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 76-77 us = 620 at 1,965 MHz,
+// no edge, item and maximum-of-nothing arithmetic; 56 heads over 8, windows of 1,078 keys 76 us = 630 at 1,965 MHz,
 // 93-95 right after work that had run into the power limit; a frame of
-// 1,620 queries over 50,220 cached tokens 1.02-1.04 ms = 960-980; prompts and tokens of 9 sequences, windows of 2,048 and
-// 64 sinks 131-132 us.  Per key tile of both row tiles, before the sums were folded (below): 3,230 cycles (16-bit), 3,780 (8-bit, where the widened tiles are
+// 1,620 queries over 50,220 cached tokens 1.02-1.05 ms = 955-980; prompts and tokens of 9 sequences, windows of 2,048 and
+// 64 sinks 127 us.  Per key tile of both row tiles, before the sums were folded (below): 3,230 cycles (16-bit), 3,780 (8-bit, where the widened tiles are
 // written and the codes read beside the operands in shared memory), 2,048 of them products: the chain scores -> softmax ->
 // P V -> next scores of a row tile bounds it, as in k_attn.
 // Measured and rejected:
@@ -150,7 +150,8 @@ struct TileItem {
     __device__ __forceinline__ int row_tiles(int bm) const { return r_end - r0 > bm ? 2 : 1; }
 };
 
-template <typename T, bool KV8>
+// LONG: an item may have more than FOLD key tiles
+template <typename T, bool KV8, bool LONG>
 __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __grid_constant__ TileParams p) {
     using namespace wtile;
     using C = TileCfg<KV8>;
@@ -218,8 +219,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     };
     // A wait that may last as long as an item, which has no bound of its own (one of 2^29 keys takes 8 s): its limit runs
     // from the last tile whose scores were asked for, so that it bounds a tile and not the item.  Only where that can be:
-    // in every role it cost the 8-bit kernel 1,063 against 1,034 us (a frame over 50,220 cached tokens), here 1,023 against
-    // 994 and 1,037 against 1,013 on two machines; no other case measured pays more than 0.2 %.
+    // in every role it cost the 8-bit kernel 1,063 against 1,034 us (a frame over 50,220 cached tokens).
     auto wait_item = [&](auto done, int code) -> bool {
         volatile int *progress = &ctl.progress;
         long long since = clock64();
@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     auto next_item = [&](int k, TileItem &it) -> bool { return wait(&ctl.item_full[k & 1], (k >> 1) & 1, H3B_ST_TIMEOUT_OTHER) && take_item(k, it); };
     // for those that have nothing to do, or are through, long before the item ends
     auto next_item_early = [&](int k, TileItem &it) -> bool {
+        if (!LONG) return next_item(k, it);
         return wait_item([&] { return mbar_try_wait(&ctl.item_full[k & 1], (k >> 1) & 1); }, H3B_ST_TIMEOUT_OTHER) && take_item(k, it);
     };
     // no row of the item sees key j: j > hi or s <= j < lo
@@ -549,7 +550,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                             const int st = (c + j) & 1, key = it.key(j);
                             if (!edge(key, it.n, hi, lo, sn)) continue;
                             // tiles that need no cleaning lie in between
-                            ok = wait_item([&] { return mbar_try_wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1); }, H3B_ST_TIMEOUT_FULL);
+                            if (LONG) ok = wait_item([&] { return mbar_try_wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1); }, H3B_ST_TIMEOUT_FULL);
+                            else ok = wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1, H3B_ST_TIMEOUT_FULL);
                             if (!ok) break;
                             if (st) raw[1]++;
                             else raw[0]++;
@@ -608,8 +610,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             // many keys comes out low, by 6e-9 of itself per key where nothing cancels (measured: 3.4e-4 at 65,536 keys, 6.5e-3
             // at a million; at 2^26 equal keys it stands still).  So it starts anew every FOLD tiles, and what it was is added
             // up here, in local memory: 128 KiB a CTA every 0.5 ms.  The bias stays at 1.5e-4 then (4 million keys of one CTA), for
-            // code that costs frames of the 6,144-token step 0.3 %, a frame over 50,220 cached tokens and the ragged cache 3 %;
-            // a loop of its own beside the rescaling costs 1 to 2 % more.
+            // code that costs a frame over 50,220 cached tokens 2 to 3 % (a loop of its own beside the rescaling 4).
             float far[HD], far_scale = 1.0f;                             // far_scale: what the maximum's growth makes of far
             for (int j = 0; j < n_kv; j++) {
                 const int key = it.key(j);
@@ -673,14 +674,14 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 if (mx != mx) l_run = mx;                                // undefined, and so is the row from here on
                 const float m_new = fmaxf(m_run, mx);
                 const bool grow = m_new > m_run + 8.0f;                  // also at the first visible key: m_run = -inf
-                const bool fold = j && j % FOLD == 0;
+                const bool fold = LONG && j && j % FOLD == 0;
                 if (__any_sync(0xffffffffu, grow) || fold) {
                     float alpha = 1.0f;
                     if (grow) {
                         alpha = ex2_approx(m_run - m_new);
                         m_run = m_new;
                         l_run *= alpha;
-                        far_scale *= alpha;
+                        if (LONG) far_scale *= alpha;
                     }
                     __syncwarp();
                     // s_full of tile j came behind the P V product of tile j - 1: the accumulator is at rest
@@ -753,7 +754,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             mine_q += n_kv > 0;
             tc_fence_after();
             const bool seen = live && h3b_win_count(wr) > 0;
-            if (n_kv > FOLD) {
+            if (LONG && n_kv > FOLD) {
 #pragma unroll 1
                 for (int ch = 0; ch < HD / 16; ch++) {
                     uint32_t o[16];
@@ -924,8 +925,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     }
 }
 
-template <typename T, bool KV8> static int launch_tile_t(h3_cuda *cuda, const TileParams &p, size_t items, char *error, size_t error_size) {
-    void (*kernel)(const TileParams) = k_attn_tile<T, KV8>;
+template <typename T, bool KV8, bool LONG> static int launch_tile_t(h3_cuda *cuda, const TileParams &p, size_t items, char *error, size_t error_size) {
+    void (*kernel)(const TileParams) = k_attn_tile<T, KV8, LONG>;
     static std::atomic<uint64_t> done;
     if (!smem_once(cuda, done, (const void *)kernel, wtile::smem_bytes<KV8>(), "attention smem attribute", error, error_size)) return 0;
     cudaLaunchConfig_t cfg;
@@ -983,8 +984,17 @@ int launch_attn_tile(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t 
     // way a frame over 50,220 cached tokens 1,006-1,016 | 985-1,001 and the 50,220-token video 8,525 | 7,650.
     p.heads_first = len * a.n_seq * a.kv_heads * (kv8 ? 256 : 512) <= (128u << 20);
     int (*launch)(h3_cuda *, const TileParams &, size_t, char *, size_t);
-    if (kv8) launch = f16 ? launch_tile_t<__half, true> : launch_tile_t<__nv_bfloat16, true>;
-    else launch = f16 ? launch_tile_t<__half, false> : launch_tile_t<__nv_bfloat16, false>;
+    // The most key tiles that an item can have, whatever the lengths on the device are: its rows' windows (their blocks may
+    // begin a block apart) and the sinks, each rounded up to tiles, or all keys that there can be.  Up to FOLD of them need
+    // neither folded sums nor waits of their own.  Measured (us, without | with them): ragged cache 127 | 131, 56 heads over 8
+    // 75.7 | 76.6, frames of the 6,144-token step 195.8 | 196.9, 50,220-token video 7,630 | 7,685.
+    const size_t capacity = kv8 ? (size_t)a.table_stride * a.page_blocks * KV8_BLOCK : (size_t)a.lk;
+    const size_t reach = attn_window_keys(a.win, capacity, std::min<size_t>(a.max_rows, 2 * (size_t)queries) + (size_t)a.win.block);
+    const bool is_long = reach / wtile::BN + 4 > (size_t)wtile::FOLD;
+    if (kv8) launch = f16 ? (is_long ? launch_tile_t<__half, true, true> : launch_tile_t<__half, true, false>)
+                          : (is_long ? launch_tile_t<__nv_bfloat16, true, true> : launch_tile_t<__nv_bfloat16, true, false>);
+    else launch = f16 ? (is_long ? launch_tile_t<__half, false, true> : launch_tile_t<__half, false, false>)
+                      : (is_long ? launch_tile_t<__nv_bfloat16, false, true> : launch_tile_t<__nv_bfloat16, false, false>);
     // Whole rounds of one item per SM run unsplit; what is left over, if it is less than half a round of one sequence's
     // long items, has its keys split so that it fills the chip too (a frame of 1,620 queries over 50,220 cached tokens,
     // 168 items: 1593 us unsplit, 1121 to 1249 split by 3 to 6 as a whole).

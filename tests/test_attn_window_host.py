@@ -5,6 +5,7 @@ import ctypes as C
 import itertools
 from pathlib import Path
 
+import numpy as np
 import pytest
 
 import h3c_b200
@@ -211,3 +212,19 @@ def test_outputs_whose_rows_or_heads_overlap_are_refused(rows, heads, orow, oh, 
     says = refused("h3b_kv8_sdpa_dev", fake_handle(), cache(kv_heads=heads),
                    attention(rows=rows, heads=heads, orow=orow, oh=oh, max_rows=1, max_len=1 << 29))
     assert ("overlap" if overlaps else "max_len") in says
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_tiles_of_an_item_stay_within_the_bound_that_picks_the_kernel(seed):
+    """The host decides by count <= reach // 128 + 4, with reach the sum of left, right, two blocks, rows and sinks, or all
+    keys; a side without a bound counts as 2^29."""
+    rng, lib, far = np.random.default_rng(seed), h3c_b200.load(), 1 << 29
+    s, f, c = C.c_int(), C.c_int(), C.c_int()
+    for _ in range(5000):
+        n, rows = int(rng.integers(1, [5000, 200000][rng.integers(2)])), int(rng.integers(1, 257))
+        pos = int(rng.integers(0, n + 500))
+        left, right = (int(rng.choice([-1, 0, rng.integers(0, 3000)])) for _ in range(2))
+        block, sinks = int(rng.choice([1, rng.integers(1, 4000)])), int(rng.choice([0, rng.integers(0, 3000)]))
+        assert lib.h3b_window_tiles(n, pos, rows, left, right, sinks, block, 128, C.byref(s), C.byref(f), C.byref(c)) == 1
+        reach = min(sum(far if x < 0 else x for x in (left, right)) + 2 * block + rows + sinks, n)
+        assert c.value <= reach // 128 + 4
