@@ -305,8 +305,12 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         if (j % 16 == 0) {
                             bi = -1;
                             if (j + (lane >> 1) < it.n_kv) {
+                                // half of a tile may lie outside every row's window (before it, or behind the sinks): the page of such a
+                                // half may be anything and is not looked up; the widening warps zero its rows
+                                int hi, lo, sn;
+                                seen_by_any(it, hi, lo, sn);
                                 const int blk = it.key(j + (lane >> 1)) / KV8_BLOCK + (lane & 1);
-                                if (blk * KV8_BLOCK < it.n) bi = (int)kv8_block_index(a, it.s, blk, it.kvh);
+                                if (h3b_win_any(hi, lo, sn, blk * KV8_BLOCK, KV8_BLOCK)) bi = (int)kv8_block_index(a, it.s, blk, it.kvh);
                             }
                             bks = bi >= 0 ? __ldg(a.ks + bi) : 1.0f;
                             const float vs = bi >= 0 ? __ldg(a.vs + bi) : 1.0f;
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                                     ctl.scales[c & 3] = sc;
                                     ctl.inv_scales[c & 3] = isc;
                                 }
-                                // a block outside the pool (reported) or behind the last token is not read: its rows are invalid or hidden
+                                // a block outside the pool (reported) or one that no row sees is not read: its rows are invalid or hidden
                                 if (b[w & 1] >= 0) {
                                     mbar_expect_tx(&ctl.c_full[w], CODES / 2);
                                     bulk_load(sC + w * (CODES / 2), (w >> 1 ? a.vc : a.kc) + (long long)b[w & 1] * (CODES / 2), CODES / 2, &ctl.c_full[w]);

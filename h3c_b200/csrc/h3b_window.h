@@ -66,6 +66,11 @@ static H3B_HD h3b_win_tiles h3b_win_tiles_of(h3b_win w, int p0, int p1, int n, i
 
 static H3B_HD int h3b_win_tile(h3b_win_tiles t, int i) { return i < t.sink ? i : t.from + i - t.sink; }
 
+/* some query of a group sees some key of [k0, k0 + unit): hi of its last row, lo of its first, s of its last */
+static H3B_HD int h3b_win_any(int hi, int lo, int s, int k0, int unit) {
+    return k0 <= hi && (k0 + unit > lo || k0 < s);
+}
+
 /* every query at p0..p1 sees every key of [k0, k0 + unit): a is the row of p0, z of p1 */
 static H3B_HD int h3b_win_full(h3b_win_row a, h3b_win_row z, int k0, int unit) {
     return k0 + unit - 1 <= a.hi && (k0 >= z.lo || k0 + unit <= a.s);
