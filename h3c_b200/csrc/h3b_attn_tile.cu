@@ -27,9 +27,10 @@
 // multiplied by anyway, log2 of the value scale part of the offset that is subtracted anyway (P carries the value scale),
 // and the row sum of 64 keys is divided by it once.
 //
-// Values that no row of the item sees are zeroed on their way (a probability of 0 times a NaN of stale memory is not 0);
-// a row that comes out non-finite because of a value that only other rows of its tile see is computed again from its own
-// keys.
+// Values that no row of the item sees are zeroed on their way (a probability of 0 times a NaN of stale memory is not 0).
+// 16-bit: an item with a row that comes out non-finite though its probabilities are finite is done a second time, as a further
+// item of its CTA, with the values that are not finite taken out of the tiles that its rows see in part (OddValues).  The
+// warp that hands out items learns of it two items later, or at the end, so that nothing waits for it in between.
 //
 // Few items and many keys: the keys are split over the CTAs of a cluster (one item each), whose partial results meet in
 // shared memory.
@@ -69,9 +70,12 @@ constexpr int CODES = 128 * 128;                          // E4M3 codes of a til
 struct Control {
     uint64_t q_full, q_empty, q_raw, k_full[2], v_full[2], k_empty[2], v_empty[2], v_raw[2], s_full[2], p_full[4] /* [tile][half] */, o_done[2];
     uint64_t c_full[4], c_empty[4] /* codes of 64 keys: [keys | values][half] */, item_full[2], item_empty[2], clc_full;
+    uint64_t rows_done[4];                                // softmax warps that are through with an item, by item modulo 4
     uint32_t tmem_base;
     int abort_word;
     int progress;                                         // tiles whose scores have been asked for
+    int search;                                           // tiles gone through for values that are not finite
+    int odd[4], cta_of[4];                                // by item modulo 4: it has rows that came out non-finite; CTA of the grid whose item it is
     alignas(16) uint32_t clc[4];
     alignas(16) int item[2][12];
     alignas(16) float4 scales[4];                         // of a tile: key scale of either half, log2 of the value scale of either half
@@ -142,7 +146,7 @@ template <bool KV8> struct TileCfg {
 };
 
 struct TileItem {
-    int kvh, s, r0, r_end, row0, n, pos0, sink, from, n_kv, t_first, nq;
+    int kvh, s, r0, r_end, row0, n, pos0, sink, from, n_kv, t_first, nq;   // s: 8-bit: the sequence; 16-bit: 1 if done a second time
     __device__ __forceinline__ int key(int j) const {                    // first key of the j-th tile
         const int i = t_first + j;
         return (i < sink ? i : from + i - sink) * wtile::BN;
@@ -189,8 +193,14 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             mbar_init(&ctl.item_empty[i], C::ITEM_READERS);
         }
         mbar_init(&ctl.clc_full, 1);
+        for (int i = 0; i < 4; i++) {
+            mbar_init(&ctl.rows_done[i], 8);
+            ctl.odd[i] = 0;
+        }
         ctl.abort_word = 0;
         ctl.progress = 0;
+        ctl.search = 0;
+        ctl.item[1][2] = -1;
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -213,22 +223,42 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         tma_prefetch_desc(&p.map_k);
         tma_prefetch_desc(&p.map_v);
     }
-    // every wait: the whole warp together, bounded
-    auto wait = [&](uint64_t *b, uint32_t parity, int code) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, a.status, code)) != 0;
+    // A bounded wait of one thread.  16-bit, long items: what its limit does not cover is a softmax warp that goes through the
+    // tiles of an item's edges for values that are not finite (tens of millions of keys of one block, say).
+    auto poll = [&](uint64_t *b, uint32_t parity, int code) -> bool {
+        if (KV8 || !LONG) return mbar_wait(b, parity, abort_word, a.status, code);
+        if (mbar_try_wait(b, parity)) return true;
+        volatile int *search = &ctl.search;
+        long long since = clock64();
+        int seen = *search;
+        for (uint32_t spins = 1;; spins++) {
+            if (mbar_try_wait(b, parity)) return true;
+            if (*abort_word) return false;
+            if ((spins & 0x3ff) == 0 && clock64() - since > H3B_WAIT_CYCLES) {
+                if (*search == seen) {
+                    *abort_word = code;
+                    if (a.status) atomicCAS(a.status, 0, code);
+                    return false;
+                }
+                seen = *search;
+                since = clock64();
+            }
+        }
     };
+    // every wait: the whole warp together, bounded
+    auto wait = [&](uint64_t *b, uint32_t parity, int code) -> bool { return __all_sync(0xffffffffu, poll(b, parity, code)) != 0; };
     // A wait that may last as long as an item, which has no bound of its own (one of 2^29 keys takes 8 s): its limit runs
     // from the last tile whose scores were asked for, so that it bounds a tile and not the item.  Only where that can be:
     // in every role it cost the 8-bit kernel 1,063 against 1,034 us (a frame over 50,220 cached tokens).
     auto wait_item = [&](auto done, int code) -> bool {
-        volatile int *progress = &ctl.progress;
+        volatile int *progress = &ctl.progress, *search = &ctl.search;
         long long since = clock64();
-        int seen = *progress;
+        int seen = *progress + (KV8 ? 0 : *search);
         bool fine = true;
         for (uint32_t spins = 1; fine && !done(); spins++) {
             if (*abort_word) fine = false;
             else if ((spins & 0xff) == 0) {
-                const int now = *progress;
+                const int now = *progress + (KV8 ? 0 : *search);
                 if (now != seen) {
                     seen = now;
                     since = clock64();
@@ -258,13 +288,23 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         if (!LONG) return next_item(k, it);
         return wait_item([&] { return mbar_try_wait(&ctl.item_full[k & 1], (k >> 1) & 1); }, H3B_ST_TIMEOUT_OTHER) && take_item(k, it);
     };
+    // what the first and the last row of an item see
+    auto rows_of = [&](const TileItem &it, h3b_win_row &ra, h3b_win_row &rz) {
+        ra = h3b_win_of(a.win, it.pos0 + it.r0 / a.group, it.n);
+        rz = h3b_win_of(a.win, it.pos0 + (it.r_end - 1) / a.group, it.n);
+    };
     // no row of the item sees key j: j > hi or s <= j < lo
     auto seen_by_any = [&](const TileItem &it, int &hi, int &lo, int &sn) {
-        const h3b_win_row ra = h3b_win_of(a.win, it.pos0 + it.r0 / a.group, it.n), rz = h3b_win_of(a.win, it.pos0 + (it.r_end - 1) / a.group, it.n);
+        h3b_win_row ra, rz;
+        rows_of(it, ra, rz);
         hi = rz.hi; lo = ra.lo; sn = rz.s;
     };
     // a tile has such keys among those that exist (16-bit: what lies behind the last key comes as zeros)
     auto edge = [&](int key, int end, int hi, int lo, int sn) { return min(key + BN, end) - 1 > hi || max(key, sn) < min(key + BN, lo); };
+    // 16-bit: a tile whose values pass through warp 3
+    auto by_hand = [&](const TileItem &it, int key, const h3b_win_row &ra, const h3b_win_row &rz) {
+        return edge(key, it.n, rz.hi, ra.lo, rz.s) || (it.s && !h3b_win_full(ra, rz, key, BN));
+    };
     bool ok = true;
 
     if (warp < SOFTMAX_WARP) {
@@ -275,8 +315,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             int c = 0;                                                   // tiles so far
             for (int k = 0; ok && next_item(k, it); k++) {
                 if (!KV8) {
-                    int hi, lo, sn;
-                    seen_by_any(it, hi, lo, sn);
+                    h3b_win_row ra, rz;
+                    rows_of(it, ra, rz);
                     for (int j = 0; j < it.n_kv && ok; j++, c++) {
                         const int st = c & 1, key = it.key(j);
                         const uint32_t ph = ((c >> 1) & 1) ^ 1;
@@ -289,8 +329,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         }
                         ok = wait(&ctl.v_empty[st], ph, H3B_ST_TIMEOUT_EMPTY);
                         if (!ok) break;
-                        if (lane == 0) {                                 // edge tiles pass through warp 3
-                            uint64_t *b = edge(key, it.n, hi, lo, sn) ? &ctl.v_raw[st] : &ctl.v_full[st];
+                        if (lane == 0) {
+                            uint64_t *b = by_hand(it, key, ra, rz) ? &ctl.v_raw[st] : &ctl.v_full[st];
                             mbar_expect_tx(b, TILE);
                             tma_load_3d(sV + st * TILE, &p.map_v, b, 0, it.kvh, key);
                             tma_load_3d(sV + st * TILE + SLAB, &p.map_v, b, 64, it.kvh, key);
@@ -350,7 +390,6 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             // stage barriers of the next iteration are polled behind an issued block, while the queue drains.
             // Its waits are not voted on: nothing within an item is collective, and a lane that gives up alone meets the others
             // at the end of the item (theirs end too, since a wait that cannot be met looks at abort_word).
-            auto poll = [&](uint64_t *b, uint32_t parity, int code) -> bool { return mbar_wait(b, parity, abort_word, a.status, code); };
             const bool lead = elect_one();
             constexpr uint32_t idesc_s = umma_idesc(1, Elem<E>::FMT, Elem<E>::FMT, BM, BN, 0, 0);
             constexpr uint32_t idesc_o = umma_idesc(1, Elem<E>::FMT, Elem<E>::FMT, BM, HD, 0, 1);
@@ -488,9 +527,9 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         q++;
                     }
             } else {
-                // item k of the CTA; `more`: there may be another
-                auto publish = [&](int k, const TileItem &x) -> bool {
-                    if (!wait(&ctl.item_empty[k & 1], ((k >> 1) & 1) ^ 1, H3B_ST_TIMEOUT_EMPTY)) return false;
+                // item k of the CTA
+                auto slot_free = [&](int k) -> bool { return wait(&ctl.item_empty[k & 1], ((k >> 1) & 1) ^ 1, H3B_ST_TIMEOUT_EMPTY); };
+                auto publish = [&](int k, const TileItem &x) {
                     if (lane == 0) {
                         int4 *dst = reinterpret_cast<int4 *>(ctl.item[k & 1]);
                         dst[0] = make_int4(x.kvh, x.s, x.r0, x.r_end);
@@ -498,17 +537,16 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         dst[2] = make_int4(x.from, x.n_kv, x.t_first, x.nq);
                         mbar_arrive(&ctl.item_full[k & 1]);
                     }
-                    return true;
                 };
                 // what CTA x of the grid has to do; false: nothing
                 auto describe = [&](int x, TileItem &d) -> bool {
                     const int i = p.first + x / p.split;
                     const int in_seq = a.kv_heads * p.row_tiles, j = i % in_seq;
-                    d.s = i / in_seq;
+                    d.s = KV8 ? i / in_seq : 0;
                     d.kvh = p.heads_first ? j % a.kv_heads : j / p.row_tiles;
                     // late rows first: under a window that is open to the left they see the most
                     d.r0 = (p.row_tiles - 1 - (p.heads_first ? j / a.kv_heads : j % p.row_tiles)) * (2 * p.bm);
-                    const SeqExt e = seq_ext<KV8>(a, d.s);
+                    const SeqExt e = seq_ext<KV8>(a, d.s);               // (16-bit: there is one)
                     const long long rows = (long long)e.nq * a.group;
                     if (d.r0 >= rows) return false;
                     d.r_end = (int)(rows < d.r0 + 2 * p.bm ? rows : d.r0 + 2 * p.bm);
@@ -521,7 +559,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     return true;
                 };
                 int x = blockIdx.x, asked = 0;
-                bool more = p.split == 1;
+                bool more = p.split == 1;                                // there may be another
                 // the next item with rows in `d`; r0 = -1: none
                 auto find = [&](bool own, TileItem &d) -> bool {
                     d.r0 = -1;
@@ -542,28 +580,73 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     }
                     return true;
                 };
+                // 16-bit: item `done` (the first that has not been looked at) has to be done a second time, as d
+                int done = 0;
+                auto second_time = [&](TileItem &d) -> bool {
+                    volatile int *odd = &ctl.odd[done & 3];
+                    const bool hit = *odd != 0;
+                    const int from = *reinterpret_cast<volatile int *>(&ctl.cta_of[done & 3]);
+                    __syncwarp();
+                    if (lane == 0) *odd = 0;
+                    done++;
+                    if (!hit || !describe(from, d)) return false;
+                    h3b_win_row ra, rz;
+                    rows_of(d, ra, rz);
+                    d.s = 1;
+                    return ra.hi != rz.hi || ra.lo != rz.lo || ra.s != rz.s;   // rows that see the same hold what they see
+                };
+                TileItem next;                                           // found and not yet handed out (r0 = -1: none)
+                // item k: one for the second time, the next one, or none
+                auto choose = [&](int k) -> bool {
+                    if (KV8) return find(k == 0, it) && slot_free(k);
+                    if (next.r0 < 0 && !find(k == 0, next)) return false;
+                    if (!slot_free(k)) return false;
+                    // every warp has taken item k - 2, so the softmax warps are through with item k - 3
+                    while (done + 3 <= k)
+                        if (second_time(it)) return true;
+                    while (next.r0 < 0 && done < k) {
+                        if (!wait(&ctl.rows_done[done & 3], (done >> 2) & 1, H3B_ST_TIMEOUT_OTHER)) return false;
+                        if (second_time(it)) return true;
+                    }
+                    if (lane == 0) ctl.cta_of[k & 3] = x;
+                    it = next;
+                    next.r0 = -1;
+                    return true;
+                };
                 int c = 0, raw[2] = {0, 0};
-                ok = find(true, it) && publish(0, it);
+                next.r0 = -1;
+                ok = choose(0);
+                if (ok) publish(0, it);
                 for (int k = 1; ok && it.r0 >= 0; k++) {
                     if (CONVERT) {
                         if (it.n_kv) ok = convert_q(it, q++);
                     } else if (!KV8) {
-                        int hi, lo, sn;
-                        seen_by_any(it, hi, lo, sn);
+                        h3b_win_row ra, rz;
+                        rows_of(it, ra, rz);
                         for (int j = 0; j < it.n_kv && ok; j++) {
                             const int st = (c + j) & 1, key = it.key(j);
-                            if (!edge(key, it.n, hi, lo, sn)) continue;
+                            if (!by_hand(it, key, ra, rz)) continue;
                             // tiles that need no cleaning lie in between
                             if (LONG) ok = wait_item([&] { return mbar_try_wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1); }, H3B_ST_TIMEOUT_FULL);
                             else ok = wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1, H3B_ST_TIMEOUT_FULL);
                             if (!ok) break;
                             if (st) raw[1]++;
                             else raw[0]++;
-                            for (int i = lane; i < BN; i += 32)
-                                if (key + i > hi || (key + i < lo && key + i >= sn))
+                            for (int i = lane; i < BN; i += 32) {
+                                uint8_t *row = sV + st * TILE + i * 128;
+                                if (key + i > rz.hi || (key + i < ra.lo && key + i >= rz.s)) {
 #pragma unroll
                                     for (int h = 0; h < 16; h++)
-                                        *reinterpret_cast<uint4 *>(sV + st * TILE + (h >> 3) * SLAB + i * 128 + ((h & 7) ^ (i & 7)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                                        *reinterpret_cast<uint4 *>(row + (h >> 3) * SLAB + ((h & 7) ^ (i & 7)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                                } else if (it.s) {
+#pragma unroll 4
+                                    for (int h = 0; h < 16; h++) {
+                                        uint4 *at = reinterpret_cast<uint4 *>(row + (h >> 3) * SLAB + ((h & 7) ^ (i & 7)) * 16);
+                                        const uint4 w = *at;
+                                        *at = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y), finite_or_zero<T>(w.z), finite_or_zero<T>(w.w));
+                                    }
+                                }
+                            }
                             fence_proxy_async_smem();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&ctl.v_full[st]);
@@ -582,7 +665,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         }, H3B_ST_TIMEOUT_OTHER);
                     }
                     c += it.n_kv;
-                    if (ok) ok = find(false, it) && publish(k, it);
+                    ok = ok && choose(k);
+                    if (ok) publish(k, it);
                 }
             }
         }
@@ -597,9 +681,19 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         int c = 0, mine = 0, q = 0, mine_q = 0;                          // tiles and items with keys so far, and those of this row tile
         for (int k = 0; ok && next_item_early(k, it); k++) {
             const int n_kv = it.n_kv;
+            // this warp's rows of the item are through (and, 16-bit, `odd`: one came out non-finite with a finite sum of probabilities)
+            auto rows_done = [&](bool odd) {
+                if (KV8) return;
+                odd = __any_sync(0xffffffffu, odd);
+                if (lane == 0) {
+                    if (odd && !it.s) *reinterpret_cast<volatile int *>(&ctl.odd[k & 3]) = 1;
+                    mbar_arrive(&ctl.rows_done[k & 3]);
+                }
+            };
             if (t >= it.row_tiles(p.bm)) {
                 c += n_kv;
                 q += n_kv > 0;
+                rows_done(false);
                 continue;
             }
             const int slot = t * BM + quarter * 32 + lane;                      // place of this thread's row in the row tiles
@@ -758,6 +852,22 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             mine_q += n_kv > 0;
             tc_fence_after();
             const bool seen = live && h3b_win_count(wr) > 0;
+            // done a second time: `add(x, r)` for every row r of the warp that sees values which were taken out
+            auto give_back = [&](auto add) {
+                h3b_win_row ra, rz;
+                rows_of(it, ra, rz);
+                OddValues x;
+                x.clear();
+                for (int j = 0; j < n_kv; j++) {
+                    const int key = it.key(j);
+                    if (h3b_win_full(ra, rz, key, BN)) continue;
+                    x.template collect<T>(a, it.kvh, key, BN, wr, live, lane);
+                    if (lane == 0) atomicAdd(&ctl.search, 1);
+                }
+                __syncwarp();                                            // the rows written above come first
+                for (int r = 0; r < 32; r++)
+                    if (x.any(r)) add(x, r);
+            };
             if (LONG && n_kv > FOLD) {
 #pragma unroll 1
                 for (int ch = 0; ch < HD / 16; ch++) {
@@ -773,6 +883,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             if (p.split > 1) {
                 // this CTA's share of the row: sums as they are, with their maximum and denominator
                 float *part = reinterpret_cast<float *>(smem) + slot * PART_ROW;
+                bool odd = false;
 #pragma unroll 1
                 for (int ch = 0; ch < HD / 32; ch++) {
                     uint32_t o[32];
@@ -782,10 +893,22 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     for (int i = 0; i < 32; i += 4)
                         *reinterpret_cast<uint4 *>(part + ch * 32 + i) =
                             n_kv ? make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_uint4(0u, 0u, 0u, 0u);
+                    if (!KV8)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) odd |= !(fabsf(__uint_as_float(o[i])) < INFINITY);
                 }
                 float *ml = reinterpret_cast<float *>(smem) + 2 * BM * PART_ROW;
                 ml[slot] = m_run;
                 ml[2 * BM + slot] = l_run;
+                if (!KV8) {
+                    if (it.s) give_back([&](const OddValues &x, int r) {
+                        float4 *at = reinterpret_cast<float4 *>(reinterpret_cast<float *>(smem) + (t * BM + quarter * 32 + r) * PART_ROW + lane * 4);
+                        const float4 y = *at;
+                        *at = make_float4(y.x + x.of(r, 0), y.y + x.of(r, 1), y.z + x.of(r, 2), y.w + x.of(r, 3));
+                    });
+                    fence_proxy_async_smem();                            // done a second time, copies come where the rows are parked
+                    rows_done(seen && n_kv && odd && ordinary(l_run));
+                }
             } else {
                 const float inv_l = 1.0f / l_run;
                 T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.row0 + qi) * a.o_rs + (long long)(it.kvh * a.group + hd) * a.o_hs;
@@ -815,17 +938,13 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     }
                 }
                 if (!KV8) {
-                    uint32_t again = __ballot_sync(0xffffffffu, seen && odd);
-                    if (again) {
-                        SeqExt e;
-                        e.row0 = it.row0; e.nq = it.nq; e.n = it.n; e.pos0 = it.pos0;
-                        __syncwarp();                                    // the rows written above come first
-                        while (again) {
-                            const int l = __ffs(again) - 1;
-                            again &= again - 1;
-                            attn_row_by_warp<T, KV8>(a, it.s, e, __shfl_sync(0xffffffffu, qi, l), it.kvh * a.group + __shfl_sync(0xffffffffu, hd, l), lane);
-                        }
-                    }
+                    if (it.s) give_back([&](const OddValues &x, int r) {
+                        const int row = __shfl_sync(0xffffffffu, qi, r), head = it.kvh * a.group + __shfl_sync(0xffffffffu, hd, r);
+                        uint2 *at = reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + (long long)(it.row0 + row) * a.o_rs + (long long)head * a.o_hs + lane * 4);
+                        const float4 y = load4(reinterpret_cast<const T *>(at));
+                        *at = make_uint2(Elem<T>::pack(y.x + x.of(r, 0), y.y + x.of(r, 1)), Elem<T>::pack(y.z + x.of(r, 2), y.w + x.of(r, 3)));
+                    });
+                    rows_done(seen && odd && ordinary(l_run));
                 }
             }
         }
@@ -892,10 +1011,10 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     }
     if (p.split > 1) {
         // ---- the shares meet: a warp finishes a row, a lane four of its dimensions
-        const int *slot0 = ctl.item[0];                                  // the one item
-        const int kvh = slot0[0], s = slot0[1], r0 = slot0[2], rows = *abort_word ? 0 : slot0[3] - slot0[2];
+        const int *slot0 = ctl.item[ctl.item[0][2] < 0];                 // the one item (the first slot has the end if it was done twice)
+        const int kvh = slot0[0], r0 = slot0[2], rows = *abort_word ? 0 : slot0[3] - slot0[2];
         SeqExt e;
-        e.row0 = slot0[4]; e.n = slot0[5]; e.pos0 = slot0[6]; e.nq = slot0[11];
+        e.row0 = slot0[4]; e.n = slot0[5]; e.pos0 = slot0[6];
         cluster_sync_all();
         const uint32_t base = smem_u32(smem);
         for (int r = rank * (C::THREADS / 32) + warp; r0 >= 0 && r < rows; r += p.split * (C::THREADS / 32)) {
@@ -915,11 +1034,6 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             const bool seen = h3b_win_count(h3b_win_of(a.win, e.pos0 + qi, e.n)) > 0;
             const float inv = 1.0f / l;
             v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-            const bool odd = !(fabsf(v.x) < INFINITY) || !(fabsf(v.y) < INFINITY) || !(fabsf(v.z) < INFINITY) || !(fabsf(v.w) < INFINITY);
-            if (!KV8 && seen && __any_sync(0xffffffffu, odd)) {
-                attn_row_by_warp<T, KV8>(a, s, e, qi, kvh * a.group + hd, lane);
-                continue;
-            }
             T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qi) * a.o_rs + (long long)(kvh * a.group + hd) * a.o_hs;
             uint2 w = make_uint2(0u, 0u);
             if (seen) w = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));

@@ -32,3 +32,108 @@ def test_pages_that_no_row_needs_are_not_looked_at(cuda, rows, n, left, right, s
         got = cuda.kv8_sdpa(cache, q, i32([0, rows]), i32([n]), i32(evicted), max_rows=rows, max_len=n, **w)
         cuda.check()
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ 16-bit values that are not finite
+
+def place(v, where, g):
+    """Puts values that are not finite into a copy of v [n, KV, 128]; returns it."""
+    v, n = v.clone(), v.shape[0]
+    inf, nan = float("inf"), float("nan")
+    if where == "one":
+        v[n // 2 + 3, 0, 77] = inf
+    elif where == "first":
+        v[0, :, 5], v[1, 0, 6] = -inf, nan
+    elif where == "last":
+        v[n - 1, 0, 0], v[n - 2, 0, 0], v[n - 3, 0, 127] = inf, -inf, nan
+    elif where == "some":
+        hit = torch.rand(v.shape, generator=g, device="cuda") < 3e-4
+        pick = torch.tensor([inf, -inf, nan], device="cuda", dtype=v.dtype)[torch.randint(0, 3, v.shape, generator=g, device="cuda")]
+        v = torch.where(hit, pick, v)
+    elif where == "column":
+        v[:, 0, 64] = inf
+    elif where == "all":
+        v[:] = nan
+    return v
+
+
+def check_odd_values(cuda, q, k, v, where, g, **w):
+    """Against the same call with zeros in place of the values that are not finite: a row that sees none in a dimension is
+    the same to the bit, one that sees some is what their sum is (probabilities here are far from underflow)."""
+    full = dict(left=-1, right=-1, sinks=0, block=1, q_pos=0) | w
+    odd = place(v, where, g)
+    got = cuda.sdpa_window(q, k, odd, **full)
+    cuda.check()
+    fine = torch.isfinite(odd)
+    want = cuda.sdpa_window(q, k, torch.where(fine, odd, 0), **full)
+    q_pos = full.pop("q_pos")
+    lq, heads, kv = q.shape[0], q.shape[1], k.shape[1]
+    keys = (~fine).any(2).any(1).nonzero()[:, 0]
+    for rows in torch.arange(lq, device="cuda").split(2000):
+        p = rows[:, None] + q_pos                              # the definition, for the keys that have such values
+        b = p - p % full["block"]
+        seen = (keys <= b + full["block"] - 1 + full["right"]) if full["right"] >= 0 else keys[None] >= 0
+        seen = (seen & ((keys >= b - full["left"]) | (keys < full["sinks"])) if full["left"] >= 0 else seen.expand(len(rows), -1)).float()
+        x = odd[keys].permute(1, 0, 2)                          # [KV, keys, 128]
+        nan, pos, neg = ((seen @ y.float()) > 0 for y in (x.isnan(), x == float("inf"), x == -float("inf")))   # [KV, rows, 128]
+        nan, inf = nan | (pos & neg), torch.where(pos, float("inf"), -float("inf"))
+        per_head = want[rows].view(-1, heads, 128).permute(1, 0, 2).float().reshape(kv, heads // kv, -1, 128)
+        per_head = torch.where(nan[:, None], float("nan"), torch.where((pos | neg)[:, None], inf[:, None], per_head))
+        expect = per_head.reshape(heads, -1, 128).permute(1, 0, 2).reshape(len(rows), -1)
+        assert torch.equal(got[rows].float().nan_to_num(nan=12345.0), expect.nan_to_num(nan=12345.0))
+
+
+ODD = ["one", "first", "last", "some", "column", "all"]
+
+
+@pytest.mark.parametrize("where", ODD)
+@pytest.mark.parametrize("lq, lk, heads, kv, dtype, w", [
+    (200, 777, 4, 2, BF, dict(left=50, right=0, sinks=3, q_pos=500)), (600, 600, 2, 2, HF, dict(left=-1, right=0)),
+    (300, 900, 7, 1, BF, dict(left=100, right=30, sinks=9, q_pos=600)), (512, 512, 2, 2, BF, dict(left=128, right=0, sinks=64, block=64)),
+    (17, 300, 1, 1, BF, dict(left=-1, right=-1)),                               # every row sees every key
+    (40, 9000, 4, 2, BF, dict(left=-1, right=0, q_pos=8960)),                   # keys split over a cluster
+    (130, 2000, 3, 1, HF, dict(left=700, right=0, sinks=200, q_pos=1870)),
+    (9000, 9000, 4, 4, BF, dict(left=5, right=0)),                              # many short items for a CTA
+    (1620, 9000, 24, 24, BF, dict(left=-1, right=0, block=1620, q_pos=7380)),   # whole rounds, then a rest that is split
+    (2500, 6000, 16, 2, HF, dict(left=-1, right=0, q_pos=3500))])
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(cuda, lq, lk, heads, kv, dtype, w, where):
+    g = gen(lq + lk)
+    q, k, v = normal(g, lq, heads, 128, dtype=dtype), normal(g, lk, kv, 128, dtype=dtype), normal(g, lk, kv, 128, dtype=dtype)
+    check_odd_values(cuda, q, k, v, where, g, **w)
+
+
+@pytest.mark.parametrize("where", ["one", "first", "column"])
+def test_values_that_are_not_finite_among_very_many_keys(cuda, where):
+    """Items of more keys than one accumulator takes, of one sequence each: 40 rows over 70,000 and 1,000 over 300,000 keys."""
+    g = gen(20)
+    for lq, lk in ((40, 70000), (1000, 300000)):
+        q, k, v = (normal(g, n, 1, 128, dtype=BF) for n in (lq, lk, lk))
+        check_odd_values(cuda, q, k, v, where, g, left=-1, right=0, q_pos=lk - lq)
+        check_odd_values(cuda, q, k, v, where, g, left=-1, right=0, q_pos=lk // 2)   # half of the keys are behind every row
+
+
+def timed(fn):
+    fn()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    torch.cuda.synchronize()
+    a.record()
+    fn()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b)
+
+
+@pytest.mark.parametrize("w", [dict(left=2048, right=0, sinks=1024, block=1024), dict(left=2047, right=0, sinks=64)], ids=str)
+def test_a_value_that_is_not_finite_costs_a_second_pass_and_no_more(cuda, w):
+    """6,144 tokens by frames (whose rows see the same, so that nothing is done twice) and by tokens: one infinity in a key that
+    stays visible, one dimension of infinities, some values, all of them.  Each item is done twice at most; the bound leaves
+    room for the search, the rows written once more, and a busy machine."""
+    g = gen(21)
+    q, k, v = (normal(g, 6144, 24, 128, dtype=BF) for _ in range(3))
+    base = min(timed(lambda: cuda.sdpa_window(q, k, v, **w)) for _ in range(5))
+    for where in ("one", "first", "column", "some", "all"):
+        odd = place(v, where, g)
+        took = min(timed(lambda: cuda.sdpa_window(q, k, odd, **w)) for _ in range(5))
+        print(f"{where}: {took:.3f} ms, {base:.3f} without")
+        assert took < 8 * base
+    cuda.check()
