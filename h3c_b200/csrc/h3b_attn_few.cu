@@ -98,14 +98,17 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
     return v;
 }
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 template <typename T> __device__ __forceinline__ float to_f(uint32_t pair, int hi) {
     if (Elem<T>::FMT == 1) return __uint_as_float(hi ? pair & 0xffff0000u : pair << 16);
     return __half2float(__ushort_as_half((unsigned short)(hi ? pair >> 16 : pair & 0xffffu)));
 }
 
-// NT: 8 NT rows
-template <typename T, bool KV8, int NT, bool WIDE> __global__ void __launch_bounds__(few::Cfg<KV8, WIDE>::THREADS, few::Cfg<KV8, WIDE>::CTAS)
-k_attn_few(const __grid_constant__ FewParams p) {
+// One pass over the keys; true: values that are not finite may have reached rows that do not see them (16-bit; the whole
+// cluster alike).  AGAIN: the pass after that, see OddValues.  NT: 8 NT rows.
+template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forceinline__ bool few_pass(const FewParams &p) {
     using C = few::Cfg<KV8, WIDE>;
     using E = typename std::conditional<KV8, __half, T>::type;                     // operand type
     constexpr int U = C::U, WARPS = C::WARPS, STAGE = C::STAGE, HALF = C::HALF;
@@ -118,13 +121,14 @@ k_attn_few(const __grid_constant__ FewParams p) {
     float *warp_ml = acc_l + 16;                                                   // [WARPS][16][2]
     uint64_t *bars = reinterpret_cast<uint64_t *>(warp_ml + WARPS * 16 * 2);       // [WARPS][keys | values]
     volatile int *abort_word = reinterpret_cast<volatile int *>(bars + WARPS * 2);
+    volatile int *again = abort_word + 1;                                          // 16-bit: the cluster goes over its keys a second time
 
     const WinArgs &a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = (int)blockIdx.x % p.split, mt = (int)blockIdx.x / p.split, kvh = blockIdx.y, s = blockIdx.z;
     const SeqExt e = seq_ext<KV8>(a, s);
     const int r_first = mt * ROWS, r_end = min(r_first + ROWS, e.nq * a.group);    // rows = query * group + head of the group
-    if (r_first >= r_end) return;                                                  // the whole cluster alike
+    if (r_first >= r_end) return false;                                            // the whole cluster alike
     const int R = r_end - r_first;
     const int qi_first = r_first / a.group, qi_last = (r_end - 1) / a.group;
     const int p0 = e.pos0 + qi_first, p1 = e.pos0 + qi_last;
@@ -132,7 +136,8 @@ k_attn_few(const __grid_constant__ FewParams p) {
     const h3b_win_row row_a = h3b_win_of(a.win, p0, e.n), row_z = h3b_win_of(a.win, p1, e.n);
     const int share = (tiles.count + p.split - 1) / p.split;
     const int first = rank * share + warp, last = min((rank + 1) * share, tiles.count);
-    const int n_it = first < last ? (last - first + WARPS - 1) / WARPS : 0;
+    // (a first pass that gave up a wait may have copies under way still: no more of them)
+    const int n_it = first < last && !(AGAIN && *abort_word) ? (last - first + WARPS - 1) / WARPS : 0;
 
     uint8_t *stage = smem + warp * STAGE;
     uint64_t *bar = bars + warp * 2;
@@ -140,12 +145,20 @@ k_attn_few(const __grid_constant__ FewParams p) {
         tma_prefetch_desc(&p.map_k);
         tma_prefetch_desc(&p.map_v);
     }
-    if (lane == 0) {
+    if (AGAIN && n_it && lane == 0) {
+        mbar_inval(&bar[0]);
+        mbar_inval(&bar[1]);
         mbar_init(&bar[0], 1);
         mbar_init(&bar[1], 1);
-        if (warp == 0) *abort_word = 0;
         mbar_fence_init();
     }
+    if (!AGAIN && lane == 0) {
+        mbar_init(&bar[0], 1);
+        mbar_init(&bar[1], 1);
+        if (warp == 0) *abort_word = 0, *again = 0;
+        mbar_fence_init();
+    }
+    if (AGAIN) fence_proxy_async_smem();                                           // copies come where rows were parked
     __syncthreads();
 
     // ---- copies: lane 0 issues, all lanes together look up 32 tiles at a time
@@ -406,6 +419,15 @@ k_attn_few(const __grid_constant__ FewParams p) {
                     for (int c = 0; c < (KV8 ? 8 : 16); c++)
                         *reinterpret_cast<uint4 *>(dst + (c >> 3) * (HALF / 2) + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     fence_proxy_async_smem();      // the next copy into the stage comes behind these stores
+                } else if (AGAIN) {
+                    uint8_t *row = stage + HALF + lane * 128;
+#pragma unroll 4
+                    for (int c = 0; c < 16; c++) {
+                        uint4 *at = reinterpret_cast<uint4 *>(row + (c >> 3) * (HALF / 2) + (c & 7) * 16);
+                        const uint4 w = *at;
+                        *at = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y), finite_or_zero<T>(w.z), finite_or_zero<T>(w.w));
+                    }
+                    fence_proxy_async_smem();
                 }
             }
             __syncwarp();
@@ -482,6 +504,21 @@ k_attn_few(const __grid_constant__ FewParams p) {
                 }
             }
         }
+    if (AGAIN) {
+        // rows that see values which were taken out get them back
+        const h3b_win_row wr = h3b_win_of(a.win, e.pos0 + min(r_first + (lane & 15), r_end - 1) / a.group, e.n);
+        OddValues x;
+        x.clear();
+        for (int it = 0; it < n_it; it++) {
+            const int key = h3b_win_tile(tiles, first + it * WARPS) * U;
+            if (!h3b_win_full(row_a, row_z, key, U)) x.template collect<T>(a, kvh, key, U, wr, lane < R, lane);
+        }
+        __syncwarp();
+        for (int r = 0; r < R; r++)
+            if (x.any(r))
+#pragma unroll
+                for (int i = 0; i < 4; i++) mine[r * C::PITCH + lane * 4 + i] += x.of(r, i);
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < R * 128; i += C::THREADS) {
         const int r = i >> 7, dim = i & 127, at = r * C::PITCH + (KV8 ? ((dim & 14) << 3) + (dim >> 4 << 1) + (dim & 1) : dim);
@@ -506,9 +543,9 @@ k_attn_few(const __grid_constant__ FewParams p) {
     cluster_sync_all();
     const uint32_t acc_addr = smem_u32(acc);
     const int d = threadIdx.x;                                                   // threads 0..127: one dimension each
+    bool odd = false;                                                            // not finite, with a finite sum of probabilities
     for (int r = rank; r < R; r += p.split) {
         const int qi = (r_first + r) / a.group, hd = (r_first + r) - qi * a.group;
-        bool odd = false;
         if (d < 128) {
             float mc[8], lc[8], vc[8], m = -INFINITY, l = 0.0f, v = 0.0f;            // at most 8 CTAs, all loads under way at once
 #pragma unroll
@@ -532,14 +569,23 @@ k_attn_few(const __grid_constant__ FewParams p) {
             const float res = h3b_win_count(h3b_win_of(a.win, e.pos0 + qi, e.n)) ? v * (1.0f / l) : 0.0f;
             T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qi) * a.o_rs + (long long)(kvh * a.group + hd) * a.o_hs;
             reinterpret_cast<unsigned short *>(dst)[d] = (unsigned short)(Elem<T>::pack(res, res) & 0xffffu);
-            odd = !(fabsf(res) < INFINITY);
-        }
-        // a value that is not finite and that other rows of the tile see: such a row is computed again from its own keys
-        if (!KV8 && __syncthreads_or(odd)) {
-            if (warp == 0) attn_row_by_warp<T, KV8>(a, s, e, qi, kvh * a.group + hd, lane);
+            odd |= !(fabsf(res) < INFINITY) && ordinary(l);
         }
     }
+    if (!KV8 && !AGAIN && odd)                                                   // every CTA of the cluster has to know
+        for (int c = 0; c < p.split; c++) st_cluster_u32(mapa_shared(smem_u32(const_cast<const int *>(again)), c), 1u);
     cluster_sync_all();                                                          // nobody leaves while its memory is read
+    // rows that see the same hold what they see
+    return !KV8 && !AGAIN && *again && (row_a.hi != row_z.hi || row_a.lo != row_z.lo || row_a.s != row_z.s);
+}
+
+// A function of its own, so that its registers are no concern of the first pass (as a loop around it, 9 to 18 % slower for 9 to
+// 16 rows of 16-bit keys).
+template <typename T, int NT, bool WIDE> __device__ __noinline__ void few_again(const FewParams &p) { few_pass<T, false, NT, WIDE, true>(p); }
+
+template <typename T, bool KV8, int NT, bool WIDE> __global__ void __launch_bounds__(few::Cfg<KV8, WIDE>::THREADS, few::Cfg<KV8, WIDE>::CTAS)
+k_attn_few(const __grid_constant__ FewParams p) {
+    if (few_pass<T, KV8, NT, WIDE, false>(p) && !KV8) few_again<T, NT, WIDE>(p);
 }
 
 // How the keys of one (sequence, K/V head, row tile) are shared out.

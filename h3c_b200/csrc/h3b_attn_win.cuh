@@ -115,68 +115,6 @@ __device__ __forceinline__ void widen4_e4m3(uint32_t w, uint32_t &lo, uint32_t &
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 
-// One row and head by one warp, from the definition: lane l holds dimensions 4l..4l+3; a key costs one warp-wide sum.
-// Only visible keys are touched, so whatever masked places hold has no part in the result.
-template <typename T, bool KV8>
-__device__ __forceinline__ void attn_row_by_warp(const WinArgs &a, int s, const SeqExt e, int row, int head, int lane) {
-    const int kvh = head / a.group;
-    const h3b_win_row r = h3b_win_of(a.win, e.pos0 + row, e.n);
-    const float4 q = load4(reinterpret_cast<const T *>(a.q) + (long long)(e.row0 + row) * a.q_rs + head * a.q_hs + lane * 4);
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int count = h3b_win_count(r), gap = max(r.lo - r.s, 0);
-    int blk_have = -1;
-    long long bi = -1;
-    float ks = 1.0f, vs = 1.0f;
-    for (int i = 0; i < count; i++) {
-        const int j = i < r.s ? i : i + gap;
-        float4 k, v;
-        if (KV8) {
-            const int blk = j / KV8_BLOCK;
-            if (blk != blk_have) {
-                blk_have = blk;
-                bi = kv8_block_index(a, s, blk, kvh);
-                if (bi >= 0) {
-                    ks = a.ks[bi];
-                    vs = a.vs[bi];
-                }
-            }
-            if (bi < 0) continue;
-            const long long off = (bi * KV8_BLOCK + (j - blk * KV8_BLOCK)) * 128 + lane * 4;
-            k = codes4(*reinterpret_cast<const uint32_t *>(a.kc + off));
-            v = codes4(*reinterpret_cast<const uint32_t *>(a.vc + off));
-        } else {
-            k = load4(reinterpret_cast<const T *>(a.k) + (long long)j * a.k_rs + kvh * a.k_hs + lane * 4);
-            v = load4(reinterpret_cast<const T *>(a.v) + (long long)j * a.v_rs + kvh * a.v_hs + lane * 4);
-        }
-        float d = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
-#pragma unroll
-        for (int w = 16; w; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
-        if (KV8) d *= ks;
-        const float x = d * a.scale_log2;
-        if (x != x || x == INFINITY) {   // undefined: so is the row
-            l = __int_as_float(0x7fffffff);
-            break;
-        }
-        if (x > m) {
-            const float f = m == -INFINITY ? 0.0f : exp2f(m - x);
-            l *= f;
-            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
-            m = x;
-        }
-        const float p = x == -INFINITY ? 0.0f : exp2f(x - m);
-        l += p;
-        const float pv = KV8 ? p * vs : p;
-        o.x += pv * v.x; o.y += pv * v.y; o.z += pv * v.z; o.w += pv * v.w;
-    }
-    const float inv = count ? 1.0f / l : 0.0f;
-    uint2 w;
-    w.x = Elem<T>::pack(o.x * inv, o.y * inv);
-    w.y = Elem<T>::pack(o.z * inv, o.w * inv);
-    if (!count) w.x = w.y = 0u;
-    *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + (long long)(e.row0 + row) * a.o_rs + head * a.o_hs + lane * 4) = w;
-}
-
 // ---- Values that are not finite, at keys that not every row of a group sees.  A probability of 0 times such a value is not 0, so
 // the matrix product hands it to rows that do not see it.  Looking for them in every tile costs time, so the kernels look at
 // the results: where a row with a finite sum of probabilities comes out non-finite and the rows of its group differ in what

@@ -95,7 +95,12 @@ ODD = ["one", "first", "last", "some", "column", "all"]
     (130, 2000, 3, 1, HF, dict(left=700, right=0, sinks=200, q_pos=1870)),
     (9000, 9000, 4, 4, BF, dict(left=5, right=0)),                              # many short items for a CTA
     (1620, 9000, 24, 24, BF, dict(left=-1, right=0, block=1620, q_pos=7380)),   # whole rounds, then a rest that is split
-    (2500, 6000, 16, 2, HF, dict(left=-1, right=0, q_pos=3500))])
+    (2500, 6000, 16, 2, HF, dict(left=-1, right=0, q_pos=3500)),
+    # up to 16 rows for a K/V head
+    (5, 777, 4, 2, BF, dict(left=50, right=0, sinks=3, q_pos=386)), (16, 400, 2, 2, HF, dict(left=-1, right=0, q_pos=384)),
+    (1, 500, 6, 6, BF, dict(left=-1, right=0, q_pos=499)), (8, 20000, 4, 2, BF, dict(left=-1, right=0, q_pos=9996)),
+    (3, 30000, 24, 24, HF, dict(left=9000, right=5, sinks=40, q_pos=15000)), (2, 3001, 7, 1, BF, dict(left=0, right=0, block=2, sinks=3, q_pos=1502)),
+    (4, 200, 300, 100, BF, dict(left=20, right=0, q_pos=100))])
 def test_values_that_are_not_finite_reach_only_rows_that_see_them(cuda, lq, lk, heads, kv, dtype, w, where):
     g = gen(lq + lk)
     q, k, v = normal(g, lq, heads, 128, dtype=dtype), normal(g, lk, kv, 128, dtype=dtype), normal(g, lk, kv, 128, dtype=dtype)
