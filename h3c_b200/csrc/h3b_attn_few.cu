@@ -5,7 +5,7 @@
 // tensor-core products whose 16 rows are KEYS, respectively dimensions: S^T = K Q^T and O^T += V^T P^T, so that nothing is
 // padded from 1 to 16 rows (8 is the least) and the widened keys and values are the operands that are used once.  Q stays
 // in registers, P goes from score fragments to operand fragments through one 8x8 transposition per 8 keys.  The running
-// maximum is looked at by a vote and followed only when it has grown by more than 2^8.  A warp has a stage of its own
+// maximum is looked at by a vote and followed only when it has grown by more than ProbRange says.  A warp has a stage of its own
 // for TMA copies: those of the next keys are under way while the values are used and the other way round, and a warp waits
 // for nobody but its own copies.  Tiles are dealt out over the warps of a CTA and the CTAs of a cluster; the partial
 // results (m, l, O) meet in shared memory, first of the CTA, then across the cluster, so a split over the keys needs
@@ -16,7 +16,7 @@
 // 8-bit cache: codes are widened to f16 in registers (E4M3 fits f16 exactly), Q goes to f16 under a power of two of its
 // row's maximum (bf16 has more range than f16; what is 2^-38 below the row's largest element is lost), and neither K
 // nor V is multiplied by its scale: the key scale multiplies 64 scores, and log2 of the value scale is added to
-// their exponent, so P carries it (2^(x + log2 vs - m)) and the row sum takes it out again per 64 keys.  The order of
+// their exponent, so P carries it (2^(x + log2 vs - m), in the range of f16 that ProbRange chooses) and the row sum takes it out again per 64 keys.  The order of
 // the 128 products of a score and of the keys of a sum is free, so every lane takes the 16 bytes it reads as they lie:
 // fragments need no shuffles, and the 128-byte swizzle of the copies keeps the reads free of bank conflicts.
 //
@@ -365,7 +365,7 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
                 if (KV8 && mx == -INFINITY) f[j] = 1.0f, off[j] = 0.0f;
                 mx = KV8 ? fmaf(mx, f[j], off[j]) : mx * f[j];
                 top[j] = mx;
-                grow |= mx > m_run[nt][j] + 8.0f;                                   // also at the first visible key: m_run = -inf
+                grow |= mx > m_run[nt][j] + ProbRange<E>::LAG;                      // also at the first visible key: m_run = -inf
             }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -387,7 +387,7 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float m_use = m_run[nt][j] == -INFINITY ? 0.0f : m_run[nt][j], c = (KV8 ? off[j] : 0.0f) - m_use;
+                const float m_use = m_run[nt][j] == -INFINITY ? 0.0f : m_run[nt][j] - ProbRange<E>::UP, c = (KV8 ? off[j] : 0.0f) - m_use;
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < MT; i++)

@@ -18,7 +18,7 @@
 //   warp 3       the next item; 16-bit: zeroes the value rows of edge tiles that no row sees; 8-bit: helps to convert Q
 //   warps 4-7    softmax of tile A, warps 8-11 of tile B: one row per thread.  They read the 128 scores once, write P back
 //                over the score columns in two halves of 64 keys, and store the rows at the end; the accumulator is
-//                rescaled only when the running maximum grew by more than 2^8
+//                rescaled only when the running maximum grew by more than ProbRange says
 //   warps 12-15  8-bit: widen the codes of a tile to f16 in the swizzled layout that the MMAs read
 // TMEM: S_A 0..127, S_B 128..255 (P overlays the first 64 columns of each), O_A 256..383, O_B 384..511.
 //
@@ -771,7 +771,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                 }
                 if (mx != mx) l_run = mx;                                // undefined, and so is the row from here on
                 const float m_new = fmaxf(m_run, mx);
-                const bool grow = m_new > m_run + 8.0f;                  // also at the first visible key: m_run = -inf
+                const bool grow = m_new > m_run + ProbRange<E>::LAG;     // also at the first visible key: m_run = -inf
                 const bool fold = LONG && j && j % FOLD == 0;
                 if (__any_sync(0xffffffffu, grow) || fold) {
                     float alpha = 1.0f;
@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     }
                     if (fold) far_scale = 1.0f;
                 }
-                const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+                const float m_use = m_run == -INFINITY ? 0.0f : m_run - ProbRange<E>::UP;
                 float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
                 auto chunk = [&](int ch, uint32_t (&packed)[16]) {
                     const float fh = f[ch >> 1], cc = KV8 ? off[ch >> 1] - m_use : -m_use;

@@ -74,6 +74,22 @@ __device__ __forceinline__ long long kv8_block_index(const WinArgs &a, int s, in
     return ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
 }
 
+// Probabilities are rounded to the operand type E as 2^(x - m + UP), with m the running maximum as it was last followed: it is
+// followed when it has grown by more than 2^LAG.  What is lost of a sum lies at the bottom of the type's range: bf16 has f32's,
+// f16 ends at 2^-25 (half its smallest number), so there its range is used up to the top (2^(LAG + UP) < 65504): one key loses at
+// most 2^-34 of the largest probability.  (With LAG = 8 and UP = 0 it was 2^-25, and a flat tail of 262,144 keys that held 0.7 % of
+// a row was lost altogether.)  Over the cache P carries the value scale, so there it is 2^-34 of the largest probability times
+// scale.  UP is whole, so that a probability of 1 stays exact.  The lower LAG is, the more often sums are rescaled.  Measured (us,
+// UP 8 | 9 | 10 | 11, LAG 15.9 - UP): 56 heads over 8 in f16 80.1 | 79.5 | 81.5 | 84.1, a frame over 50,220 cached tokens
+// 1,112 | 1,114 | 1,118 | 1,143.
+template <typename E> struct ProbRange;
+template <> struct ProbRange<__half> {
+    static constexpr float LAG = 6.9f, UP = 9.0f;
+};
+template <> struct ProbRange<__nv_bfloat16> {
+    static constexpr float LAG = 8.0f, UP = 0.0f;
+};
+
 // Largest magnitude of eight 16-bit floats, as two 16-bit patterns side by side: magnitudes order like integers, NaN above
 // infinity.
 __device__ __forceinline__ uint32_t abs_max8_pair(const uint4 &w) {

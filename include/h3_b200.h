@@ -482,7 +482,8 @@ int h3b_sdpa_strided_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row
  * (a frame of a video, 1 = each token alone) that starts at b = p - p % block; it sees key j when
  *     j <= b + block - 1 + right  and  (j >= b - left  or  j < sinks).
  * A negative left or right does not bound that side (-1, -1, 0, 1: full attention; -1, 0, 0, 1: causal).  A row that
- * sees no key is zero.  What masked keys hold (NaN, infinities) has no part in the result.  lq = 0 does nothing; out
+ * sees no key is zero.  What masked keys hold (NaN, infinities) has no part in the result.  Probabilities are held in `dtype`: in
+ * f16 a key loses at most 2^-34 of the largest one of its row.  lq = 0 does nothing; out
  * must not overlap the inputs or itself; nothing is allocated, so the call can be captured. */
 typedef struct {
     const void *d_q, *d_k, *d_v;
@@ -531,9 +532,14 @@ int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_
 /* Attention of q rows [rows, heads, 128] over the cache: sequence s has d_len[s] tokens and its rows are the last ones of
  * them (row i of nq at position d_len[s] - nq + i); windows as in h3b_sdpa_window_dev.  Rows of out that belong to no
  * sequence are left as they are.  max_len (a bound on d_len[], or an estimate) only guides how the work is split, and so
- * the order of the sums.  With up to 16 rows per K/V head, sums of values that do not cancel come out low by 5e-4 at a
- * million visible tokens where the keys are not split (2e-3 at four million); split over the chip, by a true max_len
- * and few sequences, 4e-5 (2e-4; 1e-3 at 16 million).  With more rows it is 1.5e-4 at any length. */
+ * the order of the sums.
+ * Accuracy beside half a step of the f16 probabilities and of the result, for very many tokens:
+ * - a token loses at most 2^-34 of the largest probability times value scale of its row: together 6e-5 of the largest value
+ *   at a million tokens;
+ * - sums of values that do not cancel come out low.  With more than 16 rows per K/V head: by 1.5e-4 at any length where
+ *   weights are alike, at most 1e-3 where one token outweighs all others together.  With fewer rows, a million tokens and
+ *   keys split over the chip (a true max_len and few sequences): 4e-5, at most 4e-4 (four million 2e-4 and 1.4e-3, 16 million
+ *   1e-3 and 6e-3); not split: 5e-4, at most 8e-3. */
 typedef struct {
     const void *d_q;
     void *d_out;

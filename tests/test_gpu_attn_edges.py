@@ -142,3 +142,62 @@ def test_a_value_that_is_not_finite_costs_a_second_pass_and_no_more(cuda, w):
         print(f"{where}: {took:.3f} ms, {base:.3f} without")
         assert took < 8 * base
     cuda.check()
+
+
+# ------------------------------------------------------------------ probabilities far below the largest
+
+def tail_tolerance(a, n, dtype, p_dtype, v_max, lost):
+    """Half a step of P and of the output, 2^-12 for what is computed in 32 bits (all relative to a = sum p |v|); products that
+    are cut to 2^-25 of an accumulator and its sum to 2^-27 of itself, over the up to 32,768 keys of one; and at the bottom of
+    P's range `lost` of the largest |v| per key."""
+    u = {BF: 2.0 ** -8, HF: 2.0 ** -11}
+    return (u[p_dtype] + u[dtype] + 2.0 ** -12 + min(n, 32768) * (2.0 ** -25 + 2.0 ** -27)) * a + n * lost * v_max
+
+
+def tail_of(n, step, loud):
+    """One key of weight 1 and n - 1 of 2^-step (scale ln 2, so that a score counts in powers of two); values: the heavy key
+    `loud` in dimensions 0 to 63 and nothing in the others, the rest 1 everywhere.  (q, k, v, out, sum p |v|) in 64 bits."""
+    k, v = torch.zeros(n, 128, dtype=torch.float64, device="cuda"), torch.ones(n, 128, dtype=torch.float64, device="cuda")
+    q = torch.zeros(128, dtype=torch.float64, device="cuda")
+    heavy = 5
+    k[heavy, 9], q[9] = 26.0, step / 26.0
+    v[heavy, :64], v[heavy, 64:] = loud, 0.0
+    q = q.to(BF).double()                                          # eight bits: exact in both types
+    w = 2.0 ** (q[9] * 26.0)
+    return q, k, v, (w * v[heavy] + (n - 1)) / (w + n - 1)
+
+
+@pytest.mark.parametrize("n", [50220, 262144])
+@pytest.mark.parametrize("rows", [1, 4, 40])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_a_flat_tail_far_below_the_largest_probability(cuda, n, rows, dtype):
+    """2^-25.2 each: together 0.1 % of the row at 50,220 keys and 0.7 % at 262,144, and the whole result where the heavy
+    key's value is zero."""
+    q, k, v, want = tail_of(n, 25.2, 1.0)
+    q, k, v = q.to(dtype).expand(rows, 2, 128).contiguous(), k.to(dtype)[:, None].contiguous(), v.to(dtype)[:, None].contiguous()
+    got = cuda.sdpa_window(q, k, v, scale=float(np.log(2.0))).view(-1, 128).double()
+    assert ((got - want).abs() <= tail_tolerance(want, n, dtype, dtype, 1.0, 2.0 ** -34 if dtype is HF else 0.0)).all(), (got - want).abs().amax(0)
+    cache = cuda.kv8_cache(-(-n // 256), 256, 1)
+    table = torch.arange(-(-n // 256), dtype=torch.int32, device="cuda")[None]
+    cuda.kv8_append(cache, k, v, i32([0, n]), i32([0]), table, max_rows=n)
+    got = cuda.kv8_sdpa(cache, q, i32([0, rows]), i32([n]), table, max_rows=rows, max_len=n, right=-1, scale=float(np.log(2.0))).view(-1, 128).double()
+    cuda.check()
+    assert ((got - want).abs() <= tail_tolerance(want, n, dtype, HF, 1.0, 2.0 ** -34)).all(), (got - want).abs().amax(0)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_a_loud_block_of_the_cache_does_not_drown_the_others(cuda, rows, dtype):
+    """The heavy key's block has values 2^6 louder than the rest, whose 50,219 keys hold 6 % of the row at 2^-19.5 each and are the
+    whole result in the dimensions where the heavy key is silent.  P carries the scale, so a key loses at most 2^-34 of
+    the loud one's."""
+    n = 50220
+    q, k, v, want = tail_of(n, 19.5, 64.0)
+    q, k, v = q.to(dtype).expand(rows, 2, 128).contiguous(), k.to(dtype)[:, None].contiguous(), v.to(dtype)[:, None].contiguous()
+    cache = cuda.kv8_cache(-(-n // 64), 64, 1)
+    table = torch.arange(-(-n // 64), dtype=torch.int32, device="cuda")[None]
+    cuda.kv8_append(cache, k, v, i32([0, n]), i32([0]), table, max_rows=n)
+    assert cache.v_scale[0, 0, 0] == 2.0 ** 6 * cache.v_scale[1, 0, 0]
+    got = cuda.kv8_sdpa(cache, q, i32([0, rows]), i32([n]), table, max_rows=rows, max_len=n, right=-1, scale=float(np.log(2.0))).view(-1, 128).double()
+    cuda.check()
+    assert ((got - want).abs() <= tail_tolerance(want, n, dtype, HF, 64.0, 2.0 ** -34)).all(), (got - want).abs().amax(0)
