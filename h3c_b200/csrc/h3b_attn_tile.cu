@@ -77,7 +77,7 @@ struct Control {
     int search;                                           // tiles gone through for values that are not finite
     int odd[4], cta_of[4];                                // by item modulo 4: it has rows that came out non-finite; CTA of the grid whose item it is
     alignas(16) uint32_t clc[4];
-    alignas(16) int item[2][12];
+    alignas(16) int item[2][16];
     alignas(16) float4 scales[4];                         // of a tile: key scale of either half, log2 of the value scale of either half
     float2 inv_scales[4];                                 // 1 / value scale of either half
     int8_t q_shift[2][256];                               // 8-bit: rows of Q are here times 2^shift; by item
@@ -146,7 +146,8 @@ template <bool KV8> struct TileCfg {
 };
 
 struct TileItem {
-    int kvh, s, r0, r_end, row0, n, pos0, sink, from, n_kv, t_first, nq;   // s: 8-bit: the sequence; 16-bit: 1 if done a second time
+    int kvh, s, r0, r_end, row0, n, pos0, sink, from, n_kv, t_first;       // s: 8-bit: the sequence; 16-bit: 1 if done a second time
+    int hi, lo, sn;                                       // some row sees key j: j <= hi and (j >= lo or j < sn)
     __device__ __forceinline__ int key(int j) const {                    // first key of the j-th tile
         const int i = t_first + j;
         return (i < sink ? i : from + i - sink) * wtile::BN;
@@ -274,10 +275,11 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     // the k-th item of this CTA; false: no more (or a wait gave up)
     auto take_item = [&](int k, TileItem &it) -> bool {
         const int4 *src = reinterpret_cast<const int4 *>(ctl.item[k & 1]);
-        const int4 x = src[0], y = src[1], z = src[2];
+        const int4 x = src[0], y = src[1], z = src[2], w = src[3];
         it.kvh = x.x; it.s = x.y; it.r0 = x.z; it.r_end = x.w;
         it.row0 = y.x; it.n = y.y; it.pos0 = y.z; it.sink = y.w;
-        it.from = z.x; it.n_kv = z.y; it.t_first = z.z; it.nq = z.w;
+        it.from = z.x; it.n_kv = z.y; it.t_first = z.z; it.hi = z.w;
+        it.lo = w.x; it.sn = w.y;
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.item_empty[k & 1]);
         return it.r0 >= 0;
@@ -293,17 +295,15 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         ra = h3b_win_of(a.win, it.pos0 + it.r0 / a.group, it.n);
         rz = h3b_win_of(a.win, it.pos0 + (it.r_end - 1) / a.group, it.n);
     };
-    // no row of the item sees key j: j > hi or s <= j < lo
-    auto seen_by_any = [&](const TileItem &it, int &hi, int &lo, int &sn) {
+    // a tile has keys before `end` that no row sees (16-bit: what lies behind the last key comes as zeros)
+    auto edge = [&](const TileItem &it, int key, int end) { return min(key + BN, end) - 1 > it.hi || max(key, it.sn) < min(key + BN, it.lo); };
+    // 16-bit: a tile whose values pass through warp 3
+    auto by_hand = [&](const TileItem &it, int key) {
+        if (edge(it, key, it.n)) return true;
+        if (!it.s) return false;
         h3b_win_row ra, rz;
         rows_of(it, ra, rz);
-        hi = rz.hi; lo = ra.lo; sn = rz.s;
-    };
-    // a tile has such keys among those that exist (16-bit: what lies behind the last key comes as zeros)
-    auto edge = [&](int key, int end, int hi, int lo, int sn) { return min(key + BN, end) - 1 > hi || max(key, sn) < min(key + BN, lo); };
-    // 16-bit: a tile whose values pass through warp 3
-    auto by_hand = [&](const TileItem &it, int key, const h3b_win_row &ra, const h3b_win_row &rz) {
-        return edge(key, it.n, rz.hi, ra.lo, rz.s) || (it.s && !h3b_win_full(ra, rz, key, BN));
+        return !h3b_win_full(ra, rz, key, BN);
     };
     bool ok = true;
 
@@ -315,8 +315,6 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             int c = 0;                                                   // tiles so far
             for (int k = 0; ok && next_item(k, it); k++) {
                 if (!KV8) {
-                    h3b_win_row ra, rz;
-                    rows_of(it, ra, rz);
                     for (int j = 0; j < it.n_kv && ok; j++, c++) {
                         const int st = c & 1, key = it.key(j);
                         const uint32_t ph = ((c >> 1) & 1) ^ 1;
@@ -330,7 +328,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         ok = wait(&ctl.v_empty[st], ph, H3B_ST_TIMEOUT_EMPTY);
                         if (!ok) break;
                         if (lane == 0) {
-                            uint64_t *b = by_hand(it, key, ra, rz) ? &ctl.v_raw[st] : &ctl.v_full[st];
+                            uint64_t *b = by_hand(it, key) ? &ctl.v_raw[st] : &ctl.v_full[st];
                             mbar_expect_tx(b, TILE);
                             tma_load_3d(sV + st * TILE, &p.map_v, b, 0, it.kvh, key);
                             tma_load_3d(sV + st * TILE + SLAB, &p.map_v, b, 64, it.kvh, key);
@@ -347,10 +345,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                             if (j + (lane >> 1) < it.n_kv) {
                                 // half of a tile may lie outside every row's window (before it, or behind the sinks): the page of such a
                                 // half may be anything and is not looked up; the widening warps zero its rows
-                                int hi, lo, sn;
-                                seen_by_any(it, hi, lo, sn);
                                 const int blk = it.key(j + (lane >> 1)) / KV8_BLOCK + (lane & 1);
-                                if (h3b_win_any(hi, lo, sn, blk * KV8_BLOCK, KV8_BLOCK)) bi = (int)kv8_block_index(a, it.s, blk, it.kvh);
+                                if (h3b_win_any(it.hi, it.lo, it.sn, blk * KV8_BLOCK, KV8_BLOCK)) bi = (int)kv8_block_index(a, it.s, blk, it.kvh);
                             }
                             bks = bi >= 0 ? __ldg(a.ks + bi) : 1.0f;
                             const float vs = bi >= 0 ? __ldg(a.vs + bi) : 1.0f;
@@ -534,7 +530,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         int4 *dst = reinterpret_cast<int4 *>(ctl.item[k & 1]);
                         dst[0] = make_int4(x.kvh, x.s, x.r0, x.r_end);
                         dst[1] = make_int4(x.row0, x.n, x.pos0, x.sink);
-                        dst[2] = make_int4(x.from, x.n_kv, x.t_first, x.nq);
+                        dst[2] = make_int4(x.from, x.n_kv, x.t_first, x.hi);
+                        dst[3] = make_int4(x.lo, x.sn, 0, 0);
                         mbar_arrive(&ctl.item_full[k & 1]);
                     }
                 };
@@ -550,8 +547,11 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     const long long rows = (long long)e.nq * a.group;
                     if (d.r0 >= rows) return false;
                     d.r_end = (int)(rows < d.r0 + 2 * p.bm ? rows : d.r0 + 2 * p.bm);
-                    d.row0 = e.row0; d.n = e.n; d.pos0 = e.pos0; d.nq = e.nq;
-                    const h3b_win_tiles w = h3b_win_tiles_of(a.win, e.pos0 + d.r0 / a.group, e.pos0 + (d.r_end - 1) / a.group, e.n, BN);
+                    d.row0 = e.row0; d.n = e.n; d.pos0 = e.pos0;
+                    h3b_win_row ra, rz;
+                    rows_of(d, ra, rz);
+                    const h3b_win_tiles w = h3b_win_tiles_rows(ra, rz, BN);
+                    d.hi = rz.hi; d.lo = ra.lo; d.sn = rz.s;
                     const int share = (w.count + p.split - 1) / p.split;
                     d.sink = w.sink; d.from = w.from;
                     d.t_first = rank * share;
@@ -621,11 +621,9 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                     if (CONVERT) {
                         if (it.n_kv) ok = convert_q(it, q++);
                     } else if (!KV8) {
-                        h3b_win_row ra, rz;
-                        rows_of(it, ra, rz);
                         for (int j = 0; j < it.n_kv && ok; j++) {
                             const int st = (c + j) & 1, key = it.key(j);
-                            if (!by_hand(it, key, ra, rz)) continue;
+                            if (!by_hand(it, key)) continue;
                             // tiles that need no cleaning lie in between
                             if (LONG) ok = wait_item([&] { return mbar_try_wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1); }, H3B_ST_TIMEOUT_FULL);
                             else ok = wait(&ctl.v_raw[st], (st ? raw[1] : raw[0]) & 1, H3B_ST_TIMEOUT_FULL);
@@ -634,7 +632,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                             else raw[0]++;
                             for (int i = lane; i < BN; i += 32) {
                                 uint8_t *row = sV + st * TILE + i * 128;
-                                if (key + i > rz.hi || (key + i < ra.lo && key + i >= rz.s)) {
+                                if (key + i > it.hi || (key + i < it.lo && key + i >= it.sn)) {
 #pragma unroll
                                     for (int h = 0; h < 16; h++)
                                         *reinterpret_cast<uint4 *>(row + (h >> 3) * SLAB + ((h & 7) ^ (i & 7)) * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -958,12 +956,10 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
         TileItem it;
         int c = 0;
         for (int k = 0; ok && next_item(k, it); k++) {
-            int hi, lo, sn;
-            seen_by_any(it, hi, lo, sn);
             for (int j = 0; j < it.n_kv && ok; j++, c++) {
                 const int st = c & 1, key = it.key(j);
                 const uint32_t ph = ((c >> 1) & 1) ^ 1;
-                const bool at_edge = edge(key, key + BN, hi, lo, sn);    // stale bytes behind the last token among them
+                const bool at_edge = edge(it, key, key + BN);    // stale bytes behind the last token among them
 #pragma unroll 1                                                         // its code has to stay in the instruction caches beside the others'
                 for (int w = 0; w < 4 && ok; w++) {                      // keys 0-63, 64-127, values 0-63, 64-127
                     ok = wait(&ctl.c_full[w], c & 1, H3B_ST_TIMEOUT_FULL) &&
@@ -978,7 +974,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const int x = key + (w & 1) * 64 + i * 8 + row0;
-                            if (x > hi || (x < lo && x >= sn)) raw[i] = make_uint2(0u, 0u);
+                            if (x > it.hi || (x < it.lo && x >= it.sn)) raw[i] = make_uint2(0u, 0u);
                         }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl.c_empty[w]);         // the codes are in registers

@@ -54,14 +54,18 @@ typedef struct {
     int sink, from, count;
 } h3b_win_tiles;
 
-static H3B_HD h3b_win_tiles h3b_win_tiles_of(h3b_win w, int p0, int p1, int n, int unit) {
-    const h3b_win_row a = h3b_win_of(w, p0 < 0 ? 0 : p0, n), z = h3b_win_of(w, p1, n);
+/* a, z: rows of the first and the last query (of a query in front of token 0 only lo matters, which is that of token 0) */
+static H3B_HD h3b_win_tiles h3b_win_tiles_rows(h3b_win_row a, h3b_win_row z, int unit) {
     h3b_win_tiles t;
     const int last = z.hi >= 0 ? z.hi / unit + 1 : 0, first = a.lo / unit;
     t.sink = z.s > 0 ? (z.s + unit - 1) / unit : 0;
     t.from = first > t.sink ? first : t.sink;
     t.count = t.sink + (last > t.from ? last - t.from : 0);
     return t;
+}
+
+static H3B_HD h3b_win_tiles h3b_win_tiles_of(h3b_win w, int p0, int p1, int n, int unit) {
+    return h3b_win_tiles_rows(h3b_win_of(w, p0, n), h3b_win_of(w, p1, n), unit);
 }
 
 static H3B_HD int h3b_win_tile(h3b_win_tiles t, int i) { return i < t.sink ? i : t.from + i - t.sink; }
