@@ -61,8 +61,9 @@ class Weight:
 
 class KvCache8:
     """Paged key/value cache held in E4M3 (h3b_kv8_cache): codes [pages, kv_heads, page_tokens, 128] as float8_e4m3fn
-    (or uint8) and f32 scales [pages, kv_heads, page_tokens // 64], value = code * scale.  The tensors stay the
-    caller's; `Cuda.kv8_cache` makes new ones.  A page list is an int32 row of page numbers, one per page_tokens."""
+    (or uint8) and f32 scales [pages, kv_heads, page_tokens // 64], value = code * scale (scales finite and
+    positive, one below 2^-64 counts as 2^-64; no code a NaN).  The tensors stay the caller's; `Cuda.kv8_cache` makes new ones.
+    A page list is an int32 row of page numbers, one per page_tokens."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "kv_heads", "device_index", "packed")
 

@@ -196,6 +196,8 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
     };
     auto logs = [&]() {
         if (KV8) {
+            my_ks = kv8_read_scale(my_ks);           // (not where they are asked for: the first copies do not wait for them)
+            my_vs = kv8_read_scale(my_vs);
             my_lvs = log2f(my_vs);
             my_ivs = 1.0f / my_vs;
         }

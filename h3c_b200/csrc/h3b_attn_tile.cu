@@ -348,8 +348,8 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                                 const int blk = it.key(j + (lane >> 1)) / KV8_BLOCK + (lane & 1);
                                 if (h3b_win_any(it.hi, it.lo, it.sn, blk * KV8_BLOCK, KV8_BLOCK)) bi = (int)kv8_block_index(a, it.s, blk, it.kvh);
                             }
-                            bks = bi >= 0 ? __ldg(a.ks + bi) : 1.0f;
-                            const float vs = bi >= 0 ? __ldg(a.vs + bi) : 1.0f;
+                            bks = bi >= 0 ? kv8_read_scale(__ldg(a.ks + bi)) : 1.0f;
+                            const float vs = bi >= 0 ? kv8_read_scale(__ldg(a.vs + bi)) : 1.0f;
                             blvs = log2f(vs);
                             bivs = 1.0f / vs;
                         }

@@ -74,6 +74,10 @@ __device__ __forceinline__ long long kv8_block_index(const WinArgs &a, int s, in
     return ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
 }
 
+// Scales below 2^-64 count as 2^-64, the smallest that the append writes: a zero (a new cache, a block of zeros quantised
+// elsewhere) has no inverse and no logarithm.  NaN stays, and so does a negative one, which is not allowed.
+__device__ __forceinline__ float kv8_read_scale(float s) { return s >= 0.0f && s < 0x1p-64f ? 0x1p-64f : s; }
+
 // Probabilities are rounded to the operand type E as 2^(x - m + UP), with m the running maximum as it was last followed: it is
 // followed when it has grown by more than 2^LAG.  What is lost of a sum lies at the bottom of the type's range: bf16 has f32's,
 // f16 ends at 2^-25 (half its smallest number), so there its range is used up to the top (2^(LAG + UP) < 65504): one key loses at

@@ -92,7 +92,7 @@ template <typename T> __global__ void __launch_bounds__(128) k_kv8_append(const 
         return;
     }
     const long long bi = ((long long)page * a.kv_heads + kvh) * a.page_blocks + (blk - pg * a.page_blocks);
-    const float before = from > 0 ? a.scales[w][bi] : 0.0f;      // tokens in front of the new ones keep it at least
+    const float before = from > 0 ? kv8_read_scale(a.scales[w][bi]) : 0.0f;      // tokens in front of the new ones keep it at least
     uint32_t top = 0u;
 #pragma unroll
     for (int i = 0; i < 8; i++) top = __vmaxu2(top, abs_max8_pair(raw[i]));

@@ -503,9 +503,12 @@ int h3b_window_tiles(size_t keys, int64_t pos0, size_t rows, int64_t left, int64
 /* Addition: a paged key/value cache held in 8 bits.  The caller owns the memory (16-byte aligned codes):
  *   d_k, d_v              E4M3 codes [pages][kv_heads][page_tokens][128]
  *   d_k_scale, d_v_scale  f32        [pages][kv_heads][page_tokens / 64], one scale per 64 tokens and head
- * value = code * scale, scales positive (or NaN, see below); page_tokens is a multiple of 64; pages * kv_heads *
- * page_tokens < 2^31.  The pages of sequence s are table[s * table_stride ...], its token t lies in page t / page_tokens of that list; pages that no call needs
- * (behind the length, or wholly outside the window) may hold any index.  A sequence's rows are rows cu_rows[s] ..
+ * value = code * scale; scales are finite and positive, or NaN (see below); one below 2^-64 (a zero too) counts as 2^-64; codes
+ * of values within a sequence's length are numbers (not the patterns 0x7f and 0xff, which the append never writes: as a
+ * value, such a code reaches rows that do not see it); page_tokens is a multiple of 64; pages * kv_heads *
+ * page_tokens < 2^31.  The pages of sequence s are table[s * table_stride ...], its token t lies in page t / page_tokens of
+ * that list; the list may hold any index for pages that no call needs (behind the length, or where no row of the call
+ * sees a token).  A sequence's rows are rows cu_rows[s] ..
  * cu_rows[s + 1] - 1 of the 16-bit tensors.  These tables are int32 on the device, so that a captured call follows
  * them; max_rows bounds the rows of any one sequence.  A sequence whose rows, length or page indices lie outside the
  * arrays is not followed there, its output is invalid, and h3b_cuda_check reports it. */
@@ -535,7 +538,7 @@ int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_
  * the order of the sums.
  * Accuracy beside half a step of the f16 probabilities and of the result, for very many tokens:
  * - a token loses at most 2^-34 of the largest probability times value scale of its row: together 6e-5 of the largest value
- *   at a million tokens;
+ *   at a million tokens (scales of a row's values more than 2^70 apart: the quieter tokens may drop out of its softmax);
  * - sums of values that do not cancel come out low.  With more than 16 rows per K/V head: by 1.5e-4 at any length where
  *   weights are alike, at most 1e-3 where one token outweighs all others together.  With fewer rows, a million tokens and
  *   keys split over the chip (a true max_len and few sequences): 4e-5, at most 4e-4 (four million 2e-4 and 1.4e-3, 16 million

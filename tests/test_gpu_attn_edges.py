@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_attn_window import BF, HF, check_cache, cuda, filled, gen, i32, mask, normal  # noqa: E402, F401
+from tests.test_gpu_attn_window import BF, HF, Model, check_cache, cuda, filled, gen, i32, mask, normal  # noqa: E402, F401
 
 
 # ------------------------------------------------------------------ pages that no row needs
@@ -201,3 +201,37 @@ def test_a_loud_block_of_the_cache_does_not_drown_the_others(cuda, rows, dtype):
     got = cuda.kv8_sdpa(cache, q, i32([0, rows]), i32([n]), table, max_rows=rows, max_len=n, right=-1, scale=float(np.log(2.0))).view(-1, 128).double()
     cuda.check()
     assert ((got - want).abs() <= tail_tolerance(want, n, dtype, HF, 64.0, 2.0 ** -34)).all(), (got - want).abs().amax(0)
+
+
+# ------------------------------------------------------------------ scales of zero
+
+@pytest.mark.parametrize("rows", [1, 5, 40])
+@pytest.mark.parametrize("w", [dict(), dict(left=70, sinks=3), dict(left=0)], ids=str)
+def test_a_scale_of_zero_counts_as_the_smallest_one(cuda, rows, w):
+    """A new cache holds zeros, and a block of zeros quantised by its largest magnitude has a scale of zero: its tokens are
+    zeros that take their share of the softmax."""
+    rng, g = np.random.default_rng(rows), gen(rows)
+    n = 500
+    fresh = cuda.kv8_cache(9, 64, 2)
+    q = normal(g, rows, 4, 128, dtype=BF)
+    assert not cuda.kv8_sdpa(fresh, q, i32([0, rows]), i32([n]), i32([np.arange(9)]), max_rows=rows, max_len=n, **w).any()
+    cache, table, _ = filled(cuda, rng, g, [n], 64, 2, BF, spread=False)
+    for page, k_too in ((0, True), (3, False), (6, True), (7, True)):      # 7: the last page, partly filled
+        for codes, scales in ((cache.v, cache.v_scale), (cache.k, cache.k_scale)):
+            if scales is cache.v_scale or k_too:
+                codes.view(torch.uint8)[table[0, page]] = 0
+                scales[table[0, page]] = 0
+    check_cache(cuda, cache, table, Model(cache), q, [0, rows], [n], **w)
+    cache.v_scale.masked_fill_(cache.v_scale == 0, 2.0 ** -80)              # and so does any below it
+    check_cache(cuda, cache, table, Model(cache), q, [0, rows], [n], **w)
+
+
+def test_append_behind_tokens_under_a_scale_of_zero(cuda):
+    g = gen(3)
+    cache = cuda.kv8_cache(1, 64, 1)
+    model = Model(cache)
+    zero, k = torch.zeros(10, 1, 128, dtype=BF, device="cuda"), normal(g, 10, 1, 128, dtype=BF)
+    for x, start in ((zero, 7), (k, 20)):                                    # tokens 0 to 6 were never written
+        cuda.kv8_append(cache, x, x, i32([0, 10]), i32([start]), i32([[0]]), max_rows=10)
+        model.append(x, x, [0, 10], [start], [[0]])
+        model.same_as(cache)
