@@ -596,20 +596,30 @@ struct FewPlan {
     int split;                                     // CTAs of a cluster
 };
 // Measured on 148 SMs (us; an E4M3 cache unless said otherwise):
-//   8 pairs of 100,000 keys: WIDE in clusters of 8 50, of 4 90; narrow of 8 81.  16 pairs of 20,000: WIDE of 6 19.4, of 8
-//   (which fit the chip 15 times only) 31; narrow of 8 24.8.  24 pairs of 20,000: WIDE of 5 28.2, narrow of 8 27.8, of 1 126.
+//   8 pairs of 100,000 keys: WIDE in clusters of 8 50, of 4 90; narrow of 8 81.  24 pairs of 20,000: WIDE of 5 28.2, narrow of
+//   8 27.8, of 1 126.
+//   One cluster more than the chip holds is a second wave (20,000 keys): 16 pairs, WIDE of 6 21.6, of 8 32.1; 18 pairs, of 6 22.8,
+//   of 7 33.5; narrow, 52 pairs, of 7 47.2, of 8 62.7; 61 pairs, of 6 54.7, of 7 72.4; 107 pairs, of 3 92.0, of 4 107.6.
 //   96 pairs of up to 12,000: narrow of 4 (384 CTAs, one wave) 33.6, of 1 77.6, of 5 41.7; WIDE 40.
 //   512 pairs of up to 16,000: narrow of 4 157, of 1 182; 1536 pairs of up to 2,000: of 1 80.6, of 2 96.7.
-// So: one wave where that is possible; beyond it shares of 32 tiles, below which a CTA's beginning and end cost more than
-// even shares gain.
+// So: the largest clusters of which one wave takes all pairs, where there are any; beyond that shares of 32 tiles, below which a
+// CTA's beginning and end cost more than even shares gain.
 static FewPlan few_plan(const h3_cuda *cuda, size_t units, size_t tiles) {
-    const size_t sms = (size_t)cuda->sm_count, some = std::max<size_t>(tiles / 4, 1);   // a tile for every warp of four
-    const size_t room_wide = sms * 89 / 100, room = sms * 29 / 10;                      // CTAs that clusters find room for
+    // the 8-bit kernels stand for the others too: a CTA of a size takes the same shared memory and threads in all of them
+    static AttnClusters wide, narrow;
+    auto room = [&](bool w, size_t n) {
+        return w ? attn_clusters_of(cuda, wide, (const void *)k_attn_few<__half, true, 1, true>, few::Cfg<true, true>::THREADS, few::Cfg<true, true>::SMEM_BYTES, n)
+                 : attn_clusters_of(cuda, narrow, (const void *)k_attn_few<__half, true, 1, false>, few::Cfg<true, false>::THREADS, few::Cfg<true, false>::SMEM_BYTES, n);
+    };
+    const size_t some = std::max<size_t>(tiles / 4, 1);                                 // a tile for every warp of four
     FewPlan p;
-    p.wide = units * 6 <= room_wide;
-    if (p.wide) p.split = (int)std::min(std::min<size_t>(room_wide / units, 8), some);
-    else if (2 * units <= room) p.split = (int)std::min(std::min<size_t>(room / units, 8), some);
-    else p.split = (int)std::min<size_t>(std::max<size_t>(tiles / 32, 1), 4);
+    p.wide = room(true, 6) >= units;
+    size_t n = std::min<size_t>(some, 8);
+    if (p.wide || room(false, 2) >= units)
+        while (n > 1 && room(p.wide, n) < units) n--;
+    else
+        n = std::min<size_t>(std::max<size_t>(tiles / 32, 1), 4);
+    p.split = (int)n;
     return p;
 }
 

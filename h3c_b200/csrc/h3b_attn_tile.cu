@@ -1059,15 +1059,11 @@ template <typename T, bool KV8, bool LONG> static int launch_tile_t(h3_cuda *cud
     return 1;
 }
 
-// Clusters of `n` of these CTAs (one per SM) that the chip holds at once: 74, 45, 33, 26, 22, 15, 15 for 2 .. 8 of them
-// on 148 SMs, because a cluster lies within one group of SMs.
-static size_t clusters_of(const h3_cuda *cuda, size_t n) {
-    return n < 3 ? cuda->sm_count / n : n < 7 ? (size_t)cuda->sm_count * 89 / 100 / n : (size_t)cuda->sm_count / 10 + 1;
-}
 // CTAs for each of `items` items that all run at once, at least two key tiles each
 static int split_of(const h3_cuda *cuda, size_t items, size_t tiles) {
+    static AttnClusters clusters;              // one CTA to an SM, in this variant as in the others
     size_t n = std::min<size_t>(std::max<size_t>(tiles / 2, 1), 8);
-    while (n > 1 && clusters_of(cuda, n) < items) n--;
+    while (n > 1 && attn_clusters_of(cuda, clusters, (const void *)k_attn_tile<__half, true, false>, TileCfg<true>::THREADS, wtile::smem_bytes<true>(), n) < items) n--;
     return (int)n;
 }
 

@@ -40,6 +40,32 @@ static int fill(WinArgs &a, h3_cuda *cuda, const char *who, int dtype, const voi
     return 1;
 }
 
+size_t attn_clusters_of(const h3_cuda *cuda, AttnClusters &c, const void *kernel, int threads, size_t smem, size_t n) {
+    const bool keep = cuda->device < 64;
+    if (keep) {
+        const int known = c.kept[cuda->device][n - 1].load(std::memory_order_relaxed);
+        if (known > 0) return (size_t)known;
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)n; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)n);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int count = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        count = 0;                                          // clusters of this size are not used then
+    }
+    if (keep && count > 0) c.kept[cuda->device][n - 1].store(count, std::memory_order_relaxed);
+    return (size_t)count;
+}
+
 template <bool KV8> static int launch(h3_cuda *cuda, const WinArgs &a, int f16, size_t len, char *error, size_t error_size) {
     DeviceGuard guard(cuda);
     ProfScope prof(cuda, PROF_ATTN);

@@ -204,6 +204,14 @@ struct OddValues {
     }
 };
 
+// Clusters of `n` (1 to 8) CTAs of a kernel that the chip holds at once.  A cluster lies within one group of SMs and the groups
+// of a chip are of different sizes, so this is less than CTAs / n: on one card with 148 SMs, for 1 .. 8, 148, 74, 45, 33, 26, 22, 15,
+// 15 with one CTA to an SM, 444, 222, 142, 104, 82, 71, 56, 48 with three.  Asked once for a device (`kept`: of the kernel).
+struct AttnClusters {
+    std::atomic<int> kept[64][8];
+};
+size_t attn_clusters_of(const h3_cuda *cuda, AttnClusters &c, const void *kernel, int threads, size_t smem, size_t n);
+
 // Keys that the rows of one CTA can see at most (an estimate that guides how the keys are split).
 static inline size_t attn_window_keys(const h3b_win &w, size_t len, size_t rows) {
     const size_t reach = (size_t)w.left + (size_t)w.right + (size_t)w.block + rows + (size_t)w.sinks;

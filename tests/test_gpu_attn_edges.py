@@ -1,6 +1,8 @@
 """Windowed attention and the 8-bit cache at the edges of their contracts: pages that no row needs, values that are not
 finite, probabilities far below the largest, scales of zero, orders of the cache's operands.  Definitions in 64 bits and
 tolerances as in test_gpu_attn_window.py unless a test derives its own."""
+import math
+
 import numpy as np
 import pytest
 
@@ -235,3 +237,49 @@ def test_append_behind_tokens_under_a_scale_of_zero(cuda):
         cuda.kv8_append(cache, x, x, i32([0, 10]), i32([start]), i32([[0]]), max_rows=10)
         model.append(x, x, [0, 10], [start], [[0]])
         model.same_as(cache)
+
+
+# ------------------------------------------------------------------ how keys are split over clusters
+
+def test_streams_that_just_miss_a_cluster_size_do_not_take_a_second_wave(cuda):
+    """One token for `n` streams of 20,000 tokens and one K/V head: a count for which the next larger clusters would not all fit
+    the chip at once takes no longer than some more streams in the smaller ones (a second wave: 1.3 to 1.5 times as long)."""
+    n_keys, page = 20000, 256
+    per, streams = -(-n_keys // page), 54
+    cache = cuda.kv8_cache(streams * per, page, 1)
+    cache.k.view(torch.uint8).random_(0, 120)
+    cache.v.view(torch.uint8).random_(0, 120)
+    cache.k_scale.fill_(2.0 ** -8)
+    cache.v_scale.fill_(2.0 ** -8)
+    table = torch.arange(streams * per, dtype=torch.int32, device="cuda").view(streams, per)
+    q = normal(gen(1), streams, 7, 128, dtype=BF)
+    side = torch.cuda.Stream()
+
+    def took(n):
+        args = q[:n], torch.arange(n + 1, dtype=torch.int32, device="cuda"), i32([n_keys] * n), table[:n]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            cuda.use_stream(side)
+            try:
+                step = lambda: cuda.kv8_sdpa(cache, *args, max_rows=1, max_len=n_keys)  # noqa: E731
+                step()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=side):
+                    for _ in range(20):
+                        step()
+                best = math.inf
+                for _ in range(10):
+                    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                    a.record(side)
+                    graph.replay()
+                    b.record(side)
+                    side.synchronize()
+                    best = min(best, a.elapsed_time(b))
+                return best
+            finally:
+                side.synchronize()
+                cuda.use_stream(torch.cuda.default_stream())
+
+    times = {n: took(n) for n in (16, 18, 19, 52, 54)}
+    cuda.check()
+    assert times[16] < 1.15 * times[19] and times[18] < 1.15 * times[19] and times[52] < 1.15 * times[54], times
