@@ -1,7 +1,7 @@
 // Windowed attention for few query rows per K/V head (one token of a stream, a handful of drafted ones, shared heads):
 // the time is that of reading the keys and values once, so the whole chip has to read, and nothing else may wait.
 //
-// One warp works on up to 8 NT rows (query rows x heads of one K/V head; rows beyond them are zero) with m16n8k16
+// A warp works on all rows, up to 8 NT (query rows x heads of one K/V head; rows beyond them are zero), with m16n8k16
 // tensor-core products whose 16 rows are KEYS, respectively dimensions: S^T = K Q^T and O^T += V^T P^T, so that nothing is
 // padded from 1 to 16 rows (8 is the least) and the widened keys and values are the operands that are used once.  Q stays
 // in registers, P goes from score fragments to operand fragments through one 8x8 transposition per 8 keys.  The running
@@ -113,7 +113,6 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
     using E = typename std::conditional<KV8, __half, T>::type;                     // operand type
     constexpr int U = C::U, WARPS = C::WARPS, STAGE = C::STAGE, HALF = C::HALF;
     constexpr int MT = U / 16;                                                     // score tiles of 16 keys
-    constexpr int ROWS = 8 * NT;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float *acc = reinterpret_cast<float *>(smem + WARPS * STAGE);                  // [16][128] of this CTA
@@ -125,13 +124,11 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
 
     const WinArgs &a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rank = (int)blockIdx.x % p.split, mt = (int)blockIdx.x / p.split, kvh = blockIdx.y, s = blockIdx.z;
+    const int rank = (int)blockIdx.x, kvh = blockIdx.y, s = blockIdx.z;
     const SeqExt e = seq_ext<KV8>(a, s);
-    const int r_first = mt * ROWS, r_end = min(r_first + ROWS, e.nq * a.group);    // rows = query * group + head of the group
-    if (r_first >= r_end) return false;                                            // the whole cluster alike
-    const int R = r_end - r_first;
-    const int qi_first = r_first / a.group, qi_last = (r_end - 1) / a.group;
-    const int p0 = e.pos0 + qi_first, p1 = e.pos0 + qi_last;
+    const int R = e.nq * a.group;                                                  // rows = query * group + head of the group
+    if (!R) return false;                                                          // the whole cluster alike
+    const int p0 = e.pos0, p1 = e.pos0 + e.nq - 1;
     const h3b_win_tiles tiles = h3b_win_tiles_of(a.win, p0, p1, e.n, U);
     const h3b_win_row row_a = h3b_win_of(a.win, p0, e.n), row_z = h3b_win_of(a.win, p1, e.n);
     const int share = (tiles.count + p.split - 1) / p.split;
@@ -233,9 +230,9 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
     float row_scale[NT][2];                        // rows 2t, 2t + 1: scale * log2(e), and what brings Q to f16
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int r = r_first + nt * 8 + g;
-        const bool live = r < r_end;
-        const int qi = live ? r / a.group : qi_first, hd = live ? r - qi * a.group : 0;
+        const int r = nt * 8 + g;
+        const bool live = r < R;
+        const int qi = live ? r / a.group : 0, hd = live ? r - qi * a.group : 0;
         const T *src = reinterpret_cast<const T *>(a.q) + (long long)(e.row0 + qi) * a.q_rs + (long long)(kvh * a.group + hd) * a.q_hs;
         float rs = a.scale_log2;
         if (KV8) {
@@ -350,7 +347,7 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 if (masked) {
-                    const h3b_win_row wr = h3b_win_of(a.win, e.pos0 + min(r_first + nt * 8 + 2 * t + j, r_end - 1) / a.group, e.n);
+                    const h3b_win_row wr = h3b_win_of(a.win, e.pos0 + min(nt * 8 + 2 * t + j, R - 1) / a.group, e.n);
 #pragma unroll
                     for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -508,7 +505,7 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
         }
     if (AGAIN) {
         // rows that see values which were taken out get them back
-        const h3b_win_row wr = h3b_win_of(a.win, e.pos0 + min(r_first + (lane & 15), r_end - 1) / a.group, e.n);
+        const h3b_win_row wr = h3b_win_of(a.win, e.pos0 + min(lane & 15, R - 1) / a.group, e.n);
         OddValues x;
         x.clear();
         for (int it = 0; it < n_it; it++) {
@@ -547,7 +544,7 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
     const int d = threadIdx.x;                                                   // threads 0..127: one dimension each
     bool odd = false;                                                            // not finite, with a finite sum of probabilities
     for (int r = rank; r < R; r += p.split) {
-        const int qi = (r_first + r) / a.group, hd = (r_first + r) - qi * a.group;
+        const int qi = r / a.group, hd = r - qi * a.group;
         if (d < 128) {
             float mc[8], lc[8], vc[8], m = -INFINITY, l = 0.0f, v = 0.0f;            // at most 8 CTAs, all loads under way at once
 #pragma unroll
@@ -661,11 +658,10 @@ int launch_attn_few(h3_cuda *cuda, const WinArgs &a, int f16, bool kv8, size_t l
     }
     const size_t rows = (size_t)a.max_rows * a.group;
     const int nt = rows <= 8 ? 1 : 2;
-    const size_t mtiles = ceil_div(rows, 8 * (size_t)nt);
     const size_t keys = attn_window_keys(a.win, len, (size_t)a.max_rows);
-    const FewPlan plan = few_plan(cuda, mtiles * a.kv_heads * a.n_seq, ceil_div(keys, kv8 ? few::Cfg<true, false>::U : few::Cfg<false, false>::U));
+    const FewPlan plan = few_plan(cuda, (size_t)a.kv_heads * a.n_seq, ceil_div(keys, kv8 ? few::Cfg<true, false>::U : few::Cfg<false, false>::U));
     p.split = plan.split;
-    const dim3 grid((unsigned)(mtiles * p.split), (unsigned)a.kv_heads, (unsigned)a.n_seq);
+    const dim3 grid((unsigned)p.split, (unsigned)a.kv_heads, (unsigned)a.n_seq);
     int (*launch)(h3_cuda *, const FewParams &, dim3, int, char *, size_t);
     if (kv8) launch = f16 ? (plan.wide ? launch_few_t<__half, true, true> : launch_few_t<__half, true, false>)
                           : (plan.wide ? launch_few_t<__nv_bfloat16, true, true> : launch_few_t<__nv_bfloat16, true, false>);

@@ -34,7 +34,7 @@ static int fill(WinArgs &a, h3_cuda *cuda, const char *who, int dtype, const voi
     a.q = q; a.out = out;
     a.q_rs = (long long)q_rs; a.q_hs = (long long)q_hs; a.o_rs = (long long)o_rs; a.o_hs = (long long)o_hs;
     a.rows = (int)rows; a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.group = (int)(heads / kv_heads);
-    a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale * 1.4426950408889634f;
     a.win.left = clip(left); a.win.right = clip(right); a.win.sinks = clip(sinks); a.win.block = clip(block);
     a.status = cuda->d_status;
     return 1;

@@ -19,8 +19,7 @@ struct WinArgs {
     void *out;
     long long q_rs, q_hs, o_rs, o_hs;        // elements between rows / heads
     int rows, heads, kv_heads, group;        // rows of q and out; group = heads / kv_heads
-    float scale;                             // of the scores
-    float scale_log2;                        // scale * log2(e)
+    float scale_log2;                        // scale of the scores * log2(e)
     h3b_win win;
     int *status;
     // 16-bit K/V
