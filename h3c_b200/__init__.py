@@ -445,6 +445,9 @@ class Cuda:
         with torch.cuda.stream(self.stream):
             k, v = (made(pages, kv_heads, page_tokens, 128, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
             ks, vs = (made(pages, kv_heads, page_tokens // 64, dtype=torch.float32) for _ in range(2))
+        if not self._on_current_stream():   # the caller may read or write it on the current stream
+            for t in (k, v, ks, vs):
+                t.record_stream(torch.cuda.current_stream(self.device))
         return KvCache8(k, v, ks, vs)
 
     def _batch(self, who, cache, cu_rows, ext, table):

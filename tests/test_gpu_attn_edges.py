@@ -283,3 +283,35 @@ def test_streams_that_just_miss_a_cluster_size_do_not_take_a_second_wave(cuda):
     times = {n: took(n) for n in (16, 18, 19, 52, 54)}
     cuda.check()
     assert times[16] < 1.15 * times[19] and times[18] < 1.15 * times[19] and times[52] < 1.15 * times[54], times
+
+
+# ------------------------------------------------------------------ memory of a cache
+
+def test_memory_of_a_new_cache_waits_for_the_current_stream(cuda):
+    """A cache made while the handle works on another stream than the current one: its memory comes from the handle's
+    stream and is not given out again there while the caller's own work on the current stream still reads it."""
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        cuda.use_stream(side)
+        cache = cuda.kv8_cache(301, 64, 3)
+        side.synchronize()
+        before = {t.data_ptr() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)}
+        total = lambda: sum(t.float().sum() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale))  # noqa: E731
+        total()                                                              # (its kernels are loaded)
+        torch.cuda.synchronize()
+        torch.cuda._sleep(400_000_000)                                       # some 0.2 s on the current stream, then
+        read, done = total(), torch.cuda.Event()
+        done.record()
+        del cache
+        again = cuda.kv8_cache(301, 64, 3)
+        now = {t.data_ptr() for t in (again.k, again.v, again.k_scale, again.v_scale)}
+        assert not done.query()                                              # the caller's work is still under way
+        assert not before & now
+        with torch.cuda.stream(side):
+            for t in (again.k.view(torch.uint8), again.v.view(torch.uint8), again.k_scale, again.v_scale):
+                t.fill_(1)
+        assert float(read) == 0
+    finally:
+        torch.cuda.synchronize()
+        cuda.use_stream(torch.cuda.current_stream())
