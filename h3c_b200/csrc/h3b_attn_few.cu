@@ -138,7 +138,7 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
 
     uint8_t *stage = smem + warp * STAGE;
     uint64_t *bar = bars + warp * 2;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && tiles.count) {         // (without keys there are no maps)
         tma_prefetch_desc(&p.map_k);
         tma_prefetch_desc(&p.map_v);
     }

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
     const uint32_t tmem_base = ctl.tmem_base;
 
     if (threadIdx.x == 32) tma_prefetch_desc(&p.map_q);
-    if (!KV8 && threadIdx.x == 0) {
+    if (!KV8 && threadIdx.x == 0 && a.lk) {                              // (without keys there are no maps)
         tma_prefetch_desc(&p.map_k);
         tma_prefetch_desc(&p.map_v);
     }
