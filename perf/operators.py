@@ -204,10 +204,15 @@ _kept = {}
 
 
 def _cuda():
-    if "cuda" not in _kept:
+    """The current device's handle, on the current stream (whose number is cheap to look up)."""
+    device = torch.cuda.current_device()
+    raw, kept = torch._C._cuda_getCurrentRawStream(device), _kept.get(device)
+    if kept is None or kept[0] != raw:
         import h3c_b200
-        _kept["cuda"], _kept["cache"] = h3c_b200.Cuda(torch.cuda.current_device()), h3c_b200.KvCache8
-    return _kept["cuda"], _kept["cache"]
+        cuda = kept[1] if kept else h3c_b200.Cuda(device)
+        cuda.use_stream(torch.cuda.current_stream())
+        kept = _kept[device] = raw, cuda, h3c_b200.KvCache8
+    return kept[1:]
 
 
 def run(s):
