@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_attn_window import BF, HF, Model, check_cache, cuda, filled, gen, i32, mask, normal  # noqa: E402, F401
+from tests.test_gpu_attn_window import BF, HF, Model, check_cache, cuda, filled, gen, i32, mask, normal, pages_of  # noqa: E402, F401
 
 
 # ------------------------------------------------------------------ pages that no row needs
@@ -315,3 +315,63 @@ def test_memory_of_a_new_cache_waits_for_the_current_stream(cuda):
     finally:
         torch.cuda.synchronize()
         cuda.use_stream(torch.cuda.current_stream())
+
+
+# ------------------------------------------------------------------ orders of the cache's operands
+
+def orders(g, rows, heads, dtype):
+    """Views of a [rows, heads, 128] tensor in other orders, with the same values in each."""
+    x = normal(g, rows, heads, 128, dtype=dtype)
+    fused = normal(g, rows, heads + 5, 128, dtype=dtype)                    # part of one projection's rows
+    fused[:, 3:3 + heads] = x
+    heads_first = x.transpose(0, 1).contiguous().transpose(0, 1)
+    wide = torch.full((rows, heads, 136), 9.0, dtype=dtype, device="cuda")
+    wide[..., 8:] = x
+    every = torch.full((2 * rows, heads, 128), 9.0, dtype=dtype, device="cuda")
+    every[::2] = x
+    return x, {"fused": fused[:, 3:3 + heads], "heads first": heads_first, "wide": wide[..., 8:], "every second row": every[::2]}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("codes", [torch.float8_e4m3fn, torch.uint8])
+def test_append_of_rows_in_other_orders(cuda, dtype, codes):
+    import h3c_b200
+    rng, g = np.random.default_rng(1), gen(1)
+    rows, start, page, kv = [70, 1, 130], [30, 64, 200], 128, 3
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    table = pages_of(rng, [a + b for a, b in zip(rows, start)], page, 9)
+    (k, ks), (v, vs) = orders(g, int(cu[-1]), kv, dtype), orders(g, int(cu[-1]), kv, dtype)
+    pairs = [(k, v)] + [(ks[a], vs[b]) for a, b in zip(ks, reversed(vs))] + [(ks["fused"], v), (k, vs["wide"])]
+    want = None
+    for kk, vv in pairs:
+        made = cuda.kv8_cache(9, page, kv)
+        cache = h3c_b200.KvCache8(made.k.view(codes), made.v.view(codes), made.k_scale, made.v_scale)
+        if want is None:
+            want = Model(cache)
+            want.append(k, v, cu, start, table)
+        cuda.kv8_append(cache, kk, vv, i32(cu), i32(start), i32(table), max_rows=max(rows))
+        cuda.check()
+        want.same_as(cache)
+
+
+@pytest.mark.parametrize("rows, lens, heads, kv", [([1, 3], [300, 70], 6, 2), ([40, 150], [400, 150], 6, 2), ([30, 9], [300, 90], 7, 1), ([33], [333], 4, 4)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_cache_attention_of_queries_and_outputs_in_other_orders(cuda, rows, lens, heads, kv, dtype):
+    import h3c_b200
+    rng, g = np.random.default_rng(2), gen(2)
+    cache, table, model = filled(cuda, rng, g, lens, 64, kv, dtype, spread=False)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    n, w = int(cu[-1]), dict(left=50, sinks=2)
+    q, others = orders(g, n, heads, dtype)
+    want = check_cache(cuda, cache, table, model, q, cu, lens, **w)
+    args = dict(max_rows=max(rows), max_len=max(lens), **w)
+    codes = h3c_b200.KvCache8(cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)
+    for c, qq in [(cache, x) for x in others.values()] + [(codes, q)]:
+        assert torch.equal(cuda.kv8_sdpa(c, qq, i32(cu), i32(lens), i32(table), **args), want)
+    for first, width in ((0, heads * 128 + 64), (8, heads * 128 + 24), (16, heads * 128 + 16)):   # 16- and 32-byte stores
+        room = torch.full((n + 3, width), 3.0, dtype=dtype, device="cuda")
+        out = room[1:n + 1, first:first + heads * 128]
+        got = cuda.kv8_sdpa(cache, q, i32(cu), i32(lens), i32(table), out=out, **args)
+        assert got.data_ptr() == out.data_ptr() and torch.equal(out, want)
+        room[1:n + 1, first:first + heads * 128] = 3.0
+        assert (room == 3).all()
