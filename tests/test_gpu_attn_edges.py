@@ -375,3 +375,77 @@ def test_cache_attention_of_queries_and_outputs_in_other_orders(cuda, rows, lens
         assert got.data_ptr() == out.data_ptr() and torch.equal(out, want)
         room[1:n + 1, first:first + heads * 128] = 3.0
         assert (room == 3).all()
+
+
+# ------------------------------------------------------------------ values that are not finite, in the calls of a program
+
+@pytest.mark.parametrize("where", ["one", "first", "some"])
+@pytest.mark.parametrize("lq, w", [(3, dict(left=60, right=0, sinks=6, q_pos=198)), (150, dict(left=90, right=4, sinks=6, q_pos=100)),
+                                   (60, dict(left=3, right=0, q_pos=350)), (9, dict(left=3, right=0, sinks=1, q_pos=395))])   # rows behind the keys
+def test_values_that_are_not_finite_in_views_and_outputs_of_other_orders(cuda, lq, w, where):
+    g = gen(lq)
+    fused = normal(g, 400, 6 + 2 + 2, 128, dtype=BF)
+    q, k = fused[:lq, :6], fused[:, 6:8]
+    fused[:, 8:] = place(fused[:, 8:], where, g)
+    v = fused[:, 8:]
+    check_odd_values(cuda, q, k, torch.where(torch.isfinite(v), v, 1.0), where, g, **w)
+    want = cuda.sdpa_window(q.contiguous(), k.contiguous(), v.contiguous(), **w)
+    room = torch.full((lq, 6 * 128 + 24), 3.0, dtype=BF, device="cuda")
+    out = cuda.sdpa_window(q, k, v, out=room[:, 8:8 + 768], **w)
+    assert torch.equal(out.float().nan_to_num(nan=12345.0), want.float().nan_to_num(nan=12345.0))
+    assert (room[:, :8] == 3).all() and (room[:, 776:] == 3).all()
+
+
+@pytest.mark.parametrize("lq, lk", [(2, 3000), (300, 700), (40, 9000)])
+def test_a_captured_call_follows_values_that_are_not_finite(cuda, lq, lk):
+    """Whether there is a second pass is decided on the device: a graph captured over ordinary values, replayed over others."""
+    g = gen(lq)
+    q, k, v = normal(g, lq, 4, 128, dtype=BF), normal(g, lk, 2, 128, dtype=BF), normal(g, lk, 2, 128, dtype=BF)
+    fine, w = v.clone(), dict(left=-1, right=0, q_pos=lk - lq)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    try:
+        with torch.cuda.stream(side):
+            cuda.use_stream(side)
+            cuda.sdpa_window(q, k, v, **w)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = cuda.sdpa_window(q, k, v, **w)
+            for where in ("none", "last", "some", "none", "all", "none"):
+                v.copy_(place(fine, where, g))
+                graph.replay()
+                got = out.clone()
+                want = cuda.sdpa_window(q, k, v, **w)
+                assert torch.equal(got.float().nan_to_num(nan=12345.0), want.float().nan_to_num(nan=12345.0))
+                assert bool(torch.isfinite(got).all()) == (where == "none")
+            side.synchronize()
+    finally:
+        torch.cuda.synchronize()
+        cuda.use_stream(torch.cuda.current_stream())
+    cuda.check()
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+def test_outputs_by_head_through_the_c_entry_points(cuda, rows):
+    """[heads, rows, 128] outputs, which the Python entry points do not offer."""
+    import h3c_b200
+    from h3c_b200 import lib as l
+    rng, g = np.random.default_rng(5), gen(5)
+    cache, table, model = filled(cuda, rng, g, [300], 64, 2, BF, spread=False)
+    q, cu, lens, pages = normal(g, rows, 4, 128, dtype=BF), i32([0, rows]), i32([300]), i32(table)
+    want = check_cache(cuda, cache, table, model, q, [0, rows], [300], left=40)
+    out = torch.full((4, rows + 1, 128), 3.0, dtype=BF, device="cuda")
+    h3c_b200.call("h3b_kv8_sdpa_dev", cuda.h, cache.packed, l.KV8_SDPA_ARGS.pack(
+        q.data_ptr(), out.data_ptr(), cu.data_ptr(), lens.data_ptr(), pages.data_ptr(), 512, 128, 128, (rows + 1) * 128, rows, 4, table.shape[1], 1,
+        rows, 300, 40, 0, 0, 1, 128 ** -0.5, l.BF16))
+    cuda.check()
+    assert torch.equal(out[:, :rows].transpose(0, 1).reshape(rows, -1), want) and (out[:, rows] == 3).all()
+    k, v = normal(g, 200, 2, 128, dtype=BF), normal(g, 200, 2, 128, dtype=BF)
+    v[150, 0, 3] = float("inf")                                              # seen by some rows: a second pass writes there too
+    want = cuda.sdpa_window(q, k, v, left=40, right=0, q_pos=149)
+    h3c_b200.call("h3b_sdpa_window_dev", cuda.h, l.SDPA_WINDOW_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 512, 128, 256, 128, 256, 128, 128, (rows + 1) * 128, rows, 200, 4, 2, 128, 149, 40, 0,
+        0, 1, 128 ** -0.5, l.BF16))
+    cuda.check()
+    assert torch.equal(out[:, :rows].transpose(0, 1).reshape(rows, -1).float().nan_to_num(nan=9.5), want.float().nan_to_num(nan=9.5))
+    assert not torch.isfinite(want).all() and (out[:, rows] == 3).all()
