@@ -69,10 +69,16 @@ size_t attn_clusters_of(const h3_cuda *cuda, AttnClusters &c, const void *kernel
 template <bool KV8> static int launch(h3_cuda *cuda, const WinArgs &a, int f16, size_t len, char *error, size_t error_size) {
     DeviceGuard guard(cuda);
     ProfScope prof(cuda, PROF_ATTN);
-    // 16 rows are one pass of the few-row kernel over the keys.  Measured (us, few-row | tile kernel): 16 rows of 32 streams of
-    // 4,000 cached tokens and 8 heads 78 | 137, 24 rows 158 | 137; 16 rows over 30,000 tokens and 24 heads 66 | 102, 24 rows
-    // 84 | 101, 48 rows 124 | 101; 16-bit 64 | 84, 83 | 84, 97 | 84.
-    if ((size_t)a.max_rows * a.group <= 16) return launch_attn_few(cuda, a, f16, KV8, len, error, error_size);
+    // 16 rows are one pass of the few-row kernel over the keys.  Measured (us, few-row | tile kernel), cache: 16 rows of 32 streams
+    // of 4,000 tokens and 8 heads 78 | 137, 24 rows 158 | 137; 16 rows over 30,000 tokens and 24 heads 66 | 102, 24 rows 84 | 101,
+    // 48 rows 124 | 101; 16-bit 64 | 84, 83 | 84, 97 | 84.
+    // Over some hundreds of keys the meeting of the rows and the tile kernel's start decide.  16-bit, 24 heads, 16 rows over 64,
+    // 128, 256, 384, 512 keys: 13.3 | 7.9, 13.7 | 7.9, 11.1 | 9.4, 10.5 | 10.9, 9.7 | 11.2; 9 rows 9.9 | 8.0, 10.0 | 7.9, 8.9 | 9.4,
+    // 8.1 | 11.0, 8.3 | 11.2; 8 rows 8.2 | 8.0, 8.5 | 8.0, 7.2 | 9.5, 6.9 | 11.0, 6.6 | 11.3.  Cache, 16 rows over 128 and 512
+    // tokens: 24 heads 16.2 | 13.3, 14.0 | 16.8; 32 streams of 8 heads 18.1 | 24.5, 23.8 | 34.7.
+    const size_t rows = (size_t)a.max_rows * a.group;
+    const bool brief = !KV8 && rows > 8 && attn_window_keys(a.win, len, (size_t)a.max_rows) <= 256;
+    if (rows <= 16 && !brief) return launch_attn_few(cuda, a, f16, KV8, len, error, error_size);
     return launch_attn_tile(cuda, a, f16, KV8, len, error, error_size);
 }
 

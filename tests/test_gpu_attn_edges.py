@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_attn_window import BF, HF, Model, check_cache, cuda, filled, gen, i32, mask, normal, pages_of  # noqa: E402, F401
+from tests.test_gpu_attn_window import BF, HF, Model, check_cache, check_window, cuda, filled, gen, i32, mask, normal, pages_of  # noqa: E402, F401
 
 
 # ------------------------------------------------------------------ pages that no row needs
@@ -449,3 +449,12 @@ def test_outputs_by_head_through_the_c_entry_points(cuda, rows):
     cuda.check()
     assert torch.equal(out[:, :rows].transpose(0, 1).reshape(rows, -1).float().nan_to_num(nan=9.5), want.float().nan_to_num(nan=9.5))
     assert not torch.isfinite(want).all() and (out[:, rows] == 3).all()
+
+
+@pytest.mark.parametrize("w", [dict(left=-1, right=0), dict(left=200, right=0, sinks=9), dict(left=-1, right=-1)], ids=str)
+@pytest.mark.parametrize("lq, heads, kv", [(8, 3, 3), (9, 3, 3), (16, 3, 3), (17, 3, 3), (2, 8, 2), (3, 8, 2), (4, 8, 2)])
+def test_window_on_both_sides_of_the_choice_of_kernels(cuda, lq, heads, kv, w):
+    for lk in (17, 64, 255, 256, 257, 600):
+        g = gen(lk)
+        q, k, v = normal(g, lq, heads, 128, dtype=HF), normal(g, lk, kv, 128, dtype=HF), normal(g, lk, kv, 128, dtype=HF)
+        check_window(cuda, q, k, v, q_pos=max(0, lk - lq), **w)
