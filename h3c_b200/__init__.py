@@ -118,7 +118,8 @@ class Cuda:
             self.h = None
 
     def check(self):
-        """Synchronises and raises if any kernel gave up a bounded wait."""
+        """Synchronises and raises if any kernel gave up a bounded wait, or if a sequence's rows, length or pages lay outside
+        the arrays of its call."""
         st = C.c_int(0)
         call("h3b_cuda_check", self.h, C.byref(st))
 

@@ -26,7 +26,8 @@
 //   padding and a warp alone issues one instruction in four cycles.
 //   five drafted tokens for 12 streams, 24 heads over 8 (15 rows), windows of 8,192: 46-47 us = 3.8 TB/s; twice the
 //   products and exponentials per key.  Bound by latency: no unit is half busy (DRAM 48 %, issue 33 %, tensor 27 %), and of
-//   7.6 cycles that a warp takes per instruction 2.1 are fixed latency, 1.3 loads and 1.0 barriers.
+//   7.6 cycles that a warp takes per instruction 2.1 are fixed latency, 1.3 loads and 1.0 barriers.  9 to 16 rows over the cache
+//   are the one variant that spills (168 registers, 88 bytes stored and 68 loaded).
 //   one stream of 24 heads: 8.2-8.4 us over 2,313 tokens, 6.8 over 640, 5.4 over 64, 3.6 over none: launch, look-ups one
 //   behind the other (extents, page, copy) and the meeting of warps and CTAs.  One token over 4,160 of 16,384 16-bit keys,
 //   24 heads: 12.6 us.

@@ -477,7 +477,7 @@ int h3b_sdpa_strided_dev(h3_cuda *cuda, int dtype, const void *d_q, size_t q_row
                          size_t o_row_stride, size_t o_head_stride, char *error, size_t error_size);
 /* Addition: attention with a sliding window and first keys that stay visible (sinks).  q [lq, heads, 128], k / v
  * [lk, kv_heads, 128], out [lq, heads, 128], all of `dtype` (H3B_BF16 or H3B_F16), row and head strides in elements
- * (multiples of 8, pointers 16-byte aligned); heads is a multiple of kv_heads (at most 128 times it), head h reads K/V
+ * (multiples of 8 and not 0, pointers 16-byte aligned); heads is a multiple of kv_heads (at most 128 times it), head h reads K/V
  * head h / (heads / kv_heads).  Row i of q stands at position p = q_pos + i among the keys and belongs to the block
  * (a frame of a video, 1 = each token alone) that starts at b = p - p % block; it sees key j when
  *     j <= b + block - 1 + right  and  (j >= b - left  or  j < sinks).
