@@ -30,7 +30,7 @@
 // Values that no row of the item sees are zeroed on their way (a probability of 0 times a NaN of stale memory is not 0).
 // 16-bit: an item with a row that comes out non-finite though its probabilities are finite is done a second time, as a further
 // item of its CTA, with the values that are not finite taken out of the tiles that its rows see in part (OddValues).  The
-// warp that hands out items learns of it two items later, or at the end, so that nothing waits for it in between.
+// warp that hands out items learns of it with the third item after, or at the end, so that nothing waits for it in between.
 //
 // Few items and many keys: the keys are split over the CTAs of a cluster (one item each), whose partial results meet in
 // shared memory.
@@ -609,6 +609,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                         if (second_time(it)) return true;
                     }
                     if (lane == 0) ctl.cta_of[k & 3] = x;
+                    __syncwarp();
                     it = next;
                     next.r0 = -1;
                     return true;
@@ -683,6 +684,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             auto rows_done = [&](bool odd) {
                 if (KV8) return;
                 odd = __any_sync(0xffffffffu, odd);
+                __syncwarp();                                            // what every lane has parked comes before the arrival
                 if (lane == 0) {
                     if (odd && !it.s) *reinterpret_cast<volatile int *>(&ctl.odd[k & 3]) = 1;
                     mbar_arrive(&ctl.rows_done[k & 3]);
