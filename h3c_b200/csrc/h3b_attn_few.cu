@@ -566,7 +566,7 @@ template <typename T, bool KV8, int NT, bool WIDE, bool AGAIN> __device__ __forc
                     l += lc[c] != lc[c] ? lc[c] : w * lc[c];
                     v += w * vc[c];
                 }
-            const float res = h3b_win_count(h3b_win_of(a.win, e.pos0 + qi, e.n)) ? v * (1.0f / l) : 0.0f;
+            const float res = h3b_win_count(h3b_win_of(a.win, e.pos0 + qi, e.n)) ? within_type<T, KV8>(v * (1.0f / l)) : 0.0f;
             T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qi) * a.o_rs + (long long)(kvh * a.group + hd) * a.o_hs;
             reinterpret_cast<unsigned short *>(dst)[d] = (unsigned short)(Elem<T>::pack(res, res) & 0xffffu);
             odd |= !(fabsf(res) < INFINITY) && ordinary(l);

@@ -924,7 +924,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
 #pragma unroll
                         for (int u = 0; u < 8; u++) {
                             const float x = __uint_as_float(o[i + 2 * u]) * inv_l, y = __uint_as_float(o[i + 2 * u + 1]) * inv_l;
-                            if (!KV8) odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+                            if (!KV8) odd |= !(fabsf(x) <= largest<T>()) || !(fabsf(y) <= largest<T>());
                             h[u] = seen ? Elem<T>::pack(x, y) : 0u;
                         }
                         if (live) {
@@ -934,6 +934,26 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
                                 *reinterpret_cast<uint4 *>(dst + ch * 32 + i) = make_uint4(h[0], h[1], h[2], h[3]);
                                 *reinterpret_cast<uint4 *>(dst + ch * 32 + i + 8) = make_uint4(h[4], h[5], h[6], h[7]);
                             }
+                        }
+                    }
+                }
+                if (!KV8 && Elem<T>::FMT == 0 && __any_sync(0xffffffffu, odd)) {
+                    // some row lies outside f16: what is finite goes back into it (in the loop above that cost 3 %)
+                    odd = false;
+#pragma unroll 1
+                    for (int ch = 0; ch < HD / 16; ch++) {
+                        uint32_t o[16], h[8];
+                        tmem_ld_32x32b_x16(o_addr + ch * 16, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int u = 0; u < 8; u++) {
+                            const float x = __uint_as_float(o[2 * u]) * inv_l, y = __uint_as_float(o[2 * u + 1]) * inv_l;
+                            odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+                            h[u] = seen ? Elem<T>::pack(within_type<T, KV8>(x), within_type<T, KV8>(y)) : 0u;
+                        }
+                        if (live) {
+                            *reinterpret_cast<uint4 *>(dst + ch * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4 *>(dst + ch * 16 + 8) = make_uint4(h[4], h[5], h[6], h[7]);
                         }
                     }
                 }
@@ -1034,7 +1054,7 @@ __global__ void __launch_bounds__(TileCfg<KV8>::THREADS, 1) k_attn_tile(const __
             v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
             T *dst = reinterpret_cast<T *>(a.out) + (long long)(e.row0 + qi) * a.o_rs + (long long)(kvh * a.group + hd) * a.o_hs;
             uint2 w = make_uint2(0u, 0u);
-            if (seen) w = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
+            if (seen) w = make_uint2(Elem<T>::pack(within_type<T, KV8>(v.x), within_type<T, KV8>(v.y)), Elem<T>::pack(within_type<T, KV8>(v.z), within_type<T, KV8>(v.w)));
             *reinterpret_cast<uint2 *>(dst + lane * 4) = w;
         }
         cluster_sync_all();                                              // nobody leaves while its memory is read

@@ -134,6 +134,15 @@ __device__ __forceinline__ void widen4_e4m3(uint32_t w, uint32_t &lo, uint32_t &
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 
+// largest finite number of a type that a mean of such values may be (bf16: whatever f32 holds)
+template <typename T> __device__ __forceinline__ constexpr float largest() { return Elem<T>::FMT == 1 ? 3.402823466e38f : 65504.0f; }
+// A weighted mean of f16 values lies between them; half a step of P may put it above 65504, which must not become infinity.
+// (Over the cache a code times its scale may lie above it by itself.)
+template <typename T, bool KV8> __device__ __forceinline__ float within_type(float x) {
+    if (KV8 || Elem<T>::FMT == 1 || !(fabsf(x) < INFINITY)) return x;
+    return fminf(fmaxf(x, -largest<T>()), largest<T>());
+}
+
 // ---- Values that are not finite, at keys that not every row of a group sees.  A probability of 0 times such a value is not 0, so
 // the matrix product hands it to rows that do not see it.  Looking for them in every tile costs time, so the kernels look at
 // the results: where a row with a finite sum of probabilities comes out non-finite and the rows of its group differ in what

@@ -536,6 +536,7 @@ int h3b_kv8_append_dev(h3_cuda *cuda, const h3b_kv8_cache *cache, const h3b_kv8_
  * them (row i of nq at position d_len[s] - nq + i); windows as in h3b_sdpa_window_dev.  Rows of out that belong to no
  * sequence are left as they are.  max_len (a bound on d_len[], or an estimate) only guides how the work is split, and so
  * the order of the sums.
+ * A cached value may lie 2^-4 of itself above the appended one; an f16 result above 65504 is infinite.
  * Accuracy beside half a step of the f16 probabilities and of the result, for very many tokens:
  * - a token loses at most 2^-34 of the largest probability times value scale of its row: together 6e-5 of the largest value
  *   at a million tokens (scales of a row's values more than 2^70 apart: the quieter tokens may drop out of its softmax);

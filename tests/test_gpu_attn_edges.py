@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_attn_window import BF, HF, Model, check_cache, check_window, cuda, filled, gen, i32, mask, normal, pages_of  # noqa: E402, F401
+from tests.test_gpu_attn_window import BF, HF, Model, check_cache, check_window, close, cuda, filled, gen, i32, mask, normal, pages_of  # noqa: E402, F401
 
 
 # ------------------------------------------------------------------ pages that no row needs
@@ -458,3 +458,25 @@ def test_window_on_both_sides_of_the_choice_of_kernels(cuda, lq, heads, kv, w):
         g = gen(lk)
         q, k, v = normal(g, lq, heads, 128, dtype=HF), normal(g, lk, kv, 128, dtype=HF), normal(g, lk, kv, 128, dtype=HF)
         check_window(cuda, q, k, v, q_pos=max(0, lk - lq), **w)
+
+
+@pytest.mark.parametrize("lq, lk, w", [(1, 700, dict()), (9, 700, dict(left=300, right=0, q_pos=600)), (300, 700, dict(left=300, right=0, q_pos=400)),
+                                       (40, 9000, dict(left=-1, right=0, q_pos=8960))])   # keys split over a cluster
+def test_means_of_the_largest_f16_values_stay_finite(cuda, lq, lk, w):
+    """Values clamped to the type's range, as programs in f16 do: a mean of 65504 is 65504, not infinity.  One key in 37 has the
+    largest score, the others one whose probability next to it, 1/2 + 2^-12 + 2^-15, is rounded up by 2^-12 - 2^-15: the mean
+    comes out high by 2^-11.3 of itself, and from 2^-12 on it is rounded to infinity."""
+    g = gen(lq)
+    q, k = torch.zeros(lq, 4, 128, dtype=HF, device="cuda"), torch.zeros(lk, 2, 128, dtype=HF, device="cuda")
+    q[..., 7] = 1
+    k[::37, :, 7] = 1
+    v = torch.full((lk, 2, 128), 65504.0, dtype=HF, device="cuda")
+    v[:, 1] = -65504.0
+    w = w | dict(scale=-math.log(0.5 + 2.0 ** -12 + 2.0 ** -15))
+    got = cuda.sdpa_window(q, k, v, **w)
+    want = torch.where(torch.arange(512, device="cuda") < 256, 65504.0, -65504.0).double().expand(lq, -1)
+    close(got, want, want.abs(), 65504.0, HF)
+    v[lk - 1, 0, 3] = float("inf")                                           # a value that is infinite stays so
+    got = cuda.sdpa_window(q, k, v, **w).view(lq, 4, 128)
+    sees = mask(np.arange(lq) + w.get("q_pos", 0), lk, w.get("left", -1), w.get("right", -1), 0, 1)[:, lk - 1]
+    assert (got[sees][:, :2, 3] == float("inf")).all() and torch.isfinite(got[~sees]).all() and int(torch.isinf(got).sum()) == 2 * int(sees.sum())
