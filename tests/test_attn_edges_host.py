@@ -1,5 +1,4 @@
-"""Host-side checks of the windowed operators' edge cases: the shared window arithmetic compiled as plain C, and the Python
-entry points where they need no GPU."""
+"""Host-side checks of the windowed operators' edge cases: the shared window arithmetic compiled as plain C."""
 import subprocess
 from pathlib import Path
 

@@ -142,7 +142,7 @@ def test_a_value_that_is_not_finite_costs_a_second_pass_and_no_more(cuda, w):
         odd = place(v, where, g)
         took = min(timed(lambda: cuda.sdpa_window(q, k, odd, **w)) for _ in range(5))
         print(f"{where}: {took:.3f} ms, {base:.3f} without")
-        assert took < 8 * base
+        assert took < 16 * base                                              # (up to 6 measured)
     cuda.check()
 
 
